@@ -382,6 +382,87 @@ bool q4mi_expert_reduce_x(float *d_y, const float *d_pd, const int32_t *d_rsrc,
                           const float *d_rw, uint32_t n_tok, uint32_t topk, uint32_t n_embd,
                           uint64_t x_row0, const float *d_xw);
 
+/* ------------------------------------- microscaled 4-bit rows (MXFP4, type 39)
+ *
+ * A row of `cols` values is nb = ceil(cols/32) blocks of 32.  Codes: 16*nb
+ * bytes a row, value i in byte i/2 (the even one in the low nibble): sign, two
+ * exponent bits, one mantissa bit (0, 0.5, 1, 1.5, 2, 3, 4, 6), 0 past cols.
+ * Scales: one byte s a block for 2^(s - 127), 255 for NaN; a row's scales take
+ * nb bytes rounded up to a whole dword.  Rows follow each other without gaps.
+ * Codes are 16-byte and scales 4-byte aligned.  Float rows are F32 (type 0),
+ * F16 (1) or BF16 (30), aligned to their type, `ld` elements apart.  Launches
+ * keep no state and no scratch, so calls on different streams (through
+ * q4mi_set_stream) and captured graphs are independent of each other.  The
+ * reference has no such format. */
+uint64_t q4mi_mx4_code_bytes(uint64_t rows, uint64_t cols);
+uint64_t q4mi_mx4_scale_bytes(uint64_t rows, uint64_t cols);
+/* rows (row r = x[ids ? ids[r] : r]) to codes and scales: a block's scale is
+ * 2^(floor(log2(largest magnitude)) - 2), at least 2^-127, its codes the
+ * nearest (ties to the even code), at most 6.  A block that holds an infinity
+ * or a NaN becomes all NaN.  ids are not checked. */
+bool q4mi_mx4_quant(const void *d_x, uint32_t x_type, uint64_t ld_x, const int32_t *d_ids,
+                    uint64_t rows, uint64_t cols, uint8_t *d_codes, uint8_t *d_scales);
+/* Row r = the values of row ids ? ids[r] : r, rounded once to y_type; columns
+ * past cols of y are left as they were. */
+bool q4mi_mx4_dequant(const uint8_t *d_codes, const uint8_t *d_scales, const int32_t *d_ids,
+                      uint64_t rows, uint64_t cols, void *d_y, uint32_t y_type, uint64_t ld_y);
+/* y[t][r] = W_r . x_t for t < n, r < w_rows, both sides in 4 bits, sums in
+ * fp32, rounded once to y_type.  x_type 39: x and xs are codes and scales
+ * (ld_x unused).  x_type 0 / 1 / 30: float rows, at most 8, quantised as by
+ * q4mi_mx4_quant on the way in (the same bits in y), xs NULL.  Blocks are
+ * taken whole: codes past cols must be 0 in W or in x, as the quantiser
+ * leaves them. */
+bool q4mi_mx4_mul(const uint8_t *d_w, const uint8_t *d_ws, uint64_t w_rows, uint64_t cols,
+                  const void *d_x, const uint8_t *d_xs, uint32_t x_type, uint64_t ld_x, uint64_t n,
+                  void *d_y, uint32_t y_type, uint64_t ld_y);
+/* Routed experts of a decode step: row p < n (n <= 65535) is expert eid[p]
+ * (codes at w + e*w_stride, scales at ws + e*ws_stride) times x row p / x_div
+ * (x_div = topk: the token's hidden state; 1: a row each).  x as for
+ * q4mi_mx4_mul, any number of float rows.  A row whose eid is outside
+ * 0..n_expert-1 is left as it was.  eid is what q4mi_moe_route and
+ * q4_hip_route_pf write (ostride topk). */
+bool q4mi_mx4_mul_sel(const uint8_t *d_w, const uint8_t *d_ws, uint64_t w_rows, uint64_t cols,
+                      uint64_t w_stride, uint64_t ws_stride, uint32_t n_expert, const void *d_x,
+                      const uint8_t *d_xs, uint32_t x_type, uint64_t ld_x, uint32_t x_div,
+                      const int32_t *d_eid, uint64_t n, void *d_y, uint32_t y_type,
+                      uint64_t ld_y);
+/* Routed experts of a prompt: packed rows bounds[e] .. bounds[e+1] go through
+ * expert e, packed row p reading x row act_row ? act_row[p] : p (of xrows);
+ * bounds and act_row as q4mi_assign writes them.  Rows outside every stretch,
+ * past total_rows or with act_row outside 0..xrows-1 are left as they were. */
+bool q4mi_mx4_mul_id(const uint8_t *d_w, const uint8_t *d_ws, uint64_t w_rows, uint64_t cols,
+                     uint64_t w_stride, uint64_t ws_stride, uint32_t n_expert, const uint8_t *d_xq,
+                     const uint8_t *d_xs, uint64_t xrows, const int32_t *d_act_row,
+                     const int32_t *d_bounds, uint64_t total_rows, void *d_y, uint32_t y_type,
+                     uint64_t ld_y);
+
+/* --------------------------------------------------------------- LM head logits */
+
+/* Penalties for repeated tokens, biases and grammar masks on logits
+ * [n_rows][n_vocab] (F32, F16 or BF16, `ld` apart) -> out of the same type
+ * (in place when d_out == d_logits).  Row b, token v, in this order:
+ *   n_all, n_gen = occurrences of v in hist[hist_off[b] .. hist_off[b+1]) and
+ *     in its part from entry gen[b] on (the tokens the model wrote; gen NULL: 0)
+ *   z = z > 0 ? z / rep : z * rep                   when n_all > 0
+ *   z = z - freq * n_gen - pres * (n_gen > 0)
+ *   z = z + the row's biases of v, summed in list order
+ *   z = -inf                                        when the mask's bit v is 0
+ * pen[b] = {rep, freq, pres}.  Biases of row b: bias_ids / bias[bias_off[b] ..
+ * bias_off[b+1]).  Masks: n_mask rows of mask_ld words, bit v of a row = bit
+ * v % 32 of word v / 32; mask_row[b] names row b's (below 0: none, n_mask or
+ * more: everything masked; NULL: row b).  Each of the three is optional: NULL
+ * pen and hist_off, NULL bias_off, NULL mask (a list without entries may be
+ * NULL with its offsets given).  Ids outside 0..n_vocab-1 are skipped.  fp32
+ * throughout, rounded once.  A row that a mask leaves without tokens is all
+ * -inf.  Keeps no state and no scratch.  The reference samples on the host
+ * (src/q4_tok.c:1901). */
+bool q4mi_logits_process(const void *d_logits, uint32_t type, uint64_t ld, uint32_t n_rows,
+                         uint32_t n_vocab, const int32_t *d_hist, const int64_t *d_hist_off,
+                         const int32_t *d_gen, const float *d_pen, const int32_t *d_bias_ids,
+                         const float *d_bias, const int64_t *d_bias_off, const uint32_t *d_mask,
+                         uint64_t mask_ld, uint32_t n_mask, const int32_t *d_mask_row,
+                         void *d_out, uint64_t ld_out);
+
 #ifdef __cplusplus
 }
 #endif

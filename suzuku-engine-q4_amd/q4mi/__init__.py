@@ -22,8 +22,12 @@ LIB_PATH = os.environ.get("Q4MI_LIB") or os.path.join(PKG, "lib", "libq4mi.so")
 # product library; its state (stream, scratch) is its own.
 MEAS_PATH = os.path.join(PKG, "lib", "libq4mi_meas.so")
 
+T_F32 = 0
+T_F16 = 1
 T_Q8_0 = 8
 T_IQ3_S = 21
+T_BF16 = 30
+T_MXFP4 = 39
 
 _c = ctypes
 _vp = _c.c_void_p
@@ -114,6 +118,17 @@ _SIGS = {
     "q4_xg_gu": (_b, [_u32, _vp, _u64, _u64, _u64, _u32, _u32, _vp, _u32, _vp, _vp, _vp]),
     "q4_xg_dn": (_b, [_u32, _vp, _u64, _u64, _u32, _u32, _vp, _u32, _vp, _vp]),
     "q4mi_expert_reduce_x": (_b, [_vp, _vp, _vp, _vp, _u32, _u32, _u32, _u64, _vp]),
+    "q4mi_mx4_code_bytes": (_u64, [_u64, _u64]),
+    "q4mi_mx4_scale_bytes": (_u64, [_u64, _u64]),
+    "q4mi_mx4_quant": (_b, [_vp, _u32, _u64, _vp, _u64, _u64, _vp, _vp]),
+    "q4mi_mx4_dequant": (_b, [_vp, _vp, _vp, _u64, _u64, _vp, _u32, _u64]),
+    "q4mi_mx4_mul": (_b, [_vp, _vp, _u64, _u64, _vp, _vp, _u32, _u64, _u64, _vp, _u32, _u64]),
+    "q4mi_mx4_mul_sel": (_b, [_vp, _vp, _u64, _u64, _u64, _u64, _u32, _vp, _vp, _u32, _u64, _u32,
+                              _vp, _u64, _vp, _u32, _u64]),
+    "q4mi_mx4_mul_id": (_b, [_vp, _vp, _u64, _u64, _u64, _u64, _u32, _vp, _vp, _u64, _vp, _vp,
+                             _u64, _vp, _u32, _u64]),
+    "q4mi_logits_process": (_b, [_vp, _u32, _u64, _u32, _u32, _vp, _vp, _vp, _vp, _vp, _vp, _vp,
+                                 _vp, _u64, _u32, _vp, _vp, _u64]),
 }
 
 # measurement build only
