@@ -87,6 +87,50 @@ __device__ inline uint32_t mx4_pack8(const float *v, uint32_t s) {
     return s == 255u ? 0u : q;
 }
 
+// Eight values of a float row from column c0 on (0 past cols); wide: the row
+// moves 16 bytes at a time.  row: index of the row's first element.
+__device__ inline void load_row8(const void *x, uint32_t xt, uint64_t row, uint32_t c0,
+                                 uint32_t cols, bool wide, float *v) {
+    const uint64_t at = row + c0;
+    if (wide && c0 + 8 <= cols) {
+        if (xt == kTypeF32) {
+            const float4 lo = *(const float4 *)((const float *)x + at);
+            const float4 hi = *(const float4 *)((const float *)x + at + 4);
+            v[0] = lo.x, v[1] = lo.y, v[2] = lo.z, v[3] = lo.w;
+            v[4] = hi.x, v[5] = hi.y, v[6] = hi.z, v[7] = hi.w;
+        } else {
+            const uint4 h = *(const uint4 *)((const uint16_t *)x + at);
+            const uint32_t w[4] = {h.x, h.y, h.z, h.w};
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                if (xt == kTypeBF16) {
+                    v[2 * i] = bits_f32(w[i] << 16);
+                    v[2 * i + 1] = bits_f32(w[i] & 0xffff0000u);
+                } else {
+                    v[2 * i] = (float)__builtin_bit_cast(_Float16, (uint16_t)w[i]);
+                    v[2 * i + 1] = (float)__builtin_bit_cast(_Float16, (uint16_t)(w[i] >> 16));
+                }
+            }
+        }
+    } else {
+#pragma unroll
+        for (uint32_t i = 0; i < 8; i++)
+            v[i] = c0 + i < cols ? load_as_f32(x, xt, at + i) : 0.f;
+    }
+}
+
+// Codes of this lane's eight values of a block that four adjacent lanes hold,
+// and the block's scale byte.
+__device__ inline uint32_t mx4_quant8(const float *v, uint32_t *s) {
+    uint32_t top = 0;
+#pragma unroll
+    for (int i = 0; i < 8; i++) top = max(top, f32_bits(v[i]) & 0x7fffffffu);
+    top = max(top, (uint32_t)__shfl_xor((int)top, 1, 64));
+    top = max(top, (uint32_t)__shfl_xor((int)top, 2, 64));
+    *s = mx4_scale_of(top);
+    return mx4_pack8(v, *s);
+}
+
 // 2^(s - 127) as fp32 (a subnormal for s = 0), NaN for 255.
 __device__ inline float mx4_scale_value(uint32_t s) {
     return bits_f32(s == 255u ? 0x7fc00000u : s ? s << 23 : 0x00400000u);

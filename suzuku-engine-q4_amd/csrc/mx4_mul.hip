@@ -11,6 +11,8 @@ namespace {
 
 typedef int v8i __attribute__((ext_vector_type(8)));
 typedef float v4f __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef u32x4 u32x4_a4 __attribute__((aligned(4)));   // in memory at any dword
 
 struct MulArgs {
     const uint8_t *w, *ws;          // weights: codes, scales
@@ -21,27 +23,180 @@ struct MulArgs {
     void *y;
     uint64_t w_rows, cols, w_stride, ws_stride, ldx, xrows, n, ldy;
     uint32_t n_expert, x_type, y_type, x_div;
+    uint32_t ks, seg, blocks;       // few rows: waves a tile, blocks of K in LDS, workgroups
+    bool x_wide, y_wide;            // whether rows can move 16 bytes at a time
 };
 
-__device__ inline v8i widen(uint4 q) {
-    v8i a = {(int)q.x, (int)q.y, (int)q.z, (int)q.w, 0, 0, 0, 0};
+__device__ inline v8i widen(u32x4 q) {
+    const v8i a = {(int)q.x, (int)q.y, (int)q.z, (int)q.w, 0, 0, 0, 0};
     return a;
 }
 
-// Block kb of a float row as codes and scale.
-__device__ inline uint4 quant_block(const void *x, uint32_t xt, uint64_t at, uint32_t left,
-                                    uint32_t *s) {
-    float v[32];
-    uint32_t top = 0;
-#pragma unroll
-    for (uint32_t i = 0; i < 32; i++) {
-        v[i] = i < left ? load_as_f32(x, xt, at + i) : 0.f;
-        top = max(top, f32_bits(v[i]) & 0x7fffffffu);
+// Four adjacent outputs, rounded once; `at` a multiple of 4.
+__device__ inline void store4(void *y, uint32_t yt, uint64_t at, v4f v) {
+    if (yt == kTypeF32) {
+        *(v4f *)((float *)y + at) = v;
+    } else {
+        const uint32_t lo = f32_to_16(v[0], yt) | (uint32_t)f32_to_16(v[1], yt) << 16;
+        const uint32_t hi = f32_to_16(v[2], yt) | (uint32_t)f32_to_16(v[3], yt) << 16;
+        *(uint2 *)((uint16_t *)y + at) = make_uint2(lo, hi);
     }
-    *s = mx4_scale_of(top);
-    return make_uint4(mx4_pack8(v, *s), mx4_pack8(v + 8, *s), mx4_pack8(v + 16, *s),
-                      mx4_pack8(v + 24, *s));
 }
+
+// ---------------------------------------------------------------- few rows
+//
+// Up to 16 activation rows against all weight rows: bound by reading the
+// weights once.  A wave takes 16 weight rows; lane (m, g) of it holds row m's
+// blocks 4s + g of a chunk of 16 blocks (s = 0..3), so four lanes read 64
+// adjacent bytes and a chunk's 16 scales are one 16-byte load, of which step s
+// uses byte g of dword s.  PF chunks (4 KB each with 16 rows) are in flight a
+// wave.  The activation rows sit in LDS, as codes: float rows are quantised on
+// the way there, once a workgroup.  KS waves share a tile along K and their
+// sums are joined in LDS in wave order, so a short matrix still occupies the
+// chip; the workgroups are persistent, so a tall one pays the LDS fill once.
+
+constexpr uint32_t kFewWaves = 4;
+constexpr uint32_t kFewRows = 16;
+
+// Blocks of a K segment held in LDS at once (36 KB at 8 or 16 rows).
+__host__ __device__ inline uint32_t few_segment(uint32_t rows) { return rows > 8 ? 128u : 256u; }
+// LDS strides of a row's codes and scales: 16 bytes more than a power of two,
+// so the rows of a fragment start in different banks.
+__host__ __device__ inline uint32_t few_code_ld(uint32_t seg) { return seg * 16u + 16u; }
+__host__ __device__ inline uint32_t few_scale_ld(uint32_t seg) { return seg + 16u; }
+
+// Blocks [b0, b0 + seg) of `rows` activation rows from x row xr0 into LDS;
+// blocks from nb on get codes 0 and scale 1.
+__device__ inline void few_stage(const MulArgs &a, uint64_t xr0, uint32_t rows, uint32_t b0,
+                                 uint32_t seg, uint32_t nb, uint32_t sld, uint8_t *codes,
+                                 uint8_t *scales) {
+    const uint32_t cld = few_code_ld(seg), scld = few_scale_ld(seg);
+    for (uint32_t i = threadIdx.x; i < rows * seg * 4; i += kFewWaves * 64) {
+        const uint32_t sub = i & 3u, q = i >> 2, b = q & (seg - 1), t = q / seg;
+        const uint64_t xr = xr0 + t;
+        const uint32_t bb = b0 + b;
+        uint32_t code = 0, s = 127;
+        if (bb < nb) {
+            if (a.x_type == kTypeMx4) {
+                code = *(const uint32_t *)((const uint8_t *)a.x + xr * (16ull * nb) + 16u * bb +
+                                           4u * sub);
+                s = a.xs[xr * sld + bb];
+            } else {
+                const uint32_t c0 = 32u * bb + 8u * sub;
+                float v[8];
+                load_row8(a.x, a.x_type, xr * a.ldx, c0, (uint32_t)a.cols, a.x_wide, v);
+                code = mx4_quant8(v, &s);
+            }
+        }
+        *(uint32_t *)(codes + t * cld + 16u * b + 4u * sub) = code;
+        if (sub == 0) scales[t * scld + b] = (uint8_t)s;
+    }
+}
+
+// FULL: rows are whole chunks of 16 blocks.  a.y row of activation row t is
+// y0 + t.
+template <bool FULL, uint32_t PF>
+__device__ inline void few_rows(const MulArgs &a, const uint8_t *w, const uint8_t *ws,
+                                uint64_t xr0, uint32_t rows, uint64_t y0, uint32_t block,
+                                uint32_t blocks, uint8_t *lds) {
+    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
+    const uint32_t m = lane & 15u, g = lane >> 4;
+    const uint32_t ks = a.ks, kw = wave & (ks - 1), sub = wave / ks, per = kFewWaves / ks;
+    const uint32_t nb = mx4_blocks(a.cols), sld = mx4_scale_row(nb);
+    const uint32_t seg = a.seg, nseg = (nb + seg - 1) / seg;
+    const uint32_t cld = few_code_ld(seg), scld = few_scale_ld(seg);
+    uint8_t *codes = lds, *scales = lds + rows * cld;
+    v4f *red = (v4f *)(scales + rows * scld);
+    const uint32_t tiles = (uint32_t)((a.w_rows + 15) / 16);
+    const uint32_t t = min(m, rows - 1);
+    const uint8_t *xc = codes + t * cld + 16u * g, *xsc = scales + t * scld;
+    const uint32_t rounds = (tiles + per * blocks - 1) / (per * blocks);
+    for (uint32_t i = 0; i < rounds; i++) {
+        const uint32_t tile = (i * blocks + block) * per + sub;
+        const bool mine = tile < tiles;
+        const uint64_t wr = min((uint64_t)(mine ? tile : 0u) * 16 + m, a.w_rows - 1);
+        const uint8_t *wp = w + wr * (16ull * nb), *wsp = ws + wr * sld;
+        v4f acc = {0.f, 0.f, 0.f, 0.f};
+        for (uint32_t sg = 0; sg < nseg; sg++) {
+            const uint32_t b0 = sg * seg, nch = (min(seg, nb - b0) + 15) / 16;
+            // the first batch is on its way while the activations are staged
+            uint32_t c0 = kw;
+            u32x4 wq[PF][4], wv[PF];
+            auto load = [&]() __attribute__((always_inline)) {
+#pragma unroll
+                for (uint32_t j = 0; j < PF; j++) {
+                    const uint32_t c = min(c0 + j * ks, nch - 1), bc = b0 + 16 * c;
+#pragma unroll
+                    for (uint32_t s = 0; s < 4; s++) {
+                        uint32_t b = bc + 4 * s + g;
+                        if (!FULL) b = min(b, nb - 1);
+                        wq[j][s] = *(const u32x4 *)(wp + 16u * b);
+                        if (!FULL) wv[j][s] = ((const uint32_t *)wsp)[min(bc / 4 + s, sld / 4 - 1)];
+                    }
+                    if (FULL) wv[j] = *(const u32x4_a4 *)(wsp + bc);
+                }
+            };
+            load();
+            if (nseg > 1 || i == 0) {
+                if (nseg > 1) __syncthreads();
+                few_stage(a, xr0, rows, b0, seg, nb, sld, codes, scales);
+                __syncthreads();
+            }
+            for (; c0 < nch; c0 += PF * ks) {
+                if (c0 != kw) load();
+#pragma unroll
+                for (uint32_t j = 0; j < PF; j++) {
+                    const uint32_t c = c0 + j * ks;
+                    if (c >= nch) break;
+                    const u32x4 xv = *(const u32x4 *)(xsc + 16u * c);
+#pragma unroll
+                    for (uint32_t s = 0; s < 4; s++) {
+                        const u32x4 xq = *(const u32x4 *)(xc + 256u * c + 64u * s);
+                        uint32_t wb = wv[j][s] >> (8 * g);
+                        if (!FULL && b0 + 16 * c + 4 * s + g >= nb) wb = 127;
+                        acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
+                            widen(wq[j][s]), widen(xq), acc, 4, 4, 0, (int)wb, 0,
+                            (int)(xv[s] >> (8 * g)));
+                    }
+                }
+            }
+        }
+        if (ks > 1) {
+            if (i) __syncthreads();   // the last round's sums have been read
+            red[wave * 64 + lane] = acc;
+            __syncthreads();
+            if (kw) continue;
+            for (uint32_t k = 1; k < ks; k++) acc += red[(wave + k) * 64 + lane];
+        }
+        if (!mine || m >= rows) continue;
+        const uint64_t r = (uint64_t)tile * 16 + 4 * g, at = (y0 + m) * a.ldy + r;
+        if (a.y_wide && r + 4 <= a.w_rows)
+            store4(a.y, a.y_type, at, acc);
+        else
+            for (uint32_t k = 0; k < 4; k++)
+                if (r + k < a.w_rows) store_from_f32(a.y, a.y_type, at + k, acc[k]);
+    }
+}
+
+// n <= 16 activation rows; `blocks` workgroups share the weight rows.
+template <bool FULL, uint32_t PF>
+__global__ __launch_bounds__(256) void mx4_few_k(MulArgs a) {
+    extern __shared__ __align__(16) uint8_t lds[];
+    few_rows<FULL, PF>(a, a.w, a.ws, 0, (uint32_t)a.n, 0, blockIdx.x, a.blocks, lds);
+}
+
+// Row p through the expert that the list names; grid (blocks, rows).
+template <bool FULL, uint32_t PF>
+__global__ __launch_bounds__(256) void mx4_sel_k(MulArgs a) {
+    extern __shared__ __align__(16) uint8_t lds[];
+    const uint32_t p = blockIdx.y;
+    const int32_t e = a.eid[p];
+    if (e < 0 || (uint32_t)e >= a.n_expert) return;
+    few_rows<FULL, PF>(a, a.w + e * a.w_stride, a.ws + e * a.ws_stride, p / a.x_div, 1, p,
+                       blockIdx.x, a.blocks, lds);
+}
+
+// ------------------------------------------------------------ rows in tiles
 
 // One wave: 16 weight rows from r0 against up to 16 activation rows; lane
 // l holds activation row l % 16 (xr, or -1 for none) and output row yr.
@@ -53,19 +208,14 @@ __device__ inline void wave_tile(const MulArgs &a, const uint8_t *w, const uint8
     v4f acc = {0.f, 0.f, 0.f, 0.f};
     for (uint32_t b0 = 0; b0 < nb; b0 += 4) {
         const uint32_t b = b0 + g;
-        uint4 wq = make_uint4(0, 0, 0, 0), xq = wq;
+        u32x4 wq = {0, 0, 0, 0}, xq = wq;
         uint32_t wsc = 127, xsc = 127;
         if (b < nb) {
-            wq = *(const uint4 *)(w + wr * (16ull * nb) + 16u * b);
+            wq = *(const u32x4 *)(w + wr * (16ull * nb) + 16u * b);
             wsc = ws[wr * sld + b];
             if (xr >= 0) {
-                if (a.x_type == kTypeMx4) {
-                    xq = *(const uint4 *)((const uint8_t *)a.x + xr * (16ull * nb) + 16u * b);
-                    xsc = a.xs[xr * (uint64_t)sld + b];
-                } else {
-                    const uint32_t left = (uint32_t)min((uint64_t)32, a.cols - 32ull * b);
-                    xq = quant_block(a.x, a.x_type, xr * a.ldx + 32ull * b, left, &xsc);
-                }
+                xq = *(const u32x4 *)((const uint8_t *)a.x + xr * (16ull * nb) + 16u * b);
+                xsc = a.xs[xr * (uint64_t)sld + b];
             }
         }
         acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(widen(wq), widen(xq), acc, 4, 4, 0,
@@ -87,18 +237,6 @@ __global__ __launch_bounds__(256) void mx4_dense_k(MulArgs a) {
     wave_tile(a, a.w, a.ws, r0, row, row);
 }
 
-// grid (16-row tiles / 4, rows)
-__global__ __launch_bounds__(256) void mx4_sel_k(MulArgs a) {
-    const uint64_t r0 = ((uint64_t)blockIdx.x * 4 + (threadIdx.x >> 6)) * 16;
-    if (r0 >= a.w_rows) return;
-    const uint64_t p = blockIdx.y;
-    const int32_t e = a.eid[p];
-    if (e < 0 || (uint32_t)e >= a.n_expert) return;
-    const bool me = (threadIdx.x & 15u) == 0;
-    wave_tile(a, a.w + e * a.w_stride, a.ws + e * a.ws_stride, r0, me ? (int64_t)(p / a.x_div) : -1,
-              me ? (int64_t)p : -1);
-}
-
 // grid (16-row tiles / 4, experts): every 16 packed rows of the expert
 __global__ __launch_bounds__(256) void mx4_id_k(MulArgs a) {
     const uint64_t r0 = ((uint64_t)blockIdx.x * 4 + (threadIdx.x >> 6)) * 16;
@@ -112,6 +250,34 @@ __global__ __launch_bounds__(256) void mx4_id_k(MulArgs a) {
         if (xr >= (int64_t)a.xrows) xr = -1;
         wave_tile(a, a.w + e * a.w_stride, a.ws + e * a.ws_stride, r0, xr, xr < 0 ? -1 : p);
     }
+}
+
+// Launch shape of the few-rows kernels for `rows` activation rows a workgroup
+// and `lists` independent products.
+struct FewPlan {
+    uint32_t ks, pf, blocks;
+    size_t lds;
+};
+FewPlan few_plan(MulArgs &a, uint32_t rows, uint32_t lists) {
+    const uint32_t nb = mx4_blocks(a.cols), tiles = (uint32_t)((a.w_rows + 15) / 16);
+    const uint32_t cus = (uint32_t)cu_count();
+    uint32_t seg = few_segment(rows);
+    while (seg > 16 && seg / 2 >= nb) seg /= 2;
+    const uint32_t nch = (std::min(seg, nb) + 15) / 16;
+    FewPlan p;
+    p.ks = 1;
+    while (p.ks < kFewWaves && p.ks * 2 <= nch && (uint64_t)tiles * lists * p.ks < 8ull * cus)
+        p.ks *= 2;
+    const uint32_t mine = (nch + p.ks - 1) / p.ks;
+    p.pf = mine >= 4 ? 4 : mine >= 2 ? 2 : 1;
+    const uint32_t per = kFewWaves / p.ks;
+    p.blocks = std::min((tiles + per - 1) / per, std::max(1u, cus * 4 / std::min(lists, cus * 4)));
+    p.lds = (size_t)rows * (few_code_ld(seg) + few_scale_ld(seg)) +
+            (p.ks > 1 ? kFewWaves * 64 * sizeof(v4f) : 0);
+    a.ks = p.ks, a.seg = seg, a.blocks = p.blocks;
+    a.x_wide = a.x_type != kTypeMx4 && !((uintptr_t)a.x & 15) && a.ldx * type_bytes(a.x_type) % 16 == 0;
+    a.y_wide = !((uintptr_t)a.y & 15) && a.ldy * type_bytes(a.y_type) % 16 == 0;
+    return p;
 }
 
 bool mul_ok(const char *who, const MulArgs &a) {
@@ -147,6 +313,16 @@ bool mul_ok(const char *who, const MulArgs &a) {
     return true;
 }
 
+// Launches KERNEL<rows are whole chunks, chunks in flight>.
+#define FEW_LAUNCH(KERNEL, GRID, P, A)                                                     \
+    do {                                                                                   \
+        const bool full = mx4_blocks((A).cols) % 16 == 0;                                  \
+        auto k = (P).pf == 4   ? (full ? KERNEL<true, 4> : KERNEL<false, 4>)               \
+                 : (P).pf == 2 ? (full ? KERNEL<true, 2> : KERNEL<false, 2>)               \
+                               : (full ? KERNEL<true, 1> : KERNEL<false, 1>);              \
+        k<<<GRID, dim3(kFewWaves * 64), (P).lds, stream()>>>(A);                           \
+    } while (0)
+
 constexpr uint64_t kFloatRows = 8;   // float rows that q4mi_mx4_mul takes
 
 }  // namespace
@@ -168,6 +344,11 @@ bool q4mi_mx4_mul(const uint8_t *d_w, const uint8_t *d_ws, uint64_t w_rows, uint
         return false;
     }
     if (!n) return true;
+    if (n <= kFewRows) {
+        const FewPlan p = few_plan(a, (uint32_t)n, 1);
+        FEW_LAUNCH(mx4_few_k, dim3(p.blocks), p, a);
+        return launch_ok("mx4_few_k");
+    }
     mx4_dense_k<<<dim3((uint32_t)((w_rows + 63) / 64), (uint32_t)((n + 15) / 16)), dim3(256), 0,
                   stream()>>>(a);
     return launch_ok("mx4_dense_k");
@@ -189,7 +370,8 @@ bool q4mi_mx4_mul_sel(const uint8_t *d_w, const uint8_t *d_ws, uint64_t w_rows, 
         return false;
     }
     if (!n) return true;
-    mx4_sel_k<<<dim3((uint32_t)((w_rows + 63) / 64), (uint32_t)n), dim3(256), 0, stream()>>>(a);
+    const FewPlan p = few_plan(a, 1, (uint32_t)n);
+    FEW_LAUNCH(mx4_sel_k, dim3(p.blocks, (uint32_t)n), p, a);
     return launch_ok("mx4_sel_k");
 }
 

@@ -26,40 +26,11 @@ __global__ __launch_bounds__(256) void mx4_quant_k(const void *__restrict__ x, u
     const uint32_t b = off % nb, sub = threadIdx.x & 3u;
     const uint64_t src = ids ? (uint64_t)(int64_t)ids[r] : r;
     const uint32_t c0 = b * 32 + sub * 8;
-    const uint64_t at = src * ld + c0;
     float v[8];
-    if (VEC && c0 + 8 <= cols) {
-        if (xt == kTypeF32) {
-            const float4 lo = *(const float4 *)((const float *)x + at);
-            const float4 hi = *(const float4 *)((const float *)x + at + 4);
-            v[0] = lo.x, v[1] = lo.y, v[2] = lo.z, v[3] = lo.w;
-            v[4] = hi.x, v[5] = hi.y, v[6] = hi.z, v[7] = hi.w;
-        } else {
-            const uint4 h = *(const uint4 *)((const uint16_t *)x + at);
-            const uint32_t w[4] = {h.x, h.y, h.z, h.w};
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                if (xt == kTypeBF16) {
-                    v[2 * i] = bits_f32(w[i] << 16);
-                    v[2 * i + 1] = bits_f32(w[i] & 0xffff0000u);
-                } else {
-                    v[2 * i] = (float)__builtin_bit_cast(_Float16, (uint16_t)w[i]);
-                    v[2 * i + 1] = (float)__builtin_bit_cast(_Float16, (uint16_t)(w[i] >> 16));
-                }
-            }
-        }
-    } else {
-#pragma unroll
-        for (uint32_t i = 0; i < 8; i++)
-            v[i] = c0 + i < cols ? load_as_f32(x, xt, at + i) : 0.f;
-    }
-    uint32_t top = 0;
-#pragma unroll
-    for (int i = 0; i < 8; i++) top = max(top, f32_bits(v[i]) & 0x7fffffffu);
-    top = max(top, (uint32_t)__shfl_xor((int)top, 1, 64));
-    top = max(top, (uint32_t)__shfl_xor((int)top, 2, 64));
-    const uint32_t s = mx4_scale_of(top);
-    *(uint32_t *)(codes + r * (16ull * nb) + b * 16u + sub * 4u) = mx4_pack8(v, s);
+    load_row8(x, xt, src * ld, c0, cols, VEC, v);
+    uint32_t s;
+    const uint32_t q = mx4_quant8(v, &s);
+    *(uint32_t *)(codes + r * (16ull * nb) + b * 16u + sub * 4u) = q;
     if (sub == 0) {
         uint8_t *p = scales + r * sld;
         p[b] = (uint8_t)s;

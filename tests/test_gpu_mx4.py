@@ -161,6 +161,22 @@ def test_mul_exact(gpu, n, rows, cols):
     assert (got[n:] == -7).all() and (got[:, rows:] == -7).all()
 
 
+@pytest.mark.parametrize("n,rows,cols", [(1, 50, 16384), (8, 40, 8224), (16, 70, 9000),
+                                         (16, 5000, 4128), (40, 64, 16000), (300, 260, 8192)])
+def test_mul_long_rows(gpu, n, rows, cols):
+    """Rows of many K segments; one scale, so sums are multiples of 1/4 below
+    36 * 16384 < 2^20: exact."""
+    rng = np.random.default_rng(cols)
+    w, ws = ref.random_rows(rng, rows, cols, 127, 127)
+    x, xs = ref.random_rows(rng, n, cols, 127, 127)
+    want = ref.values(x, xs, cols) @ ref.values(w, ws, cols).T
+    y = torch.empty((n, rows), device="cuda")
+    d = [dev(a) for a in (w, ws, x, xs)]
+    q4mi.check(gpu.q4mi_mx4_mul(d[0].data_ptr(), d[1].data_ptr(), rows, cols, d[2].data_ptr(),
+                                d[3].data_ptr(), MX4, 0, n, y.data_ptr(), 0, rows), "mul")
+    assert np.array_equal(host(y), want)
+
+
 @pytest.mark.parametrize("yt", sorted(TYPES))
 @pytest.mark.parametrize("n,rows,cols", [(1, 64, 2048), (5, 100, 333), (40, 200, 640),
                                          (200, 384, 1024), (260, 270, 2560)])
