@@ -2,8 +2,16 @@
 //   y[t][r] = sum over blocks b of 2^(sw + sx - 254) * sum_i w[r][32b+i] x[t][32b+i]
 // on v_mfma_scale_f32_16x16x128_f8f6f4, whose lane (row m, group g) takes one
 // block of 32 codes and its scale byte, and which adds in fp32.
+#include <type_traits>
+
 #include "mx4.h"
 #include "q4mi_internal.h"
+#ifndef MX4_L
+#define MX4_L 2, 4, 2
+#endif
+#ifndef MX4_I
+#define MX4_I 64, 128, 1, 4, 2
+#endif
 
 using namespace q4mi;
 
@@ -24,6 +32,7 @@ struct MulArgs {
     uint64_t w_rows, cols, w_stride, ws_stride, ldx, xrows, n, ldy;
     uint32_t n_expert, x_type, y_type, x_div;
     uint32_t ks, seg, blocks;       // few rows: waves a tile, blocks of K in LDS, workgroups
+    uint32_t m_tiles, n_tiles, zs;  // tiles: along the activations and weights, shares of a slice
     bool x_wide, y_wide;            // whether rows can move 16 bytes at a time
 };
 
@@ -197,58 +206,278 @@ __global__ __launch_bounds__(256) void mx4_sel_k(MulArgs a) {
 }
 
 // ------------------------------------------------------------ rows in tiles
+//
+// BM activation rows x BN weight rows a workgroup of WM x WN waves, on
+// v_mfma_scale_f32_32x32x64_f8f6f4.  K goes in stages of 8 blocks (256
+// values): 128 bytes of codes a row, a whole cache line, come by global -> LDS
+// copies into one of two buffers while the matrix units work on the other.
+// Scales come for four stages at once (32 bytes a row, a quarter of the copies
+// a stage): with 8 bytes a row and stage they asked the L2 for as many lines
+// as the codes.  Lane (row, half h) of a fragment takes blocks 4h + s of the
+// stage (s = 0..3), so one dword holds its scales and step s picks a byte of
+// it in the instruction.
+//
+// LDS places: chunk c (16 bytes) of codes row r at c ^ ((r >> 1) & 7), dword d
+// of scales row r at d ^ ((r >> 3) & 7), so that a fragment's reads spread over
+// all 64 banks; the copies fill LDS in lane order, so the lanes permute their
+// source addresses instead.
 
-// One wave: 16 weight rows from r0 against up to 16 activation rows; lane
-// l holds activation row l % 16 (xr, or -1 for none) and output row yr.
-__device__ inline void wave_tile(const MulArgs &a, const uint8_t *w, const uint8_t *ws,
-                                 uint64_t r0, int64_t xr, int64_t yr) {
-    const uint32_t lane = threadIdx.x & 63u, m = lane & 15u, g = lane >> 4;
-    const uint32_t nb = mx4_blocks(a.cols), sld = mx4_scale_row(nb);
-    const uint64_t wr = min(r0 + m, a.w_rows - 1);
-    v4f acc = {0.f, 0.f, 0.f, 0.f};
-    for (uint32_t b0 = 0; b0 < nb; b0 += 4) {
-        const uint32_t b = b0 + g;
-        u32x4 wq = {0, 0, 0, 0}, xq = wq;
-        uint32_t wsc = 127, xsc = 127;
-        if (b < nb) {
-            wq = *(const u32x4 *)(w + wr * (16ull * nb) + 16u * b);
-            wsc = ws[wr * sld + b];
-            if (xr >= 0) {
-                xq = *(const u32x4 *)((const uint8_t *)a.x + xr * (16ull * nb) + 16u * b);
-                xsc = a.xs[xr * (uint64_t)sld + b];
-            }
+typedef float v16f __attribute__((ext_vector_type(16)));
+
+__device__ inline uint32_t tile_swz(uint32_t row) { return (row >> 1) & 7u; }
+
+// Lane i's 16 (4) bytes land at LDS address lds + 16 i (4 i); from a pointer,
+// or from a uniform base and a 32-bit offset.  Inline asm, so that the
+// compiler adds no wait before the next LDS read.
+__device__ inline void copy16(const void *g, uint32_t lds) {
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(g),
+                 "s"(lds)
+                 : "memory");
+}
+__device__ inline void copy16(const void *base, uint32_t off, uint32_t lds) {
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off),
+                 "s"(base), "s"(lds)
+                 : "memory");
+}
+__device__ inline void copy4(const void *g, uint32_t lds) {
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off" ::"v"(g),
+                 "s"(lds)
+                 : "memory");
+}
+__device__ inline void copy4(const void *base, uint32_t off, uint32_t lds) {
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dword %0, %1" ::"v"(off),
+                 "s"(base), "s"(lds)
+                 : "memory");
+}
+// This wave's copies have landed and its LDS reads are done; then the
+// workgroup meets.
+__device__ inline void stage_barrier() {
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+}
+
+// LDS: two stages of codes, two windows (four stages) of scales.
+template <uint32_t BM, uint32_t BN>
+constexpr uint32_t tile_lds() { return (BM + BN) * 2 * (128 + 32); }
+
+// Weight rows [r0, r0 + BN) of w against activation rows [p0, p0 + BM), of
+// which those below phi exist; the row read for p is act[p] with GATHER, else
+// p.  Rows past either end are read as the last one and not stored.
+template <uint32_t BM, uint32_t BN, uint32_t WM, uint32_t WN, bool GATHER>
+__device__ inline void tile(const MulArgs &a, const uint8_t *w, const uint8_t *ws, uint64_t r0,
+                            int64_t p0, int64_t phi, uint8_t *lds) {
+    constexpr uint32_t NW = WM * WN;
+    constexpr uint32_t FM = BM / (32 * WM), FN = BN / (32 * WN);
+    constexpr uint32_t RA = BM / 8 / NW, RB = BN / 8 / NW;   // 8-row copies of each side a wave
+    static_assert(FM && FN && RA && RB, "tile too small for its waves");
+    constexpr uint32_t kStage = (BM + BN) * 128, kWindow = (BM + BN) * 32, kScales = 2 * kStage;
+    const uint32_t lane = threadIdx.x & 63u, l8 = lane >> 3;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t nb = mx4_blocks(a.cols), sld = mx4_scale_row(nb), nk = (nb + 7) / 8;
+    const uint32_t row_bytes = 16u * nb;
+    const uint32_t base = (uint32_t)(uintptr_t)lds;     // LDS offset: low half of the address
+
+    // sources of this lane's part of every copy, without the place in K: row
+    // pointers with GATHER, else offsets from the tile's first row
+    const uint8_t *xc = (const uint8_t *)a.x, *xs = a.xs;
+    const uint8_t *xp[GATHER ? RA : 1], *xsp[GATHER ? RA : 1];
+    uint32_t xo[RA], xso[RA], wo[RB], wso[RB];
+    if (!GATHER) xc += (uint64_t)p0 * row_bytes, xs += (uint64_t)p0 * sld;
+    w += r0 * row_bytes, ws += r0 * sld;
+    const uint32_t xlast = (uint32_t)min((int64_t)BM, phi - p0) - 1;
+    const uint32_t wlast = (uint32_t)min((uint64_t)BN, a.w_rows - r0) - 1;
+    auto gathered = [&](uint32_t m) -> uint64_t {
+        const int64_t r = a.act[p0 + m];
+        return r < 0 || r >= (int64_t)a.xrows ? 0 : (uint64_t)r;
+    };
+#pragma unroll
+    for (uint32_t j = 0; j < RA; j++) {
+        const uint32_t m = min((wave * RA + j) * 8 + l8, xlast), ms = min((wave + NW * j) * 8 + l8, xlast);
+        if constexpr (GATHER) {
+            xp[j] = xc + gathered(m) * row_bytes;
+            xsp[j] = xs + gathered(ms) * sld;
+        } else {
+            xo[j] = m * row_bytes, xso[j] = ms * sld;
         }
-        acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(widen(wq), widen(xq), acc, 4, 4, 0,
-                                                               (int)wsc, 0, (int)xsc);
     }
-    if (yr < 0) return;
-    for (uint32_t i = 0; i < 4; i++) {
-        const uint64_t r = r0 + 4 * g + i;
-        if (r < a.w_rows) store_from_f32(a.y, a.y_type, yr * a.ldy + r, acc[i]);
+#pragma unroll
+    for (uint32_t j = 0; j < RB; j++) {
+        wo[j] = min((wave * RB + j) * 8 + l8, wlast) * row_bytes;
+        wso[j] = min((wave + NW * j) * 8 + l8, wlast) * sld;
+    }
+    // stage k's codes; blocks past the last are read as the last
+    auto fetch = [&](uint32_t k) __attribute__((always_inline)) {
+        const uint32_t to = base + (k & 1u) * kStage;
+#pragma unroll
+        for (uint32_t j = 0; j < RA; j++) {
+            const uint32_t c = (lane & 7u) ^ tile_swz((wave * RA + j) * 8 + l8);
+            const uint32_t at = 16u * min(8 * k + c, nb - 1), d = to + (wave * RA + j) * 1024;
+            if constexpr (GATHER)
+                copy16(xp[j] + at, d);
+            else
+                copy16(xc, xo[j] + at, d);
+        }
+#pragma unroll
+        for (uint32_t j = 0; j < RB; j++) {
+            const uint32_t c = (lane & 7u) ^ tile_swz((wave * RB + j) * 8 + l8);
+            copy16(w, wo[j] + 16u * min(8 * k + c, nb - 1),
+                   to + BM * 128 + (wave * RB + j) * 1024);
+        }
+    };
+    // quarter q of window v's scales; dwords past the last are read as the last
+    auto fetch_scales = [&](uint32_t v, uint32_t q) __attribute__((always_inline)) {
+        const uint32_t to = base + kScales + (v & 1u) * kWindow;
+#pragma unroll
+        for (uint32_t j = 0; j < (RA > RB ? RA : RB); j++) {
+            if ((j & 3u) != q) continue;
+            const uint32_t c = wave + NW * j;
+            const uint32_t at = 4u * min(8 * v + ((lane & 7u) ^ (c & 7u)), sld / 4 - 1);
+            if (j < RA) {
+                if constexpr (GATHER)
+                    copy4(xsp[j] + at, to + c * 256);
+                else
+                    copy4(xs, xso[j] + at, to + c * 256);
+            }
+            if (j < RB) copy4(ws, wso[j] + at, to + BM * 32 + c * 256);
+        }
+    };
+
+    const uint32_t wm = wave / WN, wn = wave % WN, lr = lane & 31u, h = lane >> 5;
+    const uint32_t ra = wm * FM * 32 + lr, rb = wn * FN * 32 + lr;
+    uint32_t off[4];
+#pragma unroll
+    for (uint32_t s = 0; s < 4; s++) off[s] = 16u * ((4 * h + s) ^ tile_swz(lr));
+
+    v16f acc[FM][FN];
+#pragma unroll
+    for (uint32_t i = 0; i < FM; i++)
+#pragma unroll
+        for (uint32_t j = 0; j < FN; j++)
+#pragma unroll
+            for (uint32_t q = 0; q < 16; q++) acc[i][j][q] = 0.f;
+
+    auto work = [&](uint32_t k, auto tail) __attribute__((always_inline)) {
+        const uint8_t *st = lds + (k & 1u) * kStage;
+        const uint8_t *xa = st + ra * 128, *wb = st + (BM + rb) * 128;
+        const uint8_t *sc = lds + kScales + ((k >> 2) & 1u) * kWindow;
+        const uint32_t d = 2 * (k & 3u) + h;
+        uint32_t sx[FM], sw[FN];
+#pragma unroll
+        for (uint32_t i = 0; i < FM; i++) {
+            const uint32_t row = ra + 32 * i;
+            sx[i] = *(const uint32_t *)(sc + row * 32 + 4 * (d ^ ((row >> 3) & 7u)));
+        }
+#pragma unroll
+        for (uint32_t j = 0; j < FN; j++) {
+            const uint32_t row = rb + 32 * j;
+            sw[j] = *(const uint32_t *)(sc + (BM + row) * 32 + 4 * (d ^ ((row >> 3) & 7u)));
+        }
+        auto step = [&](auto s_) __attribute__((always_inline)) {
+            constexpr uint32_t s = decltype(s_)::value;
+            u32x4 xq[FM], wq[FN];
+#pragma unroll
+            for (uint32_t i = 0; i < FM; i++) xq[i] = *(const u32x4 *)(xa + i * 4096 + off[s]);
+#pragma unroll
+            for (uint32_t j = 0; j < FN; j++) wq[j] = *(const u32x4 *)(wb + j * 4096 + off[s]);
+            if constexpr (decltype(tail)::value) {
+                // blocks past the row's end: codes 0 on one side, scale 1 on both
+                const bool none = 8 * k + 4 * h + s >= nb;
+                const uint32_t clear = 255u << (8 * s), one = 127u << (8 * s);
+#pragma unroll
+                for (uint32_t i = 0; i < FM; i++) {
+                    xq[i] = none ? (u32x4){0, 0, 0, 0} : xq[i];
+                    sx[i] = none ? (sx[i] & ~clear) | one : sx[i];
+                }
+#pragma unroll
+                for (uint32_t j = 0; j < FN; j++) sw[j] = none ? (sw[j] & ~clear) | one : sw[j];
+            }
+#pragma unroll
+            for (uint32_t i = 0; i < FM; i++)
+#pragma unroll
+                for (uint32_t j = 0; j < FN; j++)
+                    acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(
+                        widen(wq[j]), widen(xq[i]), acc[i][j], 4, 4, s, (int)sw[j], s, (int)sx[i]);
+        };
+        step(std::integral_constant<uint32_t, 0>());
+        step(std::integral_constant<uint32_t, 1>());
+        step(std::integral_constant<uint32_t, 2>());
+        step(std::integral_constant<uint32_t, 3>());
+    };
+
+#pragma unroll
+    for (uint32_t q = 0; q < 4; q++) fetch_scales(0, q);
+    fetch(0);
+    uint32_t k = 0;
+    for (; k + 1 < nk; k++) {
+        // after the barrier nobody reads what stage k - 1 and, for k = 4v, window v - 1 held
+        stage_barrier();
+        fetch(k + 1);
+        if ((k | 3u) + 1 < nk) fetch_scales((k >> 2) + 1, k & 3u);
+        work(k, std::false_type());
+    }
+    stage_barrier();
+    work(k, std::true_type());
+
+    // lane: activation row lr of its fragment, weight rows 8q + 4h + 0..3
+#pragma unroll
+    for (uint32_t i = 0; i < FM; i++) {
+        const int64_t p = p0 + ra + 32 * i;
+        if (p >= phi) continue;
+        if (GATHER && (a.act[p] < 0 || (int64_t)a.act[p] >= (int64_t)a.xrows)) continue;
+#pragma unroll
+        for (uint32_t j = 0; j < FN; j++)
+#pragma unroll
+            for (uint32_t q = 0; q < 4; q++) {
+                const uint64_t r = r0 + wn * FN * 32 + 32 * j + 8 * q + 4 * h;
+                const v4f v = {acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2],
+                               acc[i][j][4 * q + 3]};
+                const uint64_t at = p * a.ldy + r;
+                if (a.y_wide && r + 4 <= a.w_rows)
+                    store4(a.y, a.y_type, at, v);
+                else
+                    for (uint32_t n = 0; n < 4; n++)
+                        if (r + n < a.w_rows) store_from_f32(a.y, a.y_type, at + n, v[n]);
+            }
     }
 }
 
-// grid (16-row tiles / 4, 16-row tiles of activations)
-__global__ __launch_bounds__(256) void mx4_dense_k(MulArgs a) {
-    const uint64_t r0 = ((uint64_t)blockIdx.x * 4 + (threadIdx.x >> 6)) * 16;
-    if (r0 >= a.w_rows) return;
-    const uint64_t t = (uint64_t)blockIdx.y * 16 + (threadIdx.x & 15u);
-    const int64_t row = t < a.n ? (int64_t)t : -1;
-    wave_tile(a, a.w, a.ws, r0, row, row);
+// Tiles of a dense product, `a.blocks` of them, a.m_tiles along the
+// activations.  Workgroups go to the eight dies in turn, each with an L2 of
+// its own: a die takes a contiguous run of tiles, in groups of kGroup
+// activation tiles, so that its L2 holds what its tiles share.
+constexpr uint32_t kGroup = 8;
+template <uint32_t BM, uint32_t BN, uint32_t WM, uint32_t WN, uint32_t WAVES>
+__global__ __launch_bounds__(64 * WM * WN, WAVES) void mx4_dense_k(MulArgs a) {
+    extern __shared__ __align__(16) uint8_t lds[];
+    const uint32_t die = blockIdx.x & 7u, i = blockIdx.x >> 3;
+    const uint32_t q = a.blocks >> 3, rem = a.blocks & 7u;
+    const uint32_t t = die * q + min(die, rem) + i;
+    const uint32_t n_tiles = a.blocks / a.m_tiles;
+    const uint32_t group = t / (kGroup * n_tiles), in = t - group * kGroup * n_tiles;
+    const uint32_t gm = min(kGroup, a.m_tiles - group * kGroup);
+    const uint32_t mt = group * kGroup + in % gm, nt = in / gm;
+    tile<BM, BN, WM, WN, false>(a, a.w, a.ws, (uint64_t)nt * BN, (int64_t)mt * BM, (int64_t)a.n, lds);
 }
 
-// grid (16-row tiles / 4, experts): every 16 packed rows of the expert
-__global__ __launch_bounds__(256) void mx4_id_k(MulArgs a) {
-    const uint64_t r0 = ((uint64_t)blockIdx.x * 4 + (threadIdx.x >> 6)) * 16;
-    if (r0 >= a.w_rows) return;
-    const uint32_t e = blockIdx.y;
-    const int64_t lo = max(a.bounds[e], 0), hi = min((int64_t)a.bounds[e + 1], (int64_t)a.n);
-    for (int64_t p0 = lo; p0 < hi; p0 += 16) {
-        const int64_t p = p0 + (threadIdx.x & 15u);
-        int64_t xr = -1;
-        if (p < hi) xr = a.act ? (int64_t)a.act[p] : p;
-        if (xr >= (int64_t)a.xrows) xr = -1;
-        wave_tile(a, a.w + e * a.w_stride, a.ws + e * a.ws_stride, r0, xr, xr < 0 ? -1 : p);
+// Packed rows: a workgroup takes one BN-row slice of one expert and every
+// zs-th BM-row tile of its stretch; the zs workgroups of a slice are 8 apart,
+// on one die.  No tile list: an expert without rows costs an empty workgroup.
+template <uint32_t BM, uint32_t BN, uint32_t WM, uint32_t WN, uint32_t WAVES>
+__global__ __launch_bounds__(64 * WM * WN, WAVES) void mx4_id_k(MulArgs a) {
+    extern __shared__ __align__(16) uint8_t lds[];
+    const uint32_t u = blockIdx.x / (8 * a.zs), v = blockIdx.x - u * 8 * a.zs;
+    const uint32_t slice = u * 8 + (v & 7u), z = v >> 3;
+    const uint32_t e = slice / a.n_tiles, nt = slice - e * a.n_tiles;
+    if (e >= a.n_expert) return;
+    // without a row list, packed row p is activation row p: those past xrows do not exist
+    const int64_t rows = (int64_t)(a.act ? a.n : min(a.n, a.xrows));
+    const int64_t lo = max(a.bounds[e], 0), hi = min((int64_t)a.bounds[e + 1], rows);
+    const uint8_t *w = a.w + e * a.w_stride, *ws = a.ws + e * a.ws_stride;
+    for (int64_t p0 = lo + (int64_t)z * BM; p0 < hi; p0 += (int64_t)a.zs * BM) {
+        if (a.act)
+            tile<BM, BN, WM, WN, true>(a, w, ws, (uint64_t)nt * BN, p0, hi, lds);
+        else
+            tile<BM, BN, WM, WN, false>(a, w, ws, (uint64_t)nt * BN, p0, hi, lds);
+        __syncthreads();   // the next tile's copies overwrite what slower waves may still read
     }
 }
 
@@ -313,6 +542,45 @@ bool mul_ok(const char *who, const MulArgs &a) {
     return true;
 }
 
+void wide_rows(MulArgs &a) {
+    a.y_wide = !((uintptr_t)a.y & 15) && a.ldy * type_bytes(a.y_type) % 16 == 0;
+}
+
+template <uint32_t BM, uint32_t BN, uint32_t WM, uint32_t WN, uint32_t WAVES>
+bool dense_launch(MulArgs &a) {
+    static DynLds st;
+    constexpr size_t lds = tile_lds<BM, BN>();
+    auto k = mx4_dense_k<BM, BN, WM, WN, WAVES>;
+    if (!dyn_lds_ok((const void *)k, lds, lds, st, "mx4_dense_k")) return false;
+    const uint64_t m = (a.n + BM - 1) / BM, n = (a.w_rows + BN - 1) / BN;
+    if (m * n > 0x7fffffffu) {
+        set_error("q4mi_mx4_mul: too many tiles");
+        return false;
+    }
+    a.m_tiles = (uint32_t)m, a.blocks = (uint32_t)(m * n);
+    wide_rows(a);
+    k<<<dim3(a.blocks), dim3(64 * WM * WN), lds, stream()>>>(a);
+    return launch_ok("mx4_dense_k");
+}
+
+template <uint32_t BM, uint32_t BN, uint32_t WM, uint32_t WN, uint32_t WAVES>
+bool id_launch(MulArgs &a) {
+    static DynLds st;
+    constexpr size_t lds = tile_lds<BM, BN>();
+    auto k = mx4_id_k<BM, BN, WM, WN, WAVES>;
+    if (!dyn_lds_ok((const void *)k, lds, lds, st, "mx4_id_k")) return false;
+    a.n_tiles = (uint32_t)((a.w_rows + BN - 1) / BN);
+    a.zs = 4;
+    const uint64_t slices = ((uint64_t)a.n_tiles * a.n_expert + 7) / 8 * 8;
+    if (slices * a.zs > 0x7fffffffu) {
+        set_error("q4mi_mx4_mul_id: too many tiles");
+        return false;
+    }
+    wide_rows(a);
+    k<<<dim3((uint32_t)(slices * a.zs)), dim3(64 * WM * WN), lds, stream()>>>(a);
+    return launch_ok("mx4_id_k");
+}
+
 // Launches KERNEL<rows are whole chunks, chunks in flight>.
 #define FEW_LAUNCH(KERNEL, GRID, P, A)                                                     \
     do {                                                                                   \
@@ -349,9 +617,9 @@ bool q4mi_mx4_mul(const uint8_t *d_w, const uint8_t *d_ws, uint64_t w_rows, uint
         FEW_LAUNCH(mx4_few_k, dim3(p.blocks), p, a);
         return launch_ok("mx4_few_k");
     }
-    mx4_dense_k<<<dim3((uint32_t)((w_rows + 63) / 64), (uint32_t)((n + 15) / 16)), dim3(256), 0,
-                  stream()>>>(a);
-    return launch_ok("mx4_dense_k");
+    if (n >= 512 && w_rows >= 512) return dense_launch<256, 256, MX4_L>(a);
+    if (n > 64) return dense_launch<128, 128, 2, 2, 2>(a);
+    return dense_launch<64, 128, 1, 4, 2>(a);
 }
 
 /* Every row through its own expert (see include/q4mi.h). */
@@ -392,8 +660,7 @@ bool q4mi_mx4_mul_id(const uint8_t *d_w, const uint8_t *d_ws, uint64_t w_rows, u
         return false;
     }
     if (!total_rows || !xrows) return true;
-    mx4_id_k<<<dim3((uint32_t)((w_rows + 63) / 64), n_expert), dim3(256), 0, stream()>>>(a);
-    return launch_ok("mx4_id_k");
+    return id_launch<MX4_I>(a);
 }
 
 }  // extern "C"

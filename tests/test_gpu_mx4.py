@@ -338,6 +338,27 @@ def test_mul_id_exact(gpu, counts, rows, cols, spare, gather):
     assert np.array_equal(host(y), want)
 
 
+def test_mul_id_fewer_activations_than_rows(gpu):
+    """Without a row list, packed rows past xrows are left as they were."""
+    rng = np.random.default_rng(21)
+    counts, rows, cols, xrows = [70, 90, 40], 40, 96, 100
+    w, ws, wv, st, sst = arena(rng, 3, rows, cols)
+    x, xs = ref.random_rows(rng, xrows, cols, 126, 128)
+    xv = ref.values(x, xs, cols)
+    bounds = np.concatenate([[0], np.cumsum(counts)]).astype(np.int32)
+    n = sum(counts)
+    e = np.repeat(np.arange(3), counts)
+    want = np.full((n, rows), -7.0)
+    for p in range(xrows):
+        want[p] = wv[e[p]] @ xv[p]
+    y = torch.full((n, rows), -7.0, device="cuda")
+    d = [dev(a) for a in (x, xs, bounds)]
+    q4mi.check(gpu.q4mi_mx4_mul_id(w.data_ptr(), ws.data_ptr(), rows, cols, st, sst, 3,
+                                   d[0].data_ptr(), d[1].data_ptr(), xrows, None, d[2].data_ptr(),
+                                   n, y.data_ptr(), 0, rows), "id")
+    assert np.array_equal(host(y), want)
+
+
 @pytest.mark.parametrize("yt", [q4mi.T_F16, q4mi.T_BF16])
 def test_mul_id_types(gpu, yt):
     rng = np.random.default_rng(8)
