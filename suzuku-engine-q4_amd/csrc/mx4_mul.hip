@@ -268,7 +268,7 @@ __device__ inline void tile(const MulArgs &a, const uint8_t *w, const uint8_t *w
     constexpr uint32_t NW = WM * WN;
     constexpr uint32_t FM = BM / (32 * WM), FN = BN / (32 * WN);
     constexpr uint32_t RA = BM / 8 / NW, RB = BN / 8 / NW;   // 8-row copies of each side a wave
-    static_assert(FM && FN && RA && RB, "tile too small for its waves");
+    static_assert(FM && FN && RA && RB, "tile and waves");
     constexpr uint32_t kStage = (BM + BN) * 128, kWindow = (BM + BN) * 32, kScales = 2 * kStage;
     const uint32_t lane = threadIdx.x & 63u, l8 = lane >> 3;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -280,7 +280,7 @@ __device__ inline void tile(const MulArgs &a, const uint8_t *w, const uint8_t *w
     // pointers with GATHER, else offsets from the tile's first row
     const uint8_t *xc = (const uint8_t *)a.x, *xs = a.xs;
     const uint8_t *xp[GATHER ? RA : 1], *xsp[GATHER ? RA : 1];
-    uint32_t xo[RA], xso[RA], wo[RB], wso[RB];
+    uint32_t xo[RA], wo[RB];
     if (!GATHER) xc += (uint64_t)p0 * row_bytes, xs += (uint64_t)p0 * sld;
     w += r0 * row_bytes, ws += r0 * sld;
     const uint32_t xlast = (uint32_t)min((int64_t)BM, phi - p0) - 1;
@@ -291,56 +291,73 @@ __device__ inline void tile(const MulArgs &a, const uint8_t *w, const uint8_t *w
     };
 #pragma unroll
     for (uint32_t j = 0; j < RA; j++) {
-        const uint32_t m = min((wave * RA + j) * 8 + l8, xlast), ms = min((wave + NW * j) * 8 + l8, xlast);
+        const uint32_t m = min((wave * RA + j) * 8 + l8, xlast);
         if constexpr (GATHER) {
             xp[j] = xc + gathered(m) * row_bytes;
-            xsp[j] = xs + gathered(ms) * sld;
+            xsp[j] = xs + gathered(min((wave + NW * j) * 8 + l8, xlast)) * sld;
         } else {
-            xo[j] = m * row_bytes, xso[j] = ms * sld;
+            xo[j] = m * row_bytes;
         }
     }
 #pragma unroll
-    for (uint32_t j = 0; j < RB; j++) {
-        wo[j] = min((wave * RB + j) * 8 + l8, wlast) * row_bytes;
-        wso[j] = min((wave + NW * j) * 8 + l8, wlast) * sld;
-    }
-    // stage k's codes; blocks past the last are read as the last
-    auto fetch = [&](uint32_t k) __attribute__((always_inline)) {
+    for (uint32_t j = 0; j < RB; j++) wo[j] = min((wave * RB + j) * 8 + l8, wlast) * row_bytes;
+    // Part i of FM of stage k's codes; blocks past the last are read as the last.
+    const uint32_t c0 = (lane & 7u) ^ (l8 >> 1);        // chunk of an even copy; c0 ^ 4 of an odd
+    auto fetch = [&](uint32_t k, uint32_t i) __attribute__((always_inline)) {
         const uint32_t to = base + (k & 1u) * kStage;
+        const uint32_t at[2] = {16u * min(8 * k + c0, nb - 1), 16u * min(8 * k + (c0 ^ 4u), nb - 1)};
 #pragma unroll
         for (uint32_t j = 0; j < RA; j++) {
-            const uint32_t c = (lane & 7u) ^ tile_swz((wave * RA + j) * 8 + l8);
-            const uint32_t at = 16u * min(8 * k + c, nb - 1), d = to + (wave * RA + j) * 1024;
+            if (j % FM != i) continue;
+            const uint32_t c = wave * RA + j, d = to + c * 1024;
             if constexpr (GATHER)
-                copy16(xp[j] + at, d);
+                copy16(xp[j] + at[c & 1u], d);
             else
-                copy16(xc, xo[j] + at, d);
+                copy16(xc, xo[j] + at[c & 1u], d);
         }
 #pragma unroll
         for (uint32_t j = 0; j < RB; j++) {
-            const uint32_t c = (lane & 7u) ^ tile_swz((wave * RB + j) * 8 + l8);
-            copy16(w, wo[j] + 16u * min(8 * k + c, nb - 1),
-                   to + BM * 128 + (wave * RB + j) * 1024);
+            if (j % FM != i) continue;
+            const uint32_t c = wave * RB + j;
+            copy16(w, wo[j] + at[c & 1u], to + BM * 128 + c * 1024);
         }
     };
-    // quarter q of window v's scales; dwords past the last are read as the last
+    // Quarter q of window v's scales (a side with fewer than four copies a wave
+    // makes some of them twice); dwords past the last are read as the last.
     auto fetch_scales = [&](uint32_t v, uint32_t q) __attribute__((always_inline)) {
         const uint32_t to = base + kScales + (v & 1u) * kWindow;
+        constexpr uint32_t QA = (RA + 3) / 4, QB = (RB + 3) / 4;
 #pragma unroll
-        for (uint32_t j = 0; j < (RA > RB ? RA : RB); j++) {
-            if ((j & 3u) != q) continue;
-            const uint32_t c = wave + NW * j;
+        for (uint32_t u = 0; u < QA; u++) {
+            const uint32_t i = (q * QA + u) % RA, c = wave + NW * i;
             const uint32_t at = 4u * min(8 * v + ((lane & 7u) ^ (c & 7u)), sld / 4 - 1);
-            if (j < RA) {
-                if constexpr (GATHER)
-                    copy4(xsp[j] + at, to + c * 256);
-                else
-                    copy4(xs, xso[j] + at, to + c * 256);
+            if constexpr (GATHER) {
+                const uint8_t *g = xsp[0];
+#pragma unroll
+                for (uint32_t j = 1; j < RA; j++) {
+                    const uint64_t d = (uint64_t)xsp[j] - (uint64_t)xsp[j - 1];
+                    g += i >= j ? d : 0;     // sums, not a choice of places: those would be memory
+                }
+                copy4(g + at, to + c * 256);
+            } else {
+                copy4(xs, min(c * 8 + l8, xlast) * sld + at, to + c * 256);
             }
-            if (j < RB) copy4(ws, wso[j] + at, to + BM * 32 + c * 256);
+        }
+#pragma unroll
+        for (uint32_t u = 0; u < QB; u++) {
+            const uint32_t c = wave + NW * ((q * QB + u) % RB);
+            const uint32_t at = 4u * min(8 * v + ((lane & 7u) ^ (c & 7u)), sld / 4 - 1);
+            copy4(ws, min(c * 8 + l8, wlast) * sld + at, to + BM * 32 + c * 256);
         }
     };
-
+    // The last stage, landed: zeros for the activations' blocks past the end.
+    auto clear_tail = [&]() __attribute__((always_inline)) {
+        const uint32_t first = nb & 7u, st = (nk - 1) & 1u;
+        for (uint32_t i = threadIdx.x; i < BM * 8; i += 64 * NW)
+            if (((i & 7u) ^ tile_swz(i >> 3)) >= first)
+                *(u32x4 *)(lds + st * kStage + 16 * i) = (u32x4){0, 0, 0, 0};
+        __syncthreads();
+    };
     const uint32_t wm = wave / WN, wn = wave % WN, lr = lane & 31u, h = lane >> 5;
     const uint32_t ra = wm * FM * 32 + lr, rb = wn * FN * 32 + lr;
     uint32_t off[4];
@@ -355,88 +372,144 @@ __device__ inline void tile(const MulArgs &a, const uint8_t *w, const uint8_t *w
 #pragma unroll
             for (uint32_t q = 0; q < 16; q++) acc[i][j][q] = 0.f;
 
-    auto work = [&](uint32_t k, auto tail) __attribute__((always_inline)) {
-        const uint8_t *st = lds + (k & 1u) * kStage;
-        const uint8_t *xa = st + ra * 128, *wb = st + (BM + rb) * 128;
+    // scales of stage k, a dword a fragment; 1 past the row's end, where the
+    // bytes may say NaN
+    auto read_scales = [&](uint32_t k, uint32_t *sx, uint32_t *sw) __attribute__((always_inline)) {
         const uint8_t *sc = lds + kScales + ((k >> 2) & 1u) * kWindow;
         const uint32_t d = 2 * (k & 3u) + h;
-        uint32_t sx[FM], sw[FN];
-#pragma unroll
-        for (uint32_t i = 0; i < FM; i++) {
-            const uint32_t row = ra + 32 * i;
-            sx[i] = *(const uint32_t *)(sc + row * 32 + 4 * (d ^ ((row >> 3) & 7u)));
-        }
-#pragma unroll
-        for (uint32_t j = 0; j < FN; j++) {
-            const uint32_t row = rb + 32 * j;
-            sw[j] = *(const uint32_t *)(sc + (BM + row) * 32 + 4 * (d ^ ((row >> 3) & 7u)));
-        }
-        auto step = [&](auto s_) __attribute__((always_inline)) {
-            constexpr uint32_t s = decltype(s_)::value;
-            u32x4 xq[FM], wq[FN];
-#pragma unroll
-            for (uint32_t i = 0; i < FM; i++) xq[i] = *(const u32x4 *)(xa + i * 4096 + off[s]);
-#pragma unroll
-            for (uint32_t j = 0; j < FN; j++) wq[j] = *(const u32x4 *)(wb + j * 4096 + off[s]);
-            if constexpr (decltype(tail)::value) {
-                // blocks past the row's end: codes 0 on one side, scale 1 on both
-                const bool none = 8 * k + 4 * h + s >= nb;
-                const uint32_t clear = 255u << (8 * s), one = 127u << (8 * s);
-#pragma unroll
-                for (uint32_t i = 0; i < FM; i++) {
-                    xq[i] = none ? (u32x4){0, 0, 0, 0} : xq[i];
-                    sx[i] = none ? (sx[i] & ~clear) | one : sx[i];
-                }
-#pragma unroll
-                for (uint32_t j = 0; j < FN; j++) sw[j] = none ? (sw[j] & ~clear) | one : sw[j];
-            }
-#pragma unroll
-            for (uint32_t i = 0; i < FM; i++)
-#pragma unroll
-                for (uint32_t j = 0; j < FN; j++)
-                    acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(
-                        widen(wq[j]), widen(xq[i]), acc[i][j], 4, 4, s, (int)sw[j], s, (int)sx[i]);
+        const int32_t left = (int32_t)(nb - (8 * k + 4 * h));      // blocks of this lane's four
+        const uint32_t in = left >= 4 ? ~0u : left <= 0 ? 0u : (1u << (8 * left)) - 1;
+        auto one = [&](uint32_t row, uint32_t r) __attribute__((always_inline)) {
+            const uint32_t v = *(const uint32_t *)(sc + row * 32 + 4 * (d ^ ((r >> 3) & 7u)));
+            return (v & in) | (0x7f7f7f7fu & ~in);
         };
-        step(std::integral_constant<uint32_t, 0>());
-        step(std::integral_constant<uint32_t, 1>());
-        step(std::integral_constant<uint32_t, 2>());
-        step(std::integral_constant<uint32_t, 3>());
+#pragma unroll
+        for (uint32_t i = 0; i < FM; i++) sx[i] = one(ra + 32 * i, ra + 32 * i);
+#pragma unroll
+        for (uint32_t j = 0; j < FN; j++) sw[j] = one(BM + rb + 32 * j, rb + 32 * j);
+    };
+    auto read_codes = [&](uint32_t k, uint32_t s, u32x4 *xq, u32x4 *wq) __attribute__((always_inline)) {
+        const uint8_t *st = lds + (k & 1u) * kStage + off[s];
+#pragma unroll
+        for (uint32_t i = 0; i < FM; i++) xq[i] = *(const u32x4 *)(st + (ra + 32 * i) * 128);
+#pragma unroll
+        for (uint32_t j = 0; j < FN; j++) wq[j] = *(const u32x4 *)(st + (BM + rb + 32 * j) * 128);
+    };
+    auto multiply = [&](auto s_, uint32_t i, const u32x4 *xq, const u32x4 *wq, const uint32_t *sx,
+                        const uint32_t *sw) __attribute__((always_inline)) {
+        constexpr uint32_t s = decltype(s_)::value;
+#pragma unroll
+        for (uint32_t j = 0; j < FN; j++)
+            acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(
+                widen(wq[j]), widen(xq[i]), acc[i][j], 4, 4, s, (int)sw[j], s, (int)sx[i]);
+    };
+
+    // Barrier t says that stage t has landed and that stage t - 1 is read.  It
+    // stands before the last products of stage t - 1, whose operands are in
+    // registers: they cover the first reads of stage t, and stage t + 1's
+    // copies have a whole stage of products to land.  The scheduling barriers
+    // keep the reads one step ahead of the products, no further.
+    u32x4 xa[FM], wa[FN], xb[FM], wb[FN];
+    uint32_t sx[FM], sw[FN], nx[FM], nw[FN];
+    const std::integral_constant<uint32_t, 0> s0{};
+    const std::integral_constant<uint32_t, 1> s1{};
+    const std::integral_constant<uint32_t, 2> s2{};
+    const std::integral_constant<uint32_t, 3> s3{};
+    auto all = [&](auto s_, const u32x4 *xq, const u32x4 *wq) __attribute__((always_inline)) {
+#pragma unroll
+        for (uint32_t i = 0; i < FM; i++) multiply(s_, i, xq, wq, sx, sw);
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    auto three = [&](uint32_t k) __attribute__((always_inline)) {
+        read_codes(k, 1, xb, wb);
+        all(s0, xa, wa);
+        read_codes(k, 2, xa, wa);
+        all(s1, xb, wb);
+        read_codes(k, 3, xb, wb);
+        all(s2, xa, wa);
+    };
+    auto next = [&]() __attribute__((always_inline)) {
+#pragma unroll
+        for (uint32_t i = 0; i < FM; i++) sx[i] = nx[i];
+#pragma unroll
+        for (uint32_t j = 0; j < FN; j++) sw[j] = nw[j];
     };
 
 #pragma unroll
     for (uint32_t q = 0; q < 4; q++) fetch_scales(0, q);
-    fetch(0);
-    uint32_t k = 0;
-    for (; k + 1 < nk; k++) {
-        // after the barrier nobody reads what stage k - 1 and, for k = 4v, window v - 1 held
-        stage_barrier();
-        fetch(k + 1);
-        if ((k | 3u) + 1 < nk) fetch_scales((k >> 2) + 1, k & 3u);
-        work(k, std::false_type());
-    }
+#pragma unroll
+    for (uint32_t i = 0; i < FM; i++) fetch(0, i);
     stage_barrier();
-    work(k, std::true_type());
+    if (1 < nk) {
+#pragma unroll
+        for (uint32_t i = 0; i < FM; i++) fetch(1, i);
+        fetch_scales(1, 0);
+    } else if (nb & 7u) {
+        clear_tail();
+    }
+    read_scales(0, sx, sw);
+    read_codes(0, 0, xa, wa);
+    uint32_t k = 0;
+    for (; k + 2 < nk; k++) {
+        three(k);
+        stage_barrier();
+        read_scales(k + 1, nx, nw);
+        read_codes(k + 1, 0, xa, wa);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (uint32_t i = 0; i < FM; i++) {
+            multiply(s3, i, xb, wb, sx, sw);
+            fetch(k + 2, i);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        fetch_scales(((k + 1) >> 2) + 1, (k + 1) & 3u);
+        next();
+    }
+    if (k + 1 < nk) {
+        three(k);
+        stage_barrier();
+        if (nb & 7u) clear_tail();
+        read_scales(k + 1, nx, nw);
+        read_codes(k + 1, 0, xa, wa);
+        all(s3, xb, wb);
+        next();
+        k++;
+    }
+    three(k);
+    all(s3, xb, wb);
 
-    // lane: activation row lr of its fragment, weight rows 8q + 4h + 0..3
+    // Sums of 32 activation rows at a time through LDS (the stages are read),
+    // so that a wave stores whole stretches of an output row: lane (row lr, h)
+    // holds weight rows 8q + 4h + 0..3 of its fragments.
+    constexpr uint32_t kRow = FN * 32 + 4, kLanes = FN * 8;   // floats a row, lanes that store one
+    static_assert(NW * 32 * kRow * 4 <= tile_lds<BM, BN>(), "sums fit the stages");
+    float *sums = (float *)lds + wave * 32 * kRow;
+    const uint64_t rw = r0 + wn * FN * 32 + lane % kLanes * 4;   // weight row of this lane's stores
+    __syncthreads();
 #pragma unroll
     for (uint32_t i = 0; i < FM; i++) {
-        const int64_t p = p0 + ra + 32 * i;
-        if (p >= phi) continue;
-        if (GATHER && (a.act[p] < 0 || (int64_t)a.act[p] >= (int64_t)a.xrows)) continue;
 #pragma unroll
         for (uint32_t j = 0; j < FN; j++)
 #pragma unroll
-            for (uint32_t q = 0; q < 4; q++) {
-                const uint64_t r = r0 + wn * FN * 32 + 32 * j + 8 * q + 4 * h;
-                const v4f v = {acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2],
-                               acc[i][j][4 * q + 3]};
-                const uint64_t at = p * a.ldy + r;
-                if (a.y_wide && r + 4 <= a.w_rows)
-                    store4(a.y, a.y_type, at, v);
-                else
-                    for (uint32_t n = 0; n < 4; n++)
-                        if (r + n < a.w_rows) store_from_f32(a.y, a.y_type, at + n, v[n]);
-            }
+            for (uint32_t q = 0; q < 4; q++)
+                *(v4f *)(sums + lr * kRow + 32 * j + 8 * q + 4 * h) =
+                    (v4f){acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2],
+                          acc[i][j][4 * q + 3]};
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll 1
+        for (uint32_t m = lane / kLanes; m < 32; m += 64 / kLanes) {
+            const int64_t p = p0 + (wm * FM + i) * 32 + m;
+            if (p >= phi) break;
+            if (GATHER && (a.act[p] < 0 || (int64_t)a.act[p] >= (int64_t)a.xrows)) continue;
+            const v4f v = *(const v4f *)(sums + m * kRow + lane % kLanes * 4);
+            const uint64_t at = p * a.ldy + rw;
+            if (a.y_wide && rw + 4 <= a.w_rows)
+                store4(a.y, a.y_type, at, v);
+            else
+                for (uint32_t n = 0; n < 4; n++)
+                    if (rw + n < a.w_rows) store_from_f32(a.y, a.y_type, at + n, v[n]);
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     }
 }
 
