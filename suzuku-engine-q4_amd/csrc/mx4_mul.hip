@@ -6,12 +6,6 @@
 
 #include "mx4.h"
 #include "q4mi_internal.h"
-#ifndef MX4_L
-#define MX4_L 2, 4, 2
-#endif
-#ifndef MX4_I
-#define MX4_I 64, 128, 1, 4, 2
-#endif
 
 using namespace q4mi;
 
@@ -31,8 +25,8 @@ struct MulArgs {
     void *y;
     uint64_t w_rows, cols, w_stride, ws_stride, ldx, xrows, n, ldy;
     uint32_t n_expert, x_type, y_type, x_div;
-    uint32_t ks, seg, blocks;       // few rows: waves a tile, blocks of K in LDS, workgroups
-    uint32_t m_tiles, n_tiles, zs;  // tiles: along the activations and weights, shares of a slice
+    uint32_t ks, seg, blocks;       // waves a tile, blocks of K in LDS, workgroups along the weights
+    uint32_t m_tiles, parts;        // tiles along the activations; shares of an expert's weight rows
     bool x_wide, y_wide;            // whether rows can move 16 bytes at a time
 };
 
@@ -54,78 +48,104 @@ __device__ inline void store4(void *y, uint32_t yt, uint64_t at, v4f v) {
 
 // ---------------------------------------------------------------- few rows
 //
-// Up to 16 activation rows against all weight rows: bound by reading the
-// weights once.  A wave takes 16 weight rows; lane (m, g) of it holds row m's
-// blocks 4s + g of a chunk of 16 blocks (s = 0..3), so four lanes read 64
-// adjacent bytes and a chunk's 16 scales are one 16-byte load, of which step s
-// uses byte g of dword s.  PF chunks (4 KB each with 16 rows) are in flight a
-// wave.  The activation rows sit in LDS, as codes: float rows are quantised on
-// the way there, once a workgroup.  KS waves share a tile along K and their
-// sums are joined in LDS in wave order, so a short matrix still occupies the
-// chip; the workgroups are persistent, so a tall one pays the LDS fill once.
+// Up to 16 * MT activation rows against all weight rows: bound by reading the
+// weights once.  A wave takes 16 weight rows straight from memory into
+// registers; lane (m, g) of it holds row m's blocks 4s + g of a chunk of 16
+// blocks (s = 0..3), so four lanes read 64 adjacent bytes and a chunk's 16
+// scales are one 16-byte load, of which step s uses byte g of dword s.  PF
+// chunks (4 KB each with 16 rows) are in flight a wave.  The activation rows
+// sit in LDS, as codes, in groups of 16 for one instruction each: float rows
+// are quantised on the way there, once a workgroup.  ks waves share a tile
+// along K and their sums are joined in LDS in wave order, so a short matrix
+// still occupies the chip; a workgroup goes over several tiles, so a tall one
+// pays the LDS fill once.
 
-constexpr uint32_t kFewWaves = 4;
-constexpr uint32_t kFewRows = 16;
-
-// Blocks of a K segment held in LDS at once (36 KB at 8 or 16 rows).
-__host__ __device__ inline uint32_t few_segment(uint32_t rows) { return rows > 8 ? 128u : 256u; }
-// LDS strides of a row's codes and scales: 16 bytes more than a power of two,
-// so the rows of a fragment start in different banks.
+// LDS strides of a row's codes and scales, seg blocks: 16 bytes more than a
+// power of two, so that the rows of a fragment start in different banks.
 __host__ __device__ inline uint32_t few_code_ld(uint32_t seg) { return seg * 16u + 16u; }
 __host__ __device__ inline uint32_t few_scale_ld(uint32_t seg) { return seg + 16u; }
 
-// Blocks [b0, b0 + seg) of `rows` activation rows from x row xr0 into LDS;
-// blocks from nb on get codes 0 and scale 1.
-__device__ inline void few_stage(const MulArgs &a, uint64_t xr0, uint32_t rows, uint32_t b0,
-                                 uint32_t seg, uint32_t nb, uint32_t sld, uint8_t *codes,
-                                 uint8_t *scales) {
+// The activation rows of a workgroup: `rows` packed rows from p0 on.
+struct FewRange {
+    uint64_t p0;
+    uint32_t rows, x_div;
+    const int32_t *act;      // their activation rows; NULL: p / x_div
+    __device__ int64_t x_row(uint32_t t, uint64_t xrows) const {
+        if (!act) return (int64_t)((p0 + t) / x_div);
+        const int64_t r = act[p0 + t];
+        return r < (int64_t)xrows ? r : -1;
+    }
+};
+
+// Blocks [b0, b0 + seg) of the rows into LDS; blocks from nb on get codes 0
+// and scale 1.
+template <uint32_t NW, bool FLOATS>
+__device__ inline void few_stage(const MulArgs &a, const FewRange &f, uint32_t b0, uint32_t seg,
+                                 uint32_t nb, uint32_t sld, uint8_t *codes, uint8_t *scales) {
     const uint32_t cld = few_code_ld(seg), scld = few_scale_ld(seg);
-    for (uint32_t i = threadIdx.x; i < rows * seg * 4; i += kFewWaves * 64) {
-        const uint32_t sub = i & 3u, q = i >> 2, b = q & (seg - 1), t = q / seg;
-        const uint64_t xr = xr0 + t;
-        const uint32_t bb = b0 + b;
-        uint32_t code = 0, s = 127;
-        if (bb < nb) {
-            if (a.x_type == kTypeMx4) {
-                code = *(const uint32_t *)((const uint8_t *)a.x + xr * (16ull * nb) + 16u * bb +
-                                           4u * sub);
-                s = a.xs[xr * sld + bb];
-            } else {
-                const uint32_t c0 = 32u * bb + 8u * sub;
-                float v[8];
-                load_row8(a.x, a.x_type, xr * a.ldx, c0, (uint32_t)a.cols, a.x_wide, v);
-                code = mx4_quant8(v, &s);
+    if (!FLOATS || a.x_type == kTypeMx4) {
+        const uint32_t lane = threadIdx.x & 63u;
+#pragma unroll 2
+        for (uint32_t t = threadIdx.x >> 6; t < f.rows; t += NW) {
+            const uint64_t xr = (uint64_t)max(f.x_row(t, a.xrows), (int64_t)0);
+            const u32x4 *c = (const u32x4 *)((const uint8_t *)a.x + xr * (16ull * nb));
+            const uint32_t *s = (const uint32_t *)(a.xs + xr * sld);
+            for (uint32_t b = lane; b < seg; b += 64)
+                *(u32x4 *)(codes + t * cld + 16u * b) =
+                    b0 + b < nb ? c[b0 + b] : (u32x4){0, 0, 0, 0};
+            for (uint32_t d = lane; d < seg / 4; d += 64) {
+                const int32_t left = (int32_t)(nb - (b0 + 4 * d));
+                const uint32_t in = left >= 4 ? ~0u : left <= 0 ? 0u : (1u << (8 * left)) - 1;
+                const uint32_t v = left > 0 ? s[b0 / 4 + d] : 0u;
+                *(uint32_t *)(scales + t * scld + 4u * d) = (v & in) | (0x7f7f7f7fu & ~in);
             }
+        }
+        return;
+    }
+    for (uint32_t i = threadIdx.x; i < f.rows * seg * 4; i += NW * 64) {
+        const uint32_t sub = i & 3u, q = i >> 2, t = q / seg, b = q - t * seg;
+        uint32_t code = 0, s = 127;
+        if (b0 + b < nb) {
+            float v[8];
+            load_row8(a.x, a.x_type, (uint64_t)f.x_row(t, a.xrows) * a.ldx,
+                      32u * (b0 + b) + 8u * sub, (uint32_t)a.cols, a.x_wide, v);
+            code = mx4_quant8(v, &s);
         }
         *(uint32_t *)(codes + t * cld + 16u * b + 4u * sub) = code;
         if (sub == 0) scales[t * scld + b] = (uint8_t)s;
     }
 }
 
-// FULL: rows are whole chunks of 16 blocks.  a.y row of activation row t is
-// y0 + t.
-template <bool FULL, uint32_t PF>
+// FULL: rows are whole chunks of 16 blocks.  Workgroup `block` of `blocks`
+// takes every blocks-th set of weight tiles.
+template <bool FULL, uint32_t PF, uint32_t MT, uint32_t NW, bool FLOATS>
 __device__ inline void few_rows(const MulArgs &a, const uint8_t *w, const uint8_t *ws,
-                                uint64_t xr0, uint32_t rows, uint64_t y0, uint32_t block,
-                                uint32_t blocks, uint8_t *lds) {
-    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
+                                const FewRange &f, uint32_t block, uint32_t blocks, uint8_t *lds) {
+    const uint32_t lane = threadIdx.x & 63u;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t m = lane & 15u, g = lane >> 4;
-    const uint32_t ks = a.ks, kw = wave & (ks - 1), sub = wave / ks, per = kFewWaves / ks;
+    const uint32_t ks = a.ks, kw = wave & (ks - 1), sub = wave / ks, per = NW / ks;
     const uint32_t nb = mx4_blocks(a.cols), sld = mx4_scale_row(nb);
     const uint32_t seg = a.seg, nseg = (nb + seg - 1) / seg;
     const uint32_t cld = few_code_ld(seg), scld = few_scale_ld(seg);
-    uint8_t *codes = lds, *scales = lds + rows * cld;
-    v4f *red = (v4f *)(scales + rows * scld);
+    uint8_t *codes = lds, *scales = lds + f.rows * cld;
+    v4f *red = (v4f *)(scales + f.rows * scld);
     const uint32_t tiles = (uint32_t)((a.w_rows + 15) / 16);
-    const uint32_t t = min(m, rows - 1);
-    const uint8_t *xc = codes + t * cld + 16u * g, *xsc = scales + t * scld;
+    uint32_t xc[MT], xsc[MT];       // this lane's row of every group, in codes and scales
+#pragma unroll
+    for (uint32_t n = 0; n < MT; n++) {
+        const uint32_t t = min(16 * n + m, f.rows - 1);
+        xc[n] = t * cld + 16u * g, xsc[n] = t * scld;
+    }
     const uint32_t rounds = (tiles + per * blocks - 1) / (per * blocks);
     for (uint32_t i = 0; i < rounds; i++) {
         const uint32_t tile = (i * blocks + block) * per + sub;
         const bool mine = tile < tiles;
         const uint64_t wr = min((uint64_t)(mine ? tile : 0u) * 16 + m, a.w_rows - 1);
         const uint8_t *wp = w + wr * (16ull * nb), *wsp = ws + wr * sld;
-        v4f acc = {0.f, 0.f, 0.f, 0.f};
+        v4f acc[MT];
+#pragma unroll
+        for (uint32_t n = 0; n < MT; n++) acc[n] = (v4f){0.f, 0.f, 0.f, 0.f};
         for (uint32_t sg = 0; sg < nseg; sg++) {
             const uint32_t b0 = sg * seg, nch = (min(seg, nb - b0) + 15) / 16;
             // the first batch is on its way while the activations are staged
@@ -148,61 +168,94 @@ __device__ inline void few_rows(const MulArgs &a, const uint8_t *w, const uint8_
             load();
             if (nseg > 1 || i == 0) {
                 if (nseg > 1) __syncthreads();
-                few_stage(a, xr0, rows, b0, seg, nb, sld, codes, scales);
+                few_stage<NW, FLOATS>(a, f, b0, seg, nb, sld, codes, scales);
                 __syncthreads();
             }
+            auto chunk = [&](uint32_t j, uint32_t c) __attribute__((always_inline)) {
+                u32x4 xv[MT];
+#pragma unroll
+                for (uint32_t n = 0; n < MT; n++)
+                    xv[n] = *(const u32x4 *)(scales + xsc[n] + 16u * c);
+#pragma unroll
+                for (uint32_t s = 0; s < 4; s++) {
+                    uint32_t wb = wv[j][s] >> (8 * g);
+                    if (!FULL && b0 + 16 * c + 4 * s + g >= nb) wb = 127;
+#pragma unroll
+                    for (uint32_t n = 0; n < MT; n++) {
+                        const u32x4 xq = *(const u32x4 *)(codes + xc[n] + 256u * c + 64u * s);
+                        acc[n] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
+                            widen(wq[j][s]), widen(xq), acc[n], 4, 4, 0, (int)wb, 0,
+                            (int)(xv[n][s] >> (8 * g)));
+                    }
+                    if (MT > 1) __builtin_amdgcn_sched_barrier(0);   // registers: one step's reads
+                }
+            };
             for (; c0 < nch; c0 += PF * ks) {
                 if (c0 != kw) load();
 #pragma unroll
                 for (uint32_t j = 0; j < PF; j++) {
                     const uint32_t c = c0 + j * ks;
                     if (c >= nch) break;
-                    const u32x4 xv = *(const u32x4 *)(xsc + 16u * c);
-#pragma unroll
-                    for (uint32_t s = 0; s < 4; s++) {
-                        const u32x4 xq = *(const u32x4 *)(xc + 256u * c + 64u * s);
-                        uint32_t wb = wv[j][s] >> (8 * g);
-                        if (!FULL && b0 + 16 * c + 4 * s + g >= nb) wb = 127;
-                        acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
-                            widen(wq[j][s]), widen(xq), acc, 4, 4, 0, (int)wb, 0,
-                            (int)(xv[s] >> (8 * g)));
-                    }
+                    chunk(j, c);
                 }
             }
         }
         if (ks > 1) {
             if (i) __syncthreads();   // the last round's sums have been read
-            red[wave * 64 + lane] = acc;
+#pragma unroll
+            for (uint32_t n = 0; n < MT; n++) red[(wave * MT + n) * 64 + lane] = acc[n];
             __syncthreads();
             if (kw) continue;
-            for (uint32_t k = 1; k < ks; k++) acc += red[(wave + k) * 64 + lane];
+            for (uint32_t k = 1; k < ks; k++)
+#pragma unroll
+                for (uint32_t n = 0; n < MT; n++) acc[n] += red[((wave + k) * MT + n) * 64 + lane];
         }
-        if (!mine || m >= rows) continue;
-        const uint64_t r = (uint64_t)tile * 16 + 4 * g, at = (y0 + m) * a.ldy + r;
-        if (a.y_wide && r + 4 <= a.w_rows)
-            store4(a.y, a.y_type, at, acc);
-        else
-            for (uint32_t k = 0; k < 4; k++)
-                if (r + k < a.w_rows) store_from_f32(a.y, a.y_type, at + k, acc[k]);
+        if (!mine) continue;
+        const uint64_t r = (uint64_t)tile * 16 + 4 * g;
+#pragma unroll
+        for (uint32_t n = 0; n < MT; n++) {
+            const uint32_t t = 16 * n + m;
+            if (t >= f.rows || f.x_row(t, a.xrows) < 0) continue;
+            const uint64_t at = (f.p0 + t) * a.ldy + r;
+            if (a.y_wide && r + 4 <= a.w_rows)
+                store4(a.y, a.y_type, at, acc[n]);
+            else
+                for (uint32_t k = 0; k < 4; k++)
+                    if (r + k < a.w_rows) store_from_f32(a.y, a.y_type, at + k, acc[n][k]);
+        }
     }
 }
 
-// n <= 16 activation rows; `blocks` workgroups share the weight rows.
-template <bool FULL, uint32_t PF>
-__global__ __launch_bounds__(256) void mx4_few_k(MulArgs a) {
+// Sets of up to 16 * MT rows, by how many groups are there.
+template <bool FULL, uint32_t PF, uint32_t MT, uint32_t NW>
+__device__ inline void few_groups(const MulArgs &a, const uint8_t *w, const uint8_t *ws,
+                                  const FewRange &f, uint32_t block, uint32_t blocks,
+                                  uint8_t *lds) {
+    static_assert(MT <= 2, "one or two groups");
+    if (MT == 1 || f.rows <= 16)
+        few_rows<FULL, PF, 1, NW, MT == 1>(a, w, ws, f, block, blocks, lds);
+    else
+        few_rows<FULL, PF, MT, NW, false>(a, w, ws, f, block, blocks, lds);
+}
+
+// Dense: grid (blocks, sets of 16 * MT activation rows).
+template <bool FULL, uint32_t PF, uint32_t MT, uint32_t NW>
+__global__ __launch_bounds__(64 * NW, MT > 1 ? 4 : 1) void mx4_few_k(MulArgs a) {
     extern __shared__ __align__(16) uint8_t lds[];
-    few_rows<FULL, PF>(a, a.w, a.ws, 0, (uint32_t)a.n, 0, blockIdx.x, a.blocks, lds);
+    const uint64_t p0 = (uint64_t)blockIdx.y * 16 * MT;
+    const FewRange f = {p0, (uint32_t)min((uint64_t)16 * MT, a.n - p0), 1, nullptr};
+    few_groups<FULL, PF, MT, NW>(a, a.w, a.ws, f, blockIdx.x, a.blocks, lds);
 }
 
 // Row p through the expert that the list names; grid (blocks, rows).
-template <bool FULL, uint32_t PF>
-__global__ __launch_bounds__(256) void mx4_sel_k(MulArgs a) {
+template <bool FULL, uint32_t PF, uint32_t MT, uint32_t NW>
+__global__ __launch_bounds__(64 * NW) void mx4_sel_k(MulArgs a) {
     extern __shared__ __align__(16) uint8_t lds[];
-    const uint32_t p = blockIdx.y;
-    const int32_t e = a.eid[p];
+    const int32_t e = a.eid[blockIdx.y];
     if (e < 0 || (uint32_t)e >= a.n_expert) return;
-    few_rows<FULL, PF>(a, a.w + e * a.w_stride, a.ws + e * a.ws_stride, p / a.x_div, 1, p,
-                       blockIdx.x, a.blocks, lds);
+    const FewRange f = {blockIdx.y, 1, a.x_div, nullptr};
+    few_groups<FULL, PF, MT, NW>(a, a.w + e * a.w_stride, a.ws + e * a.ws_stride, f, blockIdx.x,
+                               a.blocks, lds);
 }
 
 // ------------------------------------------------------------ rows in tiles
@@ -286,7 +339,7 @@ __device__ inline void tile(const MulArgs &a, const uint8_t *w, const uint8_t *w
     const uint32_t xlast = (uint32_t)min((int64_t)BM, phi - p0) - 1;
     const uint32_t wlast = (uint32_t)min((uint64_t)BN, a.w_rows - r0) - 1;
     auto gathered = [&](uint32_t m) -> uint64_t {
-        const int64_t r = a.act[p0 + m];
+        const int64_t r = a.act ? (int64_t)a.act[p0 + m] : p0 + m;
         return r < 0 || r >= (int64_t)a.xrows ? 0 : (uint64_t)r;
     };
 #pragma unroll
@@ -500,7 +553,7 @@ __device__ inline void tile(const MulArgs &a, const uint8_t *w, const uint8_t *w
         for (uint32_t m = lane / kLanes; m < 32; m += 64 / kLanes) {
             const int64_t p = p0 + (wm * FM + i) * 32 + m;
             if (p >= phi) break;
-            if (GATHER && (a.act[p] < 0 || (int64_t)a.act[p] >= (int64_t)a.xrows)) continue;
+            if (GATHER && a.act && (a.act[p] < 0 || (int64_t)a.act[p] >= (int64_t)a.xrows)) continue;
             const v4f v = *(const v4f *)(sums + m * kRow + lane % kLanes * 4);
             const uint64_t at = p * a.ldy + rw;
             if (a.y_wide && rw + 4 <= a.w_rows)
@@ -531,55 +584,102 @@ __global__ __launch_bounds__(64 * WM * WN, WAVES) void mx4_dense_k(MulArgs a) {
     tile<BM, BN, WM, WN, false>(a, a.w, a.ws, (uint64_t)nt * BN, (int64_t)mt * BM, (int64_t)a.n, lds);
 }
 
-// Packed rows: a workgroup takes one BN-row slice of one expert and every
-// zs-th BM-row tile of its stretch; the zs workgroups of a slice are 8 apart,
-// on one die.  No tile list: an expert without rows costs an empty workgroup.
-template <uint32_t BM, uint32_t BN, uint32_t WM, uint32_t WN, uint32_t WAVES>
-__global__ __launch_bounds__(64 * WM * WN, WAVES) void mx4_id_k(MulArgs a) {
-    extern __shared__ __align__(16) uint8_t lds[];
-    const uint32_t u = blockIdx.x / (8 * a.zs), v = blockIdx.x - u * 8 * a.zs;
-    const uint32_t slice = u * 8 + (v & 7u), z = v >> 3;
-    const uint32_t e = slice / a.n_tiles, nt = slice - e * a.n_tiles;
-    if (e >= a.n_expert) return;
-    // without a row list, packed row p is activation row p: those past xrows do not exist
-    const int64_t rows = (int64_t)(a.act ? a.n : min(a.n, a.xrows));
-    const int64_t lo = max(a.bounds[e], 0), hi = min((int64_t)a.bounds[e + 1], rows);
-    const uint8_t *w = a.w + e * a.w_stride, *ws = a.ws + e * a.ws_stride;
-    for (int64_t p0 = lo + (int64_t)z * BM; p0 < hi; p0 += (int64_t)a.zs * BM) {
-        if (a.act)
-            tile<BM, BN, WM, WN, true>(a, w, ws, (uint64_t)nt * BN, p0, hi, lds);
-        else
-            tile<BM, BN, WM, WN, false>(a, w, ws, (uint64_t)nt * BN, p0, hi, lds);
-        __syncthreads();   // the next tile's copies overwrite what slower waves may still read
+// ------------------------------------------------------------- packed rows
+//
+// Experts differ: of a prompt's, a few take most of the rows and many take a
+// handful.  One persistent workgroup a CU goes over a list of items: first
+// tiles of kIdM rows x kIdN weight rows of the experts with more than kIdFew
+// rows (bound by the matrix units), then weight-row shares of the others,
+// whose weights are streamed once past all of their rows (bound by memory).
+// Every workgroup makes the list by itself, as prefix sums over the experts'
+// stretches in LDS: no scratch in memory, no launch before, and no workgroups
+// that find nothing to do.
+constexpr uint32_t kIdM = 128, kIdN = 256, kIdWM = 2, kIdWN = 4, kIdWaves = kIdWM * kIdWN;
+constexpr uint32_t kIdFew = 32, kIdExperts = 1024;
+constexpr size_t kIdLists = 2 * (kIdExperts + 1) * 4;
+
+// Inclusive sums over a workgroup's threads.
+__device__ inline uint2 block_sums(uint2 v, uint32_t *tmp) {
+    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
+#pragma unroll
+    for (uint32_t d = 1; d < 64; d *= 2) {
+        const uint32_t x = __shfl_up(v.x, d, 64), y = __shfl_up(v.y, d, 64);
+        if (lane >= d) v.x += x, v.y += y;
     }
+    if (lane == 63) tmp[2 * wave] = v.x, tmp[2 * wave + 1] = v.y;
+    __syncthreads();
+    for (uint32_t w = 0; w < wave; w++) v.x += tmp[2 * w], v.y += tmp[2 * w + 1];
+    __syncthreads();
+    return v;
 }
 
-// Launch shape of the few-rows kernels for `rows` activation rows a workgroup
-// and `lists` independent products.
-struct FewPlan {
-    uint32_t ks, pf, blocks;
-    size_t lds;
-};
-FewPlan few_plan(MulArgs &a, uint32_t rows, uint32_t lists) {
-    const uint32_t nb = mx4_blocks(a.cols), tiles = (uint32_t)((a.w_rows + 15) / 16);
-    const uint32_t cus = (uint32_t)cu_count();
-    uint32_t seg = few_segment(rows);
-    while (seg > 16 && seg / 2 >= nb) seg /= 2;
-    const uint32_t nch = (std::min(seg, nb) + 15) / 16;
-    FewPlan p;
-    p.ks = 1;
-    while (p.ks < kFewWaves && p.ks * 2 <= nch && (uint64_t)tiles * lists * p.ks < 8ull * cus)
-        p.ks *= 2;
-    const uint32_t mine = (nch + p.ks - 1) / p.ks;
-    p.pf = mine >= 4 ? 4 : mine >= 2 ? 2 : 1;
-    const uint32_t per = kFewWaves / p.ks;
-    p.blocks = std::min((tiles + per - 1) / per, std::max(1u, cus * 4 / std::min(lists, cus * 4)));
-    p.lds = (size_t)rows * (few_code_ld(seg) + few_scale_ld(seg)) +
-            (p.ks > 1 ? kFewWaves * 64 * sizeof(v4f) : 0);
-    a.ks = p.ks, a.seg = seg, a.blocks = p.blocks;
-    a.x_wide = a.x_type != kTypeMx4 && !((uintptr_t)a.x & 15) && a.ldx * type_bytes(a.x_type) % 16 == 0;
-    a.y_wide = !((uintptr_t)a.y & 15) && a.ldy * type_bytes(a.y_type) % 16 == 0;
-    return p;
+// The last e with list[e] <= i, of n + 1 ascending sums.
+__device__ inline uint32_t owner(const uint32_t *list, uint32_t n, uint32_t i) {
+    uint32_t lo = 0, hi = n;
+    while (hi - lo > 1) {
+        const uint32_t mid = (lo + hi) / 2;
+        if (list[mid] <= i)
+            lo = mid;
+        else
+            hi = mid;
+    }
+    return __builtin_amdgcn_readfirstlane(lo);
+}
+
+template <bool FULL>
+__global__ __launch_bounds__(64 * kIdWaves, 2) void mx4_id_k(MulArgs a) {
+    extern __shared__ __align__(16) uint8_t lds[];
+    uint32_t *tiles = (uint32_t *)lds, *shares = tiles + kIdExperts + 1;
+    uint8_t *work = lds + (kIdLists + 15) / 16 * 16;
+    // without a row list, packed row p is activation row p: those past xrows do not exist
+    const int64_t end = (int64_t)(a.act ? a.n : min(a.n, a.xrows));
+    const uint32_t n = a.n_expert;
+    auto stretch = [&](uint32_t e, int64_t *lo) __attribute__((always_inline)) -> int64_t {
+        *lo = max(a.bounds[e], 0);
+        return min((int64_t)a.bounds[e + 1], end) - *lo;
+    };
+    constexpr uint32_t kEach = kIdExperts / (64 * kIdWaves);
+    uint2 mine[kEach], sum = make_uint2(0, 0);
+#pragma unroll
+    for (uint32_t i = 0; i < kEach; i++) {
+        const uint32_t e = threadIdx.x * kEach + i;
+        int64_t lo, rows = e < n ? stretch(e, &lo) : 0;
+        mine[i] = make_uint2(rows > kIdFew ? (uint32_t)((rows + kIdM - 1) / kIdM) : 0u,
+                             rows > 0 && rows <= kIdFew ? 1u : 0u);
+        sum.x += mine[i].x, sum.y += mine[i].y;
+    }
+    uint2 at = block_sums(sum, (uint32_t *)work);
+    at.x -= sum.x, at.y -= sum.y;
+#pragma unroll
+    for (uint32_t i = 0; i < kEach; i++) {
+        const uint32_t e = threadIdx.x * kEach + i;
+        if (e <= n) tiles[e] = at.x, shares[e] = at.y;
+        at.x += mine[i].x, at.y += mine[i].y;
+    }
+    if (n == kIdExperts && threadIdx.x == 64 * kIdWaves - 1) tiles[n] = at.x, shares[n] = at.y;
+    __syncthreads();
+    const uint32_t slices = (uint32_t)((a.w_rows + kIdN - 1) / kIdN);
+    const uint32_t heavy = tiles[n] * slices, all = heavy + shares[n] * a.parts;
+    for (uint32_t i = blockIdx.x; i < all; i += a.blocks) {
+        const bool big = i < heavy;
+        const uint32_t j = big ? i : i - heavy, each = big ? slices : a.parts;
+        const uint32_t unit = j / each, part = j - unit * each;
+        const uint32_t *list = big ? tiles : shares;
+        const uint32_t e = owner(list, n, unit);
+        int64_t lo;
+        const int64_t rows = stretch(e, &lo);
+        const uint8_t *w = a.w + e * a.w_stride, *ws = a.ws + e * a.ws_stride;
+        const int64_t skip = (int64_t)(unit - tiles[e]) * kIdM;
+        if (big) {
+            if (skip < rows)    // always, with bounds that ascend
+                tile<kIdM, kIdN, kIdWM, kIdWN, true>(a, w, ws, (uint64_t)part * kIdN, lo + skip,
+                                                     lo + rows, work);
+        } else {
+            const FewRange f = {(uint64_t)lo, (uint32_t)rows, 1, a.act};
+            few_groups<FULL, 2, kIdFew / 16, kIdWaves>(a, w, ws, f, part, a.parts, work);
+        }
+        __syncthreads();   // the next item overwrites what slower waves may still read
+    }
 }
 
 bool mul_ok(const char *who, const MulArgs &a) {
@@ -615,7 +715,10 @@ bool mul_ok(const char *who, const MulArgs &a) {
     return true;
 }
 
+// Whether float and output rows can move 16 bytes at a time.
 void wide_rows(MulArgs &a) {
+    a.x_wide = is_float_type(a.x_type) && !((uintptr_t)a.x & 15) &&
+               a.ldx * type_bytes(a.x_type) % 16 == 0;
     a.y_wide = !((uintptr_t)a.y & 15) && a.ldy * type_bytes(a.y_type) % 16 == 0;
 }
 
@@ -636,33 +739,133 @@ bool dense_launch(MulArgs &a) {
     return launch_ok("mx4_dense_k");
 }
 
-template <uint32_t BM, uint32_t BN, uint32_t WM, uint32_t WN, uint32_t WAVES>
+// K segment of the few-rows kernels for `rows` activation rows a workgroup of
+// `waves`: whole rows where they fit in `room` bytes, else equal parts of whole
+// chunks; returns the LDS bytes.
+size_t few_fit(MulArgs &a, uint32_t rows, uint32_t groups, uint32_t waves, size_t room) {
+    const uint32_t nb = mx4_blocks(a.cols);
+    uint32_t parts = 1;
+    size_t need;
+    do {
+        a.seg = ((nb + parts - 1) / parts + 15) / 16 * 16;
+        need = (size_t)rows * (few_code_ld(a.seg) + few_scale_ld(a.seg));
+        parts++;
+    } while (need > room && a.seg > 16);
+    return need + (a.ks > 1 ? (size_t)waves * groups * 64 * sizeof(v4f) : 0);
+}
+
+// Waves a weight tile: as many as there are chunks, while the whole launch has
+// fewer than 8 waves a CU.
+uint32_t few_split(const MulArgs &a, uint32_t waves, uint64_t tiles) {
+    const uint32_t chunks = (mx4_blocks(a.cols) + 15) / 16;
+    uint32_t ks = 1;
+    while (ks < waves && ks * 2 <= chunks && tiles * ks < 8ull * cu_count()) ks *= 2;
+    return ks;
+}
+
+// One group: `rows` (<= 16) activation rows a workgroup, `lists` of them.
+template <class F>
+bool few_launch(MulArgs &a, uint32_t rows, uint32_t lists, F pick, const char *name) {
+    constexpr uint32_t NW = 4;
+    const uint64_t tiles = (a.w_rows + 15) / 16;
+    const uint32_t room = 4 * cu_count();
+    a.ks = few_split(a, NW, tiles * lists);
+    const size_t lds = few_fit(a, rows, 1, NW, 40 * 1024);
+    const uint32_t per = NW / a.ks, chunks = (std::min(a.seg, mx4_blocks(a.cols)) + 15) / 16;
+    const uint32_t mine = (chunks + a.ks - 1) / a.ks;
+    a.blocks = (uint32_t)std::min<uint64_t>((tiles + per - 1) / per,
+                                            std::max(1u, room / std::min(lists, room)));
+    wide_rows(a);
+    auto k = pick(mx4_blocks(a.cols) % 16 == 0, mine >= 4 ? 4 : mine >= 2 ? 2 : 1);
+    k<<<dim3(a.blocks, lists), dim3(64 * NW), lds, stream()>>>(a);
+    return launch_ok(name);
+}
+typedef void (*MulKernel)(MulArgs);
+MulKernel few_kernel(bool full, uint32_t pf) {
+    return pf == 4   ? (full ? mx4_few_k<true, 4, 1, 4> : mx4_few_k<false, 4, 1, 4>)
+           : pf == 2 ? (full ? mx4_few_k<true, 2, 1, 4> : mx4_few_k<false, 2, 1, 4>)
+                     : (full ? mx4_few_k<true, 1, 1, 4> : mx4_few_k<false, 1, 1, 4>);
+}
+MulKernel sel_kernel(bool full, uint32_t pf) {
+    return pf == 4   ? (full ? mx4_sel_k<true, 4, 1, 4> : mx4_sel_k<false, 4, 1, 4>)
+           : pf == 2 ? (full ? mx4_sel_k<true, 2, 1, 4> : mx4_sel_k<false, 2, 1, 4>)
+                     : (full ? mx4_sel_k<true, 1, 1, 4> : mx4_sel_k<false, 1, 1, 4>);
+}
+
+// Two groups: 17 to 32 activation rows, eight waves.
+bool few2_launch(MulArgs &a) {
+    constexpr uint32_t NW = 8, MT = 2;
+    const uint64_t tiles = (a.w_rows + 15) / 16;
+    a.ks = few_split(a, NW, tiles);
+    // whole rows up to 5632 columns; longer ones a segment at a time, each tile anew
+    constexpr size_t kRoom = 100 * 1024, kMost = kRoom + NW * MT * 64 * sizeof(v4f);
+    const size_t lds = few_fit(a, (uint32_t)a.n, MT, NW, kRoom);
+    const uint32_t per = NW / a.ks;
+    a.blocks = (uint32_t)std::min<uint64_t>((tiles + per - 1) / per, 2 * cu_count());
+    wide_rows(a);
+    const bool full = mx4_blocks(a.cols) % 16 == 0;
+    auto k = full ? mx4_few_k<true, 2, MT, NW> : mx4_few_k<false, 2, MT, NW>;
+    static DynLds st[2];
+    if (!dyn_lds_ok((const void *)k, lds, kMost, st[full], "mx4_few_k")) return false;
+    k<<<dim3(a.blocks), dim3(64 * NW), lds, stream()>>>(a);
+    return launch_ok("mx4_few_k");
+}
+
+// Which kernel a dense product takes.  A workgroup's time hardly depends on
+// its tile while the chip has room for all of them, so the smallest tile wins
+// that still gives at most two workgroups a CU (64 x 64: two and a half);
+// measured in us, bf16 out (rows x cols, activation rows):
+//   few rows    against 64 x 64:   1024 x 2048, 128: 5.7 / 6.8; 4096 x 4096, 32: 7.6 / 10.1;
+//                                  2560 x 2560, 77: 9.3 / 7.7
+//   two groups  against 64 x 64:   8192 x 8192, 32: 17.3 / 20.2; 64: 22.0 / 20.5
+//   64 x 64     against 64 x 128:  4096 x 4096, 512: 13.6 / 14.1; 1024: 22.0 / 19.8
+//   64 x 128    against 128 x 128: 8192 x 8192, 512: 33.4 / 34.2; 1024: 63.6 / 50.5
+//   128 x 128   against 256 x 256: 8192 x 8192, 1024: 50.5 / 63.8; 2048: 96.8 / 83.3
+// Past that the two largest are compared by their full rounds: 50 us for two
+// 128 x 128 a CU, 83 us for one 256 x 256 (8192 columns).
+bool mul_pick(MulArgs &a) {
+    const uint64_t cus = cu_count();
+    auto tiles = [&](uint64_t bm, uint64_t bn) {
+        return ((a.n + bm - 1) / bm) * ((a.w_rows + bn - 1) / bn);
+    };
+    if (a.n <= 16 || tiles(16, 16) <= 2 * cus)
+        return few_launch(a, (uint32_t)std::min<uint64_t>(a.n, 16), (uint32_t)((a.n + 15) / 16),
+                          few_kernel, "mx4_few_k");
+    if (a.n <= 32) return few2_launch(a);
+    if (2 * tiles(64, 64) <= 5 * cus) return dense_launch<64, 64, 2, 2, 2>(a);
+    if (tiles(64, 128) <= 2 * cus) return dense_launch<64, 128, 1, 4, 2>(a);
+    const uint64_t rounds128 = (tiles(128, 128) + 2 * cus - 1) / (2 * cus);
+    const uint64_t rounds256 = (tiles(256, 256) + cus - 1) / cus;
+    if (3 * rounds128 <= 5 * rounds256) return dense_launch<128, 128, 2, 2, 2>(a);
+    return dense_launch<256, 256, 2, 4, 2>(a);
+}
+
 bool id_launch(MulArgs &a) {
-    static DynLds st;
-    constexpr size_t lds = tile_lds<BM, BN>();
-    auto k = mx4_id_k<BM, BN, WM, WN, WAVES>;
-    if (!dyn_lds_ok((const void *)k, lds, lds, st, "mx4_id_k")) return false;
-    a.n_tiles = (uint32_t)((a.w_rows + BN - 1) / BN);
-    a.zs = 4;
-    const uint64_t slices = ((uint64_t)a.n_tiles * a.n_expert + 7) / 8 * 8;
-    if (slices * a.zs > 0x7fffffffu) {
+    // waves a tile while the experts that can have rows do not fill the chip
+    const uint32_t tiles = (uint32_t)((a.w_rows + 15) / 16);
+    const uint64_t units = std::min<uint64_t>(a.n, a.n_expert) * tiles;
+    a.ks = few_split(a, kIdWaves, units);
+    const size_t few = few_fit(a, kIdFew, kIdFew / 16, kIdWaves, 112 * 1024);
+    const uint32_t per = kIdWaves / a.ks;
+    // two rounds of tiles a share where that leaves every CU several shares
+    const uint32_t rounds = units / (2 * per) >= 4ull * cu_count() ? 2 : 1;
+    a.parts = (tiles + per * rounds - 1) / (per * rounds);
+    const uint64_t slices = (a.w_rows + kIdN - 1) / kIdN;
+    if ((a.n / kIdM + a.n_expert) * slices + (uint64_t)a.n_expert * a.parts > 0x7fffffffu) {
         set_error("q4mi_mx4_mul_id: too many tiles");
         return false;
     }
+    a.blocks = (uint32_t)cu_count();
     wide_rows(a);
-    k<<<dim3((uint32_t)(slices * a.zs)), dim3(64 * WM * WN), lds, stream()>>>(a);
+    constexpr size_t kMost = 160 * 1024;
+    const size_t lds = (kIdLists + 15) / 16 * 16 + std::max(few, (size_t)tile_lds<kIdM, kIdN>());
+    static DynLds st[2];
+    const bool full = mx4_blocks(a.cols) % 16 == 0;
+    auto k = full ? mx4_id_k<true> : mx4_id_k<false>;
+    if (!dyn_lds_ok((const void *)k, lds, kMost, st[full], "mx4_id_k")) return false;
+    k<<<dim3(a.blocks), dim3(64 * kIdWaves), lds, stream()>>>(a);
     return launch_ok("mx4_id_k");
 }
-
-// Launches KERNEL<rows are whole chunks, chunks in flight>.
-#define FEW_LAUNCH(KERNEL, GRID, P, A)                                                     \
-    do {                                                                                   \
-        const bool full = mx4_blocks((A).cols) % 16 == 0;                                  \
-        auto k = (P).pf == 4   ? (full ? KERNEL<true, 4> : KERNEL<false, 4>)               \
-                 : (P).pf == 2 ? (full ? KERNEL<true, 2> : KERNEL<false, 2>)               \
-                               : (full ? KERNEL<true, 1> : KERNEL<false, 1>);              \
-        k<<<GRID, dim3(kFewWaves * 64), (P).lds, stream()>>>(A);                           \
-    } while (0)
 
 constexpr uint64_t kFloatRows = 8;   // float rows that q4mi_mx4_mul takes
 
@@ -685,14 +888,7 @@ bool q4mi_mx4_mul(const uint8_t *d_w, const uint8_t *d_ws, uint64_t w_rows, uint
         return false;
     }
     if (!n) return true;
-    if (n <= kFewRows) {
-        const FewPlan p = few_plan(a, (uint32_t)n, 1);
-        FEW_LAUNCH(mx4_few_k, dim3(p.blocks), p, a);
-        return launch_ok("mx4_few_k");
-    }
-    if (n >= 512 && w_rows >= 512) return dense_launch<256, 256, MX4_L>(a);
-    if (n > 64) return dense_launch<128, 128, 2, 2, 2>(a);
-    return dense_launch<64, 128, 1, 4, 2>(a);
+    return mul_pick(a);
 }
 
 /* Every row through its own expert (see include/q4mi.h). */
@@ -711,9 +907,7 @@ bool q4mi_mx4_mul_sel(const uint8_t *d_w, const uint8_t *d_ws, uint64_t w_rows, 
         return false;
     }
     if (!n) return true;
-    const FewPlan p = few_plan(a, 1, (uint32_t)n);
-    FEW_LAUNCH(mx4_sel_k, dim3(p.blocks, (uint32_t)n), p, a);
-    return launch_ok("mx4_sel_k");
+    return few_launch(a, 1, (uint32_t)n, sel_kernel, "mx4_sel_k");
 }
 
 /* Packed rows, each expert's in one stretch (see include/q4mi.h). */
@@ -728,12 +922,12 @@ bool q4mi_mx4_mul_id(const uint8_t *d_w, const uint8_t *d_ws, uint64_t w_rows, u
     a.x = d_xq, a.xs = d_xs, a.x_type = kTypeMx4, a.xrows = xrows, a.act = d_act_row;
     a.bounds = d_bounds, a.n = total_rows, a.y = d_y, a.y_type = y_type, a.ldy = ld_y;
     if (!mul_ok("q4mi_mx4_mul_id", a)) return false;
-    if (!d_bounds || !n_expert || n_expert > 65535) {
-        set_error("q4mi_mx4_mul_id: needs bounds of 1 to 65535 experts");
+    if (!d_bounds || !n_expert || n_expert > kIdExperts) {
+        set_error("q4mi_mx4_mul_id: needs bounds of 1 to %u experts", kIdExperts);
         return false;
     }
     if (!total_rows || !xrows) return true;
-    return id_launch<MX4_I>(a);
+    return id_launch(a);
 }
 
 }  // extern "C"
