@@ -11,6 +11,9 @@
 // A workgroup owns a slice of one row's vocabulary and counts the history's
 // tokens of that slice in LDS (integer atomics, so their order does not
 // matter): no counters in memory, nothing kept between calls, one launch.
+// Bound by reading and writing the logits once; every slice reads its row's
+// whole history (from the L2), sixteen tokens a thread at a time, while the
+// slice's own logits and mask are on their way to registers.
 #include "mx4.h"
 #include "q4mi_internal.h"
 
@@ -26,86 +29,190 @@ struct LogitsArgs {
     const float *pen, *bias;
     const uint32_t *mask;
     uint64_t ld, ldo, mask_ld;
-    uint32_t type, vocab, n_mask, slices, slice;
+    uint32_t type, vocab, n_mask, slices;
 };
 
+constexpr uint32_t kThreads = 512;
 constexpr uint32_t kPrompt = 0x80000000u;   // counter bit: the token is in the row's prompt
 
-}  // namespace
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef u32x4 u32x4_a4 __attribute__((aligned(4)));   // in memory at any dword
+typedef u32x2 u32x2_a2 __attribute__((aligned(2)));   // at any half word
 
-__global__ __launch_bounds__(256) void logits_k(LogitsArgs a) {
-    extern __shared__ uint32_t lds[];
-    const uint32_t tid = threadIdx.x;
-    const uint32_t b = blockIdx.x / a.slices;
-    const uint32_t v0 = (blockIdx.x % a.slices) * a.slice;
-    const uint32_t nv = min(a.slice, a.vocab - v0);
-    uint32_t *cnt = lds;
-    float *add = (float *)(lds + (a.hist ? a.slice : 0u));
-    float rep = 1.f, freq = 0.f, pres = 0.f;
-    if (a.hist) {
-        rep = a.pen[3 * b], freq = a.pen[3 * b + 1], pres = a.pen[3 * b + 2];
-    }
-    const bool pen = a.hist && !(rep == 1.f && freq == 0.f && pres == 0.f);
-    if (pen)
-        for (uint32_t i = tid; i < nv; i += 256) cnt[i] = 0;
-    if (a.bias)
-        for (uint32_t i = tid; i < nv; i += 256) add[i] = 0.f;
-    __syncthreads();
-    if (pen) {
-        const int64_t lo = a.hist_off[b], hi = a.hist_off[b + 1];
-        const int64_t wrote = lo + (a.gen ? max(a.gen[b], 0) : 0);
-        for (int64_t i = lo + tid; i < hi; i += 256) {
-            const uint32_t t = (uint32_t)a.hist[i] - v0;
-            if (t < nv) {
-                if (i >= wrote)
-                    atomicAdd(&cnt[t], 1u);
-                else
-                    atomicOr(&cnt[t], kPrompt);
+// Four logits from element i of a row, `left` of them in the slice.
+__device__ inline float4 load_four(const LogitsArgs &a, uint64_t i, uint32_t left) {
+    float v[4] = {0.f, 0.f, 0.f, 0.f};
+    if (left >= 4) {
+        if (a.type == kTypeF32) {
+            const u32x4 q = *(const u32x4_a4 *)((const float *)a.x + i);
+#pragma unroll
+            for (int k = 0; k < 4; k++) v[k] = bits_f32(q[k]);
+        } else {
+            const u32x2 q = *(const u32x2_a2 *)((const uint16_t *)a.x + i);
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                const uint32_t h = k & 1 ? q[k >> 1] >> 16 : q[k >> 1] & 0xffffu;
+                v[k] = a.type == kTypeF16 ? (float)__builtin_bit_cast(_Float16, (uint16_t)h)
+                                          : bits_f32(h << 16);
             }
         }
+    } else {
+        for (uint32_t k = 0; k < left; k++) v[k] = load_as_f32(a.x, a.type, i + k);
     }
-    if (a.bias && tid < 64) {
-        // one wave, in list order: entries of one token among a wave's 64 are
-        // taken in turn
-        const int64_t lo = a.bias_off[b], hi = a.bias_off[b + 1];
-        for (int64_t i0 = lo; i0 < hi; i0 += 64) {
-            const int64_t i = i0 + tid;
-            const uint32_t t = i < hi ? (uint32_t)a.bias_ids[i] - v0 : nv;
-            const bool in = t < nv;
-            const float v = in ? a.bias[i] : 0.f;
+    return make_float4(v[0], v[1], v[2], v[3]);
+}
+
+__device__ inline void store_four(const LogitsArgs &a, uint64_t i, uint32_t left, const float *z) {
+    if (left >= 4) {
+        if (a.type == kTypeF32) {
+            *(u32x4_a4 *)((float *)a.out + i) =
+                (u32x4){f32_bits(z[0]), f32_bits(z[1]), f32_bits(z[2]), f32_bits(z[3])};
+        } else {
+            *(u32x2_a2 *)((uint16_t *)a.out + i) =
+                (u32x2){f32_to_16(z[0], a.type) | (uint32_t)f32_to_16(z[1], a.type) << 16,
+                        f32_to_16(z[2], a.type) | (uint32_t)f32_to_16(z[3], a.type) << 16};
+        }
+    } else {
+        for (uint32_t k = 0; k < left; k++) store_from_f32(a.out, a.type, i + k, z[k]);
+    }
+}
+
+// Occurrences of the slice's tokens in the row's history.
+__device__ inline void count_history(const LogitsArgs &a, uint32_t b, uint32_t v0, uint32_t nv,
+                                     uint32_t *cnt) {
+    const int64_t lo = a.hist_off[b], hi = a.hist_off[b + 1];
+    const int64_t wrote = lo + (a.gen ? max(a.gen[b], 0) : 0);
+    constexpr uint32_t U = 4;       // loads of four tokens in flight a thread
+    for (int64_t i0 = lo + 4 * threadIdx.x; i0 < hi; i0 += 4 * kThreads * U) {
+        u32x4 t[U];
+#pragma unroll
+        for (uint32_t u = 0; u < U; u++) {
+            const int64_t i = i0 + 4 * kThreads * u;
+            t[u] = (u32x4){~0u, ~0u, ~0u, ~0u};
+            if (i + 4 <= hi)
+                t[u] = *(const u32x4_a4 *)(a.hist + i);
+            else
+#pragma unroll
+                for (int k = 0; k < 3; k++)
+                    if (i + k < hi) t[u][k] = (uint32_t)a.hist[i + k];
+        }
+#pragma unroll
+        for (uint32_t u = 0; u < U; u++)
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                const uint32_t v = t[u][k] - v0;
+                if (v >= nv || (int32_t)t[u][k] < 0) continue;
+                if (i0 + 4 * kThreads * u + k >= wrote)
+                    atomicAdd(&cnt[v], 1u);
+                else
+                    atomicOr(&cnt[v], kPrompt);
+            }
+    }
+}
+
+// Sums of the row's biases in list order, by one wave: entries of one token
+// among 64 are taken in turn.
+__device__ inline void sum_biases(const LogitsArgs &a, int64_t lo, int64_t hi, uint32_t v0,
+                                  uint32_t nv, float *add) {
+    constexpr uint32_t U = 4;
+    const uint32_t lane = threadIdx.x & 63u;
+    for (int64_t i0 = lo; i0 < hi; i0 += 64 * U) {
+        uint32_t t[U];
+        float v[U];
+#pragma unroll
+        for (uint32_t u = 0; u < U; u++) {
+            const int64_t i = i0 + 64 * u + lane;
+            t[u] = i < hi ? (uint32_t)a.bias_ids[i] : ~0u;
+            v[u] = i < hi ? a.bias[i] : 0.f;
+        }
+#pragma unroll
+        for (uint32_t u = 0; u < U; u++) {
+            const uint32_t at = t[u] - v0;
+            const bool in = at < nv && (int32_t)t[u] >= 0;
             uint32_t turn = 0;
-            const uint64_t all = __ballot(in);
-            for (uint64_t m = all; m; m &= m - 1) {
+            for (uint64_t m = __ballot(in); m; m &= m - 1) {
                 const uint32_t l = (uint32_t)__builtin_ctzll(m);
-                const uint32_t o = (uint32_t)__builtin_amdgcn_readlane((int)t, (int)l);
-                if (in && l < tid && o == t) turn++;
+                const uint32_t o = (uint32_t)__builtin_amdgcn_readlane((int)at, (int)l);
+                if (in && l < lane && o == at) turn++;
             }
             for (uint32_t k = 0; __ballot(in && turn >= k); k++) {
-                if (in && turn == k) add[t] += v;
+                if (in && turn == k) add[at] += v[u];
                 __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
             }
         }
     }
-    __syncthreads();
+}
+
+}  // namespace
+
+// NG groups of four logits a thread.
+template <uint32_t NG>
+__global__ __launch_bounds__(kThreads) void logits_k(LogitsArgs a) {
+    extern __shared__ __align__(16) uint32_t lds[];
+    constexpr uint32_t kSlice = NG * kThreads * 4;
+    const uint32_t tid = threadIdx.x;
+    const uint32_t b = blockIdx.x / a.slices;
+    const uint32_t v0 = (blockIdx.x - b * a.slices) * kSlice;
+    const uint32_t nv = min(kSlice, a.vocab - v0);
+    float4 x[NG];
+    uint32_t bits[NG];
     const uint32_t *mask = nullptr;
     bool none = false;
     if (a.mask) {
         const int32_t r = a.mask_row ? a.mask_row[b] : (int32_t)b;
         none = r >= 0 && (uint32_t)r >= a.n_mask;
-        if (r >= 0 && !none) mask = a.mask + (uint64_t)r * a.mask_ld;
+        if (r >= 0 && !none) mask = a.mask + (uint64_t)r * a.mask_ld + v0 / 32;
     }
-    for (uint32_t i = tid; i < nv; i += 256) {
-        const uint32_t v = v0 + i;
-        float z = load_as_f32(a.x, a.type, (uint64_t)b * a.ld + v);
-        if (pen && cnt[i]) {
-            const float n = (float)(cnt[i] & ~kPrompt);
-            z = z > 0.f ? z / rep : z * rep;
-            z = z - freq * n;
-            if (n > 0.f) z = z - pres;
+#pragma unroll
+    for (uint32_t n = 0; n < NG; n++) {
+        const uint32_t i = (n * kThreads + tid) * 4, left = i < nv ? nv - i : 0u;
+        x[n] = load_four(a, (uint64_t)b * a.ld + v0 + i, left);
+        bits[n] = none ? 0u : mask && left ? mask[i / 32] >> (i & 31u) : 15u;
+    }
+    const bool counted = a.hist && !(a.pen[3 * b] == 1.f && a.pen[3 * b + 1] == 0.f &&
+                                     a.pen[3 * b + 2] == 0.f);
+    const int64_t blo = a.bias ? a.bias_off[b] : 0, bhi = a.bias ? a.bias_off[b + 1] : 0;
+    const bool biased = bhi > blo;
+    uint32_t *cnt = lds;
+    float *add = (float *)(lds + (a.hist ? kSlice : 0u));
+#pragma unroll
+    for (uint32_t n = 0; n < NG; n++) {
+        const uint32_t i = (n * kThreads + tid) * 4;
+        if (counted) *(u32x4 *)(cnt + i) = (u32x4){0, 0, 0, 0};
+        if (biased) *(u32x4 *)(add + i) = (u32x4){0, 0, 0, 0};
+    }
+    __syncthreads();
+    if (biased && tid >= kThreads - 64) sum_biases(a, blo, bhi, v0, nv, add);
+    if (counted) count_history(a, b, v0, nv, cnt);
+    __syncthreads();
+    float rep = 1.f, freq = 0.f, pres = 0.f;
+    if (counted) rep = a.pen[3 * b], freq = a.pen[3 * b + 1], pres = a.pen[3 * b + 2];
+#pragma unroll
+    for (uint32_t n = 0; n < NG; n++) {
+        const uint32_t i = (n * kThreads + tid) * 4;
+        if (i >= nv) break;
+        float z[4] = {x[n].x, x[n].y, x[n].z, x[n].w};
+        if (counted) {
+            const u32x4 c = *(const u32x4 *)(cnt + i);
+            if (c[0] | c[1] | c[2] | c[3])
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    if (!c[k]) continue;
+                    const float m = (float)(c[k] & ~kPrompt);
+                    z[k] = z[k] > 0.f ? z[k] / rep : z[k] * rep;
+                    z[k] = z[k] - freq * m;
+                    if (m > 0.f) z[k] = z[k] - pres;
+                }
         }
-        if (a.bias) z += add[i];
-        if (none || (mask && !((mask[v >> 5] >> (v & 31u)) & 1u))) z = -__builtin_inff();
-        store_from_f32(a.out, a.type, (uint64_t)b * a.ldo + v, z);
+        if (biased) {
+            const float4 d = *(const float4 *)(add + i);
+            z[0] += d.x, z[1] += d.y, z[2] += d.z, z[3] += d.w;
+        }
+#pragma unroll
+        for (int k = 0; k < 4; k++)
+            if (!((bits[n] >> k) & 1u)) z[k] = -__builtin_inff();
+        store_four(a, (uint64_t)b * a.ldo + v0 + i, nv - i, z);
     }
 }
 
@@ -153,15 +260,20 @@ bool q4mi_logits_process(const void *d_logits, uint32_t type, uint64_t ld, uint3
     a.mask_row = d_mask_row, a.hist_off = d_hist_off, a.bias_off = d_bias_off, a.pen = d_pen;
     a.bias = d_bias, a.mask = d_mask, a.ld = ld, a.ldo = ld_out, a.mask_ld = mask_ld;
     a.type = type, a.vocab = n_vocab, a.n_mask = n_mask;
-    a.slice = 4096;
-    a.slices = (n_vocab + a.slice - 1) / a.slice;
+    // Slices of 2048 tokens until they give every CU four workgroups: then
+    // larger ones, which read the history less often.
+    const uint64_t least = (n_vocab + 2047ull) / 2048 * n_rows, fill = 4ull * cu_count();
+    const uint32_t ng = least <= fill ? 1 : least <= 2 * fill ? 2 : 4;
+    const uint32_t slice = ng * kThreads * 4;
+    a.slices = (n_vocab + slice - 1) / slice;
     if ((uint64_t)a.slices * n_rows > 0x7fffffffu) {
         set_error("%s: %u rows of %u logits too large", who, n_rows, n_vocab);
         return false;
     }
     if (!n_rows) return true;
-    const size_t bytes = (size_t)a.slice * 4 * ((d_hist ? 1 : 0) + (d_bias ? 1 : 0));
-    logits_k<<<dim3(a.slices * n_rows), dim3(256), bytes, stream()>>>(a);
+    const size_t lds = (size_t)slice * 4 * ((d_hist ? 1 : 0) + (d_bias ? 1 : 0));
+    auto k = ng == 1 ? logits_k<1> : ng == 2 ? logits_k<2> : logits_k<4>;
+    k<<<dim3(a.slices * n_rows), dim3(kThreads), lds, stream()>>>(a);
     return launch_ok("logits_k");
 }
 
