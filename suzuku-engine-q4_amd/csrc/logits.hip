@@ -102,7 +102,7 @@ __device__ inline void count_history(const LogitsArgs &a, uint32_t b, uint32_t v
 #pragma unroll
             for (int k = 0; k < 4; k++) {
                 const uint32_t v = t[u][k] - v0;
-                if (v >= nv || (int32_t)t[u][k] < 0) continue;
+                if (v >= nv) continue;      // another slice's, or no token
                 if (i0 + 4 * kThreads * u + k >= wrote)
                     atomicAdd(&cnt[v], 1u);
                 else
@@ -129,7 +129,7 @@ __device__ inline void sum_biases(const LogitsArgs &a, int64_t lo, int64_t hi, u
 #pragma unroll
         for (uint32_t u = 0; u < U; u++) {
             const uint32_t at = t[u] - v0;
-            const bool in = at < nv && (int32_t)t[u] >= 0;
+            const bool in = at < nv;        // else another slice's, or no token
             uint32_t turn = 0;
             for (uint64_t m = __ballot(in); m; m &= m - 1) {
                 const uint32_t l = (uint32_t)__builtin_ctzll(m);
@@ -174,45 +174,54 @@ __global__ __launch_bounds__(kThreads) void logits_k(LogitsArgs a) {
                                      a.pen[3 * b + 2] == 0.f);
     const int64_t blo = a.bias ? a.bias_off[b] : 0, bhi = a.bias ? a.bias_off[b + 1] : 0;
     const bool biased = bhi > blo;
-    uint32_t *cnt = lds;
-    float *add = (float *)(lds + (a.hist ? kSlice : 0u));
+    // The counters' LDS holds the biases afterwards: half the LDS, and twice the
+    // workgroups a CU to hide what each waits for.
+    auto clear = [&]() __attribute__((always_inline)) {
 #pragma unroll
-    for (uint32_t n = 0; n < NG; n++) {
-        const uint32_t i = (n * kThreads + tid) * 4;
-        if (counted) *(u32x4 *)(cnt + i) = (u32x4){0, 0, 0, 0};
-        if (biased) *(u32x4 *)(add + i) = (u32x4){0, 0, 0, 0};
+        for (uint32_t n = 0; n < NG; n++)
+            *(u32x4 *)(lds + (n * kThreads + tid) * 4) = (u32x4){0, 0, 0, 0};
+        __syncthreads();
+    };
+    float z[NG][4];
+#pragma unroll
+    for (uint32_t n = 0; n < NG; n++) z[n][0] = x[n].x, z[n][1] = x[n].y, z[n][2] = x[n].z, z[n][3] = x[n].w;
+    if (counted) {
+        clear();
+        count_history(a, b, v0, nv, lds);
+        __syncthreads();
+        const float rep = a.pen[3 * b], freq = a.pen[3 * b + 1], pres = a.pen[3 * b + 2];
+#pragma unroll
+        for (uint32_t n = 0; n < NG; n++) {
+            const u32x4 c = *(const u32x4 *)(lds + (n * kThreads + tid) * 4);
+            if (!(c[0] | c[1] | c[2] | c[3])) continue;
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                if (!c[k]) continue;
+                const float m = (float)(c[k] & ~kPrompt);
+                z[n][k] = z[n][k] > 0.f ? z[n][k] / rep : z[n][k] * rep;
+                z[n][k] = z[n][k] - freq * m;
+                if (m > 0.f) z[n][k] = z[n][k] - pres;
+            }
+        }
     }
-    __syncthreads();
-    if (biased && tid >= kThreads - 64) sum_biases(a, blo, bhi, v0, nv, add);
-    if (counted) count_history(a, b, v0, nv, cnt);
-    __syncthreads();
-    float rep = 1.f, freq = 0.f, pres = 0.f;
-    if (counted) rep = a.pen[3 * b], freq = a.pen[3 * b + 1], pres = a.pen[3 * b + 2];
+    if (biased) {
+        clear();    // each thread clears what it alone has read
+        if (tid < 64) sum_biases(a, blo, bhi, v0, nv, (float *)lds);
+        __syncthreads();
+#pragma unroll
+        for (uint32_t n = 0; n < NG; n++) {
+            const float4 d = *(const float4 *)(lds + (n * kThreads + tid) * 4);
+            z[n][0] += d.x, z[n][1] += d.y, z[n][2] += d.z, z[n][3] += d.w;
+        }
+    }
 #pragma unroll
     for (uint32_t n = 0; n < NG; n++) {
         const uint32_t i = (n * kThreads + tid) * 4;
         if (i >= nv) break;
-        float z[4] = {x[n].x, x[n].y, x[n].z, x[n].w};
-        if (counted) {
-            const u32x4 c = *(const u32x4 *)(cnt + i);
-            if (c[0] | c[1] | c[2] | c[3])
-#pragma unroll
-                for (int k = 0; k < 4; k++) {
-                    if (!c[k]) continue;
-                    const float m = (float)(c[k] & ~kPrompt);
-                    z[k] = z[k] > 0.f ? z[k] / rep : z[k] * rep;
-                    z[k] = z[k] - freq * m;
-                    if (m > 0.f) z[k] = z[k] - pres;
-                }
-        }
-        if (biased) {
-            const float4 d = *(const float4 *)(add + i);
-            z[0] += d.x, z[1] += d.y, z[2] += d.z, z[3] += d.w;
-        }
 #pragma unroll
         for (int k = 0; k < 4; k++)
-            if (!((bits[n] >> k) & 1u)) z[k] = -__builtin_inff();
-        store_four(a, (uint64_t)b * a.ldo + v0 + i, nv - i, z);
+            if (!((bits[n] >> k) & 1u)) z[n][k] = -__builtin_inff();
+        store_four(a, (uint64_t)b * a.ldo + v0 + i, nv - i, z[n]);
     }
 }
 
@@ -271,7 +280,7 @@ bool q4mi_logits_process(const void *d_logits, uint32_t type, uint64_t ld, uint3
         return false;
     }
     if (!n_rows) return true;
-    const size_t lds = (size_t)slice * 4 * ((d_hist ? 1 : 0) + (d_bias ? 1 : 0));
+    const size_t lds = d_hist || d_bias ? (size_t)slice * 4 : 0;
     auto k = ng == 1 ? logits_k<1> : ng == 2 ? logits_k<2> : logits_k<4>;
     k<<<dim3(a.slices * n_rows), dim3(kThreads), lds, stream()>>>(a);
     return launch_ok("logits_k");
