@@ -248,13 +248,13 @@ __global__ __launch_bounds__(64 * NW, MT > 1 ? 4 : 1) void mx4_few_k(MulArgs a) 
 }
 
 // Row p through the expert that the list names; grid (blocks, rows).
-template <bool FULL, uint32_t PF, uint32_t MT, uint32_t NW>
-__global__ __launch_bounds__(64 * NW) void mx4_sel_k(MulArgs a) {
+template <bool FULL, uint32_t PF>
+__global__ __launch_bounds__(256) void mx4_sel_k(MulArgs a) {
     extern __shared__ __align__(16) uint8_t lds[];
     const int32_t e = a.eid[blockIdx.y];
     if (e < 0 || (uint32_t)e >= a.n_expert) return;
     const FewRange f = {blockIdx.y, 1, a.x_div, nullptr};
-    few_groups<FULL, PF, MT, NW>(a, a.w + e * a.w_stride, a.ws + e * a.ws_stride, f, blockIdx.x,
+    few_groups<FULL, PF, 1, 4>(a, a.w + e * a.w_stride, a.ws + e * a.ws_stride, f, blockIdx.x,
                                a.blocks, lds);
 }
 
@@ -763,33 +763,36 @@ uint32_t few_split(const MulArgs &a, uint32_t waves, uint64_t tiles) {
     return ks;
 }
 
-// One group: `rows` (<= 16) activation rows a workgroup, `lists` of them.
+// One group: `rows` (<= 16) activation rows a workgroup, `lists` of them.  Two
+// chunks in flight a wave: four leave room for three waves a SIMD instead of
+// four (LM head 151936 x 2048, one token: 32.8 us against 30.7; eight float
+// rows: 40.8 against 36.1).  As many workgroups as are resident at once, each
+// with the same number of rounds (40 rows' 2048 x 512: 8.8 -> 6.9 us).
 template <class F>
 bool few_launch(MulArgs &a, uint32_t rows, uint32_t lists, F pick, const char *name) {
     constexpr uint32_t NW = 4;
     const uint64_t tiles = (a.w_rows + 15) / 16;
-    const uint32_t room = 4 * cu_count();
     a.ks = few_split(a, NW, tiles * lists);
     const size_t lds = few_fit(a, rows, 1, NW, 40 * 1024);
-    const uint32_t per = NW / a.ks, chunks = (std::min(a.seg, mx4_blocks(a.cols)) + 15) / 16;
-    const uint32_t mine = (chunks + a.ks - 1) / a.ks;
-    a.blocks = (uint32_t)std::min<uint64_t>((tiles + per - 1) / per,
-                                            std::max(1u, room / std::min(lists, room)));
+    const uint32_t chunks = (std::min(a.seg, mx4_blocks(a.cols)) + 15) / 16;
+    const uint32_t pf = chunks > a.ks ? 2 : 1;
+    const uint64_t sets = (tiles * a.ks + NW - 1) / NW;
+    const uint64_t resident = std::max(1u, (pf == 1 ? 6u : 4u) * cu_count() / lists);
+    const uint64_t rounds = (sets + resident - 1) / resident;
+    a.blocks = (uint32_t)((sets + rounds - 1) / rounds);
     wide_rows(a);
-    auto k = pick(mx4_blocks(a.cols) % 16 == 0, mine >= 4 ? 4 : mine >= 2 ? 2 : 1);
+    auto k = pick(mx4_blocks(a.cols) % 16 == 0, pf);
     k<<<dim3(a.blocks, lists), dim3(64 * NW), lds, stream()>>>(a);
     return launch_ok(name);
 }
 typedef void (*MulKernel)(MulArgs);
 MulKernel few_kernel(bool full, uint32_t pf) {
-    return pf == 4   ? (full ? mx4_few_k<true, 4, 1, 4> : mx4_few_k<false, 4, 1, 4>)
-           : pf == 2 ? (full ? mx4_few_k<true, 2, 1, 4> : mx4_few_k<false, 2, 1, 4>)
-                     : (full ? mx4_few_k<true, 1, 1, 4> : mx4_few_k<false, 1, 1, 4>);
+    return pf == 2 ? (full ? mx4_few_k<true, 2, 1, 4> : mx4_few_k<false, 2, 1, 4>)
+                   : (full ? mx4_few_k<true, 1, 1, 4> : mx4_few_k<false, 1, 1, 4>);
 }
 MulKernel sel_kernel(bool full, uint32_t pf) {
-    return pf == 4   ? (full ? mx4_sel_k<true, 4, 1, 4> : mx4_sel_k<false, 4, 1, 4>)
-           : pf == 2 ? (full ? mx4_sel_k<true, 2, 1, 4> : mx4_sel_k<false, 2, 1, 4>)
-                     : (full ? mx4_sel_k<true, 1, 1, 4> : mx4_sel_k<false, 1, 1, 4>);
+    return pf == 2 ? (full ? mx4_sel_k<true, 2> : mx4_sel_k<false, 2>)
+                   : (full ? mx4_sel_k<true, 1> : mx4_sel_k<false, 1>);
 }
 
 // Two groups: 17 to 32 activation rows, eight waves.
