@@ -26,7 +26,7 @@ struct MulArgs {
     uint64_t w_rows, cols, w_stride, ws_stride, ldx, xrows, n, ldy;
     uint32_t n_expert, x_type, y_type, x_div;
     uint32_t ks, seg, blocks;       // waves a tile, blocks of K in LDS, workgroups along the weights
-    uint32_t m_tiles, parts;        // tiles along the activations; shares of an expert's weight rows
+    uint32_t m_tiles;               // tiles along the activations
     bool x_wide, y_wide;            // whether rows can move 16 bytes at a time
 };
 
@@ -116,11 +116,12 @@ __device__ inline void few_stage(const MulArgs &a, const FewRange &f, uint32_t b
     }
 }
 
-// FULL: rows are whole chunks of 16 blocks.  Workgroup `block` of `blocks`
-// takes every blocks-th set of weight tiles.
+// FULL: rows are whole chunks of 16 blocks.  Weight tiles [first, last), of
+// which workgroup `block` of `blocks` takes every blocks-th set.
 template <bool FULL, uint32_t PF, uint32_t MT, uint32_t NW, bool FLOATS>
 __device__ inline void few_rows(const MulArgs &a, const uint8_t *w, const uint8_t *ws,
-                                const FewRange &f, uint32_t block, uint32_t blocks, uint8_t *lds) {
+                                const FewRange &f, uint32_t first, uint32_t last, uint32_t block,
+                                uint32_t blocks, uint8_t *lds) {
     const uint32_t lane = threadIdx.x & 63u;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t m = lane & 15u, g = lane >> 4;
@@ -130,18 +131,17 @@ __device__ inline void few_rows(const MulArgs &a, const uint8_t *w, const uint8_
     const uint32_t cld = few_code_ld(seg), scld = few_scale_ld(seg);
     uint8_t *codes = lds, *scales = lds + f.rows * cld;
     v4f *red = (v4f *)(scales + f.rows * scld);
-    const uint32_t tiles = (uint32_t)((a.w_rows + 15) / 16);
     uint32_t xc[MT], xsc[MT];       // this lane's row of every group, in codes and scales
 #pragma unroll
     for (uint32_t n = 0; n < MT; n++) {
         const uint32_t t = min(16 * n + m, f.rows - 1);
         xc[n] = t * cld + 16u * g, xsc[n] = t * scld;
     }
-    const uint32_t rounds = (tiles + per * blocks - 1) / (per * blocks);
+    const uint32_t rounds = (last - first + per * blocks - 1) / (per * blocks);
     for (uint32_t i = 0; i < rounds; i++) {
-        const uint32_t tile = (i * blocks + block) * per + sub;
-        const bool mine = tile < tiles;
-        const uint64_t wr = min((uint64_t)(mine ? tile : 0u) * 16 + m, a.w_rows - 1);
+        const uint32_t tile = first + (i * blocks + block) * per + sub;
+        const bool mine = tile < last;
+        const uint64_t wr = min((uint64_t)(mine ? tile : first) * 16 + m, a.w_rows - 1);
         const uint8_t *wp = w + wr * (16ull * nb), *wsp = ws + wr * sld;
         v4f acc[MT];
 #pragma unroll
@@ -229,14 +229,16 @@ __device__ inline void few_rows(const MulArgs &a, const uint8_t *w, const uint8_
 // Sets of up to 16 * MT rows, by how many groups are there.
 template <bool FULL, uint32_t PF, uint32_t MT, uint32_t NW>
 __device__ inline void few_groups(const MulArgs &a, const uint8_t *w, const uint8_t *ws,
-                                  const FewRange &f, uint32_t block, uint32_t blocks,
-                                  uint8_t *lds) {
+                                  const FewRange &f, uint32_t first, uint32_t last,
+                                  uint32_t block, uint32_t blocks, uint8_t *lds) {
     static_assert(MT <= 2, "one or two groups");
     if (MT == 1 || f.rows <= 16)
-        few_rows<FULL, PF, 1, NW, MT == 1>(a, w, ws, f, block, blocks, lds);
+        few_rows<FULL, PF, 1, NW, MT == 1>(a, w, ws, f, first, last, block, blocks, lds);
     else
-        few_rows<FULL, PF, MT, NW, false>(a, w, ws, f, block, blocks, lds);
+        few_rows<FULL, PF, MT, NW, false>(a, w, ws, f, first, last, block, blocks, lds);
 }
+
+__device__ inline uint32_t row_tiles(const MulArgs &a) { return (uint32_t)((a.w_rows + 15) / 16); }
 
 // Dense: grid (blocks, sets of 16 * MT activation rows).
 template <bool FULL, uint32_t PF, uint32_t MT, uint32_t NW>
@@ -244,7 +246,7 @@ __global__ __launch_bounds__(64 * NW, MT > 1 ? 4 : 1) void mx4_few_k(MulArgs a) 
     extern __shared__ __align__(16) uint8_t lds[];
     const uint64_t p0 = (uint64_t)blockIdx.y * 16 * MT;
     const FewRange f = {p0, (uint32_t)min((uint64_t)16 * MT, a.n - p0), 1, nullptr};
-    few_groups<FULL, PF, MT, NW>(a, a.w, a.ws, f, blockIdx.x, a.blocks, lds);
+    few_groups<FULL, PF, MT, NW>(a, a.w, a.ws, f, 0, row_tiles(a), blockIdx.x, a.blocks, lds);
 }
 
 // Row p through the expert that the list names; grid (blocks, rows).
@@ -254,8 +256,8 @@ __global__ __launch_bounds__(256) void mx4_sel_k(MulArgs a) {
     const int32_t e = a.eid[blockIdx.y];
     if (e < 0 || (uint32_t)e >= a.n_expert) return;
     const FewRange f = {blockIdx.y, 1, a.x_div, nullptr};
-    few_groups<FULL, PF, 1, 4>(a, a.w + e * a.w_stride, a.ws + e * a.ws_stride, f, blockIdx.x,
-                               a.blocks, lds);
+    few_groups<FULL, PF, 1, 4>(a, a.w + e * a.w_stride, a.ws + e * a.ws_stride, f, 0,
+                               row_tiles(a), blockIdx.x, a.blocks, lds);
 }
 
 // ------------------------------------------------------------ rows in tiles
@@ -589,13 +591,15 @@ __global__ __launch_bounds__(64 * WM * WN, WAVES) void mx4_dense_k(MulArgs a) {
 // Experts differ: of a prompt's, a few take most of the rows and many take a
 // handful.  One persistent workgroup a CU goes over a list of items: first
 // tiles of kIdM rows x kIdN weight rows of the experts with more than kIdFew
-// rows (bound by the matrix units), then weight-row shares of the others,
-// whose weights are streamed once past all of their rows (bound by memory).
+// rows (bound by the matrix units), then the others' 16-row weight tiles, each
+// streamed once past all of its expert's rows (bound by memory).  Of the list
+// of those, expert by expert, a workgroup takes one stretch, so it stages few
+// experts' rows, and one shorter by kIdCost tiles for each of its large tiles.
 // Every workgroup makes the list by itself, as prefix sums over the experts'
 // stretches in LDS: no scratch in memory, no launch before, and no workgroups
 // that find nothing to do.
 constexpr uint32_t kIdM = 128, kIdN = 256, kIdWM = 2, kIdWN = 4, kIdWaves = kIdWM * kIdWN;
-constexpr uint32_t kIdFew = 32, kIdExperts = 1024;
+constexpr uint32_t kIdFew = 32, kIdExperts = 1024, kIdCost = 11;
 constexpr size_t kIdLists = 2 * (kIdExperts + 1) * 4;
 
 // Inclusive sums over a workgroup's threads.
@@ -658,27 +662,41 @@ __global__ __launch_bounds__(64 * kIdWaves, 2) void mx4_id_k(MulArgs a) {
     }
     if (n == kIdExperts && threadIdx.x == 64 * kIdWaves - 1) tiles[n] = at.x, shares[n] = at.y;
     __syncthreads();
-    const uint32_t slices = (uint32_t)((a.w_rows + kIdN - 1) / kIdN);
-    const uint32_t heavy = tiles[n] * slices, all = heavy + shares[n] * a.parts;
-    for (uint32_t i = blockIdx.x; i < all; i += a.blocks) {
-        const bool big = i < heavy;
-        const uint32_t j = big ? i : i - heavy, each = big ? slices : a.parts;
-        const uint32_t unit = j / each, part = j - unit * each;
-        const uint32_t *list = big ? tiles : shares;
-        const uint32_t e = owner(list, n, unit);
+    const uint32_t slices = (uint32_t)((a.w_rows + kIdN - 1) / kIdN), per = row_tiles(a);
+    const uint32_t heavy = tiles[n] * slices;
+    for (uint32_t i = blockIdx.x; i < heavy; i += a.blocks) {
+        const uint32_t unit = i / slices, part = i - unit * slices;
+        const uint32_t e = owner(tiles, n, unit);
+        int64_t lo;
+        const int64_t rows = stretch(e, &lo), skip = (int64_t)(unit - tiles[e]) * kIdM;
+        if (skip < rows)    // always, with bounds that ascend
+            tile<kIdM, kIdN, kIdWM, kIdWN, true>(a, a.w + e * a.w_stride, a.ws + e * a.ws_stride,
+                                                 (uint64_t)part * kIdN, lo + skip, lo + rows, work);
+        __syncthreads();    // the next tile overwrites what slower waves may still read
+    }
+    // this workgroup's stretch of the others' tiles
+    const uint64_t few = (uint64_t)shares[n] * per, all = few + (uint64_t)heavy * kIdCost;
+    const uint64_t fair = (all + a.blocks - 1) / a.blocks;
+    const uint32_t q = heavy / a.blocks, more = heavy - q * a.blocks;   // large tiles of each
+    const uint64_t less = (uint64_t)q * kIdCost;
+    const uint64_t s0 = fair > less ? fair - less : 0;                  // with q of them
+    const uint64_t s1 = fair > less + kIdCost ? fair - less - kIdCost : 0;
+    auto start = [&](uint32_t b) -> uint64_t {
+        return min(few, b < more ? b * s1 : more * s1 + (b - more) * s0);
+    };
+    uint64_t t = start(blockIdx.x);
+    const uint64_t end_t = start(blockIdx.x + 1);
+    while (t < end_t) {
+        const uint32_t unit = (uint32_t)(t / per), first = (uint32_t)(t - (uint64_t)unit * per);
+        const uint32_t last = (uint32_t)min((uint64_t)per, first + (end_t - t));
+        const uint32_t e = owner(shares, n, unit);
         int64_t lo;
         const int64_t rows = stretch(e, &lo);
-        const uint8_t *w = a.w + e * a.w_stride, *ws = a.ws + e * a.ws_stride;
-        const int64_t skip = (int64_t)(unit - tiles[e]) * kIdM;
-        if (big) {
-            if (skip < rows)    // always, with bounds that ascend
-                tile<kIdM, kIdN, kIdWM, kIdWN, true>(a, w, ws, (uint64_t)part * kIdN, lo + skip,
-                                                     lo + rows, work);
-        } else {
-            const FewRange f = {(uint64_t)lo, (uint32_t)rows, 1, a.act};
-            few_groups<FULL, 2, kIdFew / 16, kIdWaves>(a, w, ws, f, part, a.parts, work);
-        }
-        __syncthreads();   // the next item overwrites what slower waves may still read
+        const FewRange f = {(uint64_t)lo, (uint32_t)rows, 1, a.act};
+        few_groups<FULL, 2, kIdFew / 16, kIdWaves>(a, a.w + e * a.w_stride, a.ws + e * a.ws_stride,
+                                                   f, first, last, 0, 1, work);
+        t += last - first;
+        __syncthreads();    // the next expert's rows overwrite what slower waves may still read
     }
 }
 
@@ -849,12 +867,8 @@ bool id_launch(MulArgs &a) {
     const uint64_t units = std::min<uint64_t>(a.n, a.n_expert) * tiles;
     a.ks = few_split(a, kIdWaves, units);
     const size_t few = few_fit(a, kIdFew, kIdFew / 16, kIdWaves, 112 * 1024);
-    const uint32_t per = kIdWaves / a.ks;
-    // two rounds of tiles a share where that leaves every CU several shares
-    const uint32_t rounds = units / (2 * per) >= 4ull * cu_count() ? 2 : 1;
-    a.parts = (tiles + per * rounds - 1) / (per * rounds);
     const uint64_t slices = (a.w_rows + kIdN - 1) / kIdN;
-    if ((a.n / kIdM + a.n_expert) * slices + (uint64_t)a.n_expert * a.parts > 0x7fffffffu) {
+    if ((a.n / kIdM + a.n_expert) * slices > 0x7fffffffu) {
         set_error("q4mi_mx4_mul_id: too many tiles");
         return false;
     }
