@@ -53,7 +53,7 @@ __device__ inline void store4(void *y, uint32_t yt, uint64_t at, v4f v) {
 // registers; lane (m, g) of it holds row m's blocks 4s + g of a chunk of 16
 // blocks (s = 0..3), so four lanes read 64 adjacent bytes and a chunk's 16
 // scales are one 16-byte load, of which step s uses byte g of dword s.  PF
-// chunks (4 KB each with 16 rows) are in flight a wave.  The activation rows
+// chunks (4 KB each with 16 rows) are multiplied while PF more are in flight.  The activation rows
 // sit in LDS, as codes, in groups of 16 for one instruction each: float rows
 // are quantised on the way there, once a workgroup.  ks waves share a tile
 // along K and their sums are joined in LDS in wave order, so a short matrix
@@ -138,79 +138,67 @@ __device__ inline void few_rows(const MulArgs &a, const uint8_t *w, const uint8_
         xc[n] = t * cld + 16u * g, xsc[n] = t * scld;
     }
     const uint32_t rounds = (last - first + per * blocks - 1) / (per * blocks);
-    for (uint32_t i = 0; i < rounds; i++) {
-        const uint32_t tile = first + (i * blocks + block) * per + sub;
-        const bool mine = tile < last;
-        const uint64_t wr = min((uint64_t)(mine ? tile : first) * 16 + m, a.w_rows - 1);
+    auto tile_of = [&](uint32_t i) { return first + (i * blocks + block) * per + sub; };
+    auto chunks = [&](uint32_t sg) { return (min(seg, nb - sg * seg) + 15) / 16; };
+    struct Batch {
+        u32x4 codes[PF][4], scales[PF];
+    };
+    // chunks c, c + ks, .. (PF of them) of segment sg of round i's weight tile
+    auto load = [&](Batch &q, uint32_t i, uint32_t sg, uint32_t c0) __attribute__((always_inline)) {
+        const uint32_t tile = min(tile_of(i), last - 1), most = chunks(sg) - 1;
+        const uint64_t wr = min((uint64_t)tile * 16 + m, a.w_rows - 1);
         const uint8_t *wp = w + wr * (16ull * nb), *wsp = ws + wr * sld;
-        v4f acc[MT];
 #pragma unroll
-        for (uint32_t n = 0; n < MT; n++) acc[n] = (v4f){0.f, 0.f, 0.f, 0.f};
-        for (uint32_t sg = 0; sg < nseg; sg++) {
-            const uint32_t b0 = sg * seg, nch = (min(seg, nb - b0) + 15) / 16;
-            // the first batch is on its way while the activations are staged
-            uint32_t c0 = kw;
-            u32x4 wq[PF][4], wv[PF];
-            auto load = [&]() __attribute__((always_inline)) {
+        for (uint32_t j = 0; j < PF; j++) {
+            const uint32_t bc = sg * seg + 16 * min(c0 + j * ks, most);
 #pragma unroll
-                for (uint32_t j = 0; j < PF; j++) {
-                    const uint32_t c = min(c0 + j * ks, nch - 1), bc = b0 + 16 * c;
-#pragma unroll
-                    for (uint32_t s = 0; s < 4; s++) {
-                        uint32_t b = bc + 4 * s + g;
-                        if (!FULL) b = min(b, nb - 1);
-                        wq[j][s] = *(const u32x4 *)(wp + 16u * b);
-                        if (!FULL) wv[j][s] = ((const uint32_t *)wsp)[min(bc / 4 + s, sld / 4 - 1)];
-                    }
-                    if (FULL) wv[j] = *(const u32x4_a4 *)(wsp + bc);
-                }
-            };
-            load();
-            if (nseg > 1 || i == 0) {
-                if (nseg > 1) __syncthreads();
-                few_stage<NW, FLOATS>(a, f, b0, seg, nb, sld, codes, scales);
-                __syncthreads();
+            for (uint32_t s = 0; s < 4; s++) {
+                uint32_t b = bc + 4 * s + g;
+                if (!FULL) b = min(b, nb - 1);
+                q.codes[j][s] = *(const u32x4 *)(wp + 16u * b);
+                if (!FULL) q.scales[j][s] = ((const uint32_t *)wsp)[min(bc / 4 + s, sld / 4 - 1)];
             }
-            auto chunk = [&](uint32_t j, uint32_t c) __attribute__((always_inline)) {
-                u32x4 xv[MT];
+            if (FULL) q.scales[j] = *(const u32x4_a4 *)(wsp + bc);
+        }
+    };
+    v4f acc[MT];
+    auto multiply = [&](const Batch &q, uint32_t sg, uint32_t c0) __attribute__((always_inline)) {
+        const uint32_t nch = chunks(sg);
 #pragma unroll
-                for (uint32_t n = 0; n < MT; n++)
-                    xv[n] = *(const u32x4 *)(scales + xsc[n] + 16u * c);
+        for (uint32_t j = 0; j < PF; j++) {
+            const uint32_t c = c0 + j * ks;
+            if (c >= nch) break;
+            u32x4 xv[MT];
 #pragma unroll
-                for (uint32_t s = 0; s < 4; s++) {
-                    uint32_t wb = wv[j][s] >> (8 * g);
-                    if (!FULL && b0 + 16 * c + 4 * s + g >= nb) wb = 127;
+            for (uint32_t n = 0; n < MT; n++) xv[n] = *(const u32x4 *)(scales + xsc[n] + 16u * c);
 #pragma unroll
-                    for (uint32_t n = 0; n < MT; n++) {
-                        const u32x4 xq = *(const u32x4 *)(codes + xc[n] + 256u * c + 64u * s);
-                        acc[n] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
-                            widen(wq[j][s]), widen(xq), acc[n], 4, 4, 0, (int)wb, 0,
-                            (int)(xv[n][s] >> (8 * g)));
-                    }
-                    if (MT > 1) __builtin_amdgcn_sched_barrier(0);   // registers: one step's reads
+            for (uint32_t s = 0; s < 4; s++) {
+                uint32_t wb = q.scales[j][s] >> (8 * g);
+                if (!FULL && sg * seg + 16 * c + 4 * s + g >= nb) wb = 127;
+#pragma unroll
+                for (uint32_t n = 0; n < MT; n++) {
+                    const u32x4 xq = *(const u32x4 *)(codes + xc[n] + 256u * c + 64u * s);
+                    acc[n] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
+                        widen(q.codes[j][s]), widen(xq), acc[n], 4, 4, 0, (int)wb, 0,
+                        (int)(xv[n][s] >> (8 * g)));
                 }
-            };
-            for (; c0 < nch; c0 += PF * ks) {
-                if (c0 != kw) load();
-#pragma unroll
-                for (uint32_t j = 0; j < PF; j++) {
-                    const uint32_t c = c0 + j * ks;
-                    if (c >= nch) break;
-                    chunk(j, c);
-                }
+                if (MT > 1) __builtin_amdgcn_sched_barrier(0);   // registers: one step's reads
             }
         }
+    };
+    auto finish = [&](uint32_t i) __attribute__((always_inline)) {
         if (ks > 1) {
             if (i) __syncthreads();   // the last round's sums have been read
 #pragma unroll
             for (uint32_t n = 0; n < MT; n++) red[(wave * MT + n) * 64 + lane] = acc[n];
             __syncthreads();
-            if (kw) continue;
+            if (kw) return;
             for (uint32_t k = 1; k < ks; k++)
 #pragma unroll
                 for (uint32_t n = 0; n < MT; n++) acc[n] += red[((wave + k) * MT + n) * 64 + lane];
         }
-        if (!mine) continue;
+        const uint32_t tile = tile_of(i);
+        if (tile >= last) return;
         const uint64_t r = (uint64_t)tile * 16 + 4 * g;
 #pragma unroll
         for (uint32_t n = 0; n < MT; n++) {
@@ -223,6 +211,42 @@ __device__ inline void few_rows(const MulArgs &a, const uint8_t *w, const uint8_
                 for (uint32_t k = 0; k < 4; k++)
                     if (r + k < a.w_rows) store_from_f32(a.y, a.y_type, at + k, acc[n][k]);
         }
+    };
+    auto clear = [&]() __attribute__((always_inline)) {
+#pragma unroll
+        for (uint32_t n = 0; n < MT; n++) acc[n] = (v4f){0.f, 0.f, 0.f, 0.f};
+    };
+
+    // The next batch, of this tile or of the next round's, is on its way while
+    // one is multiplied, the first one while the activations are staged.  Every
+    // wave goes through every segment of every round, so all meet the barriers.
+    Batch now, then;
+    uint32_t i = 0, sg = 0, c0 = kw;
+    load(now, 0, 0, kw);
+    few_stage<NW, FLOATS>(a, f, 0, seg, nb, sld, codes, scales);
+    __syncthreads();
+    clear();
+    for (;;) {
+        uint32_t ni = i, nsg = sg, nc = c0 + PF * ks;
+        const bool done = nc >= chunks(sg);
+        if (done) {
+            nc = kw;
+            if (++nsg == nseg) nsg = 0, ni++;
+        }
+        const bool more = ni < rounds;
+        if (more) load(then, ni, nsg, nc);
+        multiply(now, sg, c0);
+        if (ni != i) {
+            finish(i);
+            clear();
+        }
+        if (!more) break;
+        if (done && nseg > 1) {
+            __syncthreads();
+            few_stage<NW, FLOATS>(a, f, nsg * seg, seg, nb, sld, codes, scales);
+            __syncthreads();
+        }
+        now = then, i = ni, sg = nsg, c0 = nc;
     }
 }
 
@@ -241,22 +265,22 @@ __device__ inline void few_groups(const MulArgs &a, const uint8_t *w, const uint
 __device__ inline uint32_t row_tiles(const MulArgs &a) { return (uint32_t)((a.w_rows + 15) / 16); }
 
 // Dense: grid (blocks, sets of 16 * MT activation rows).
-template <bool FULL, uint32_t PF, uint32_t MT, uint32_t NW>
+template <bool FULL, uint32_t MT, uint32_t NW>
 __global__ __launch_bounds__(64 * NW, MT > 1 ? 4 : 1) void mx4_few_k(MulArgs a) {
     extern __shared__ __align__(16) uint8_t lds[];
     const uint64_t p0 = (uint64_t)blockIdx.y * 16 * MT;
     const FewRange f = {p0, (uint32_t)min((uint64_t)16 * MT, a.n - p0), 1, nullptr};
-    few_groups<FULL, PF, MT, NW>(a, a.w, a.ws, f, 0, row_tiles(a), blockIdx.x, a.blocks, lds);
+    few_groups<FULL, 1, MT, NW>(a, a.w, a.ws, f, 0, row_tiles(a), blockIdx.x, a.blocks, lds);
 }
 
 // Row p through the expert that the list names; grid (blocks, rows).
-template <bool FULL, uint32_t PF>
+template <bool FULL>
 __global__ __launch_bounds__(256) void mx4_sel_k(MulArgs a) {
     extern __shared__ __align__(16) uint8_t lds[];
     const int32_t e = a.eid[blockIdx.y];
     if (e < 0 || (uint32_t)e >= a.n_expert) return;
     const FewRange f = {blockIdx.y, 1, a.x_div, nullptr};
-    few_groups<FULL, PF, 1, 4>(a, a.w + e * a.w_stride, a.ws + e * a.ws_stride, f, 0,
+    few_groups<FULL, 1, 1, 4>(a, a.w + e * a.w_stride, a.ws + e * a.ws_stride, f, 0,
                                row_tiles(a), blockIdx.x, a.blocks, lds);
 }
 
@@ -595,11 +619,13 @@ __global__ __launch_bounds__(64 * WM * WN, WAVES) void mx4_dense_k(MulArgs a) {
 // streamed once past all of its expert's rows (bound by memory).  Of the list
 // of those, expert by expert, a workgroup takes one stretch, so it stages few
 // experts' rows, and one shorter by kIdCost tiles for each of its large tiles.
+// Half of the workgroups begin with those, so that memory and matrix units work
+// at the same time.
 // Every workgroup makes the list by itself, as prefix sums over the experts'
 // stretches in LDS: no scratch in memory, no launch before, and no workgroups
 // that find nothing to do.
 constexpr uint32_t kIdM = 128, kIdN = 256, kIdWM = 2, kIdWN = 4, kIdWaves = kIdWM * kIdWN;
-constexpr uint32_t kIdFew = 32, kIdExperts = 1024, kIdCost = 11;
+constexpr uint32_t kIdFew = 32, kIdExperts = 1024, kIdCost = 22;
 constexpr size_t kIdLists = 2 * (kIdExperts + 1) * 4;
 
 // Inclusive sums over a workgroup's threads.
@@ -664,16 +690,6 @@ __global__ __launch_bounds__(64 * kIdWaves, 2) void mx4_id_k(MulArgs a) {
     __syncthreads();
     const uint32_t slices = (uint32_t)((a.w_rows + kIdN - 1) / kIdN), per = row_tiles(a);
     const uint32_t heavy = tiles[n] * slices;
-    for (uint32_t i = blockIdx.x; i < heavy; i += a.blocks) {
-        const uint32_t unit = i / slices, part = i - unit * slices;
-        const uint32_t e = owner(tiles, n, unit);
-        int64_t lo;
-        const int64_t rows = stretch(e, &lo), skip = (int64_t)(unit - tiles[e]) * kIdM;
-        if (skip < rows)    // always, with bounds that ascend
-            tile<kIdM, kIdN, kIdWM, kIdWN, true>(a, a.w + e * a.w_stride, a.ws + e * a.ws_stride,
-                                                 (uint64_t)part * kIdN, lo + skip, lo + rows, work);
-        __syncthreads();    // the next tile overwrites what slower waves may still read
-    }
     // this workgroup's stretch of the others' tiles
     const uint64_t few = (uint64_t)shares[n] * per, all = few + (uint64_t)heavy * kIdCost;
     const uint64_t fair = (all + a.blocks - 1) / a.blocks;
@@ -684,19 +700,36 @@ __global__ __launch_bounds__(64 * kIdWaves, 2) void mx4_id_k(MulArgs a) {
     auto start = [&](uint32_t b) -> uint64_t {
         return min(few, b < more ? b * s1 : more * s1 + (b - more) * s0);
     };
-    uint64_t t = start(blockIdx.x);
-    const uint64_t end_t = start(blockIdx.x + 1);
-    while (t < end_t) {
-        const uint32_t unit = (uint32_t)(t / per), first = (uint32_t)(t - (uint64_t)unit * per);
-        const uint32_t last = (uint32_t)min((uint64_t)per, first + (end_t - t));
-        const uint32_t e = owner(shares, n, unit);
-        int64_t lo;
-        const int64_t rows = stretch(e, &lo);
-        const FewRange f = {(uint64_t)lo, (uint32_t)rows, 1, a.act};
-        few_groups<FULL, 2, kIdFew / 16, kIdWaves>(a, a.w + e * a.w_stride, a.ws + e * a.ws_stride,
-                                                   f, first, last, 0, 1, work);
-        t += last - first;
-        __syncthreads();    // the next expert's rows overwrite what slower waves may still read
+    // every second workgroup of a die takes the streamed tiles first
+    for (uint32_t phase = 0; phase < 2; phase++) {
+        if (phase == ((blockIdx.x >> 3) & 1u)) {
+            for (uint32_t i = blockIdx.x; i < heavy; i += a.blocks) {
+                const uint32_t unit = i / slices, part = i - unit * slices;
+                const uint32_t e = owner(tiles, n, unit);
+                int64_t lo;
+                const int64_t rows = stretch(e, &lo), skip = (int64_t)(unit - tiles[e]) * kIdM;
+                if (skip < rows)    // always, with bounds that ascend
+                    tile<kIdM, kIdN, kIdWM, kIdWN, true>(
+                        a, a.w + e * a.w_stride, a.ws + e * a.ws_stride, (uint64_t)part * kIdN,
+                        lo + skip, lo + rows, work);
+                __syncthreads();    // the next item overwrites what slower waves may still read
+            }
+            continue;
+        }
+        const uint64_t end_t = start(blockIdx.x + 1);
+        for (uint64_t t = start(blockIdx.x); t < end_t;) {
+            const uint32_t unit = (uint32_t)(t / per), first = (uint32_t)(t - (uint64_t)unit * per);
+            const uint32_t last = (uint32_t)min((uint64_t)per, first + (end_t - t));
+            const uint32_t e = owner(shares, n, unit);
+            int64_t lo;
+            const int64_t rows = stretch(e, &lo);
+            const FewRange f = {(uint64_t)lo, (uint32_t)rows, 1, a.act};
+            few_groups<FULL, 2, kIdFew / 16, kIdWaves>(a, a.w + e * a.w_stride,
+                                                       a.ws + e * a.ws_stride, f, first, last, 0,
+                                                       1, work);
+            t += last - first;
+            __syncthreads();    // as above
+        }
     }
 }
 
@@ -781,37 +814,29 @@ uint32_t few_split(const MulArgs &a, uint32_t waves, uint64_t tiles) {
     return ks;
 }
 
-// One group: `rows` (<= 16) activation rows a workgroup, `lists` of them.  Two
-// chunks in flight a wave: four leave room for three waves a SIMD instead of
-// four (LM head 151936 x 2048, one token: 32.8 us against 30.7; eight float
-// rows: 40.8 against 36.1).  As many workgroups as are resident at once, each
-// with the same number of rounds (40 rows' 2048 x 512: 8.8 -> 6.9 us).
+// One group: `rows` (<= 16) activation rows a workgroup, `lists` of them.  One
+// chunk a wave is multiplied while one is in flight: two of each are slower
+// (three waves a SIMD instead of four: ten experts' 1280 x 2560 8.7 us against
+// 7.6, LM head 151936 x 2048 with eight float rows 40.2 against 35.7).  As
+// many workgroups as are resident at once, each with the same number of rounds.
 template <class F>
 bool few_launch(MulArgs &a, uint32_t rows, uint32_t lists, F pick, const char *name) {
     constexpr uint32_t NW = 4;
     const uint64_t tiles = (a.w_rows + 15) / 16;
     a.ks = few_split(a, NW, tiles * lists);
     const size_t lds = few_fit(a, rows, 1, NW, 40 * 1024);
-    const uint32_t chunks = (std::min(a.seg, mx4_blocks(a.cols)) + 15) / 16;
-    const uint32_t pf = chunks > a.ks ? 2 : 1;
     const uint64_t sets = (tiles * a.ks + NW - 1) / NW;
-    const uint64_t resident = std::max(1u, (pf == 1 ? 6u : 4u) * cu_count() / lists);
+    const uint64_t resident = std::max(1u, 4u * cu_count() / lists);
     const uint64_t rounds = (sets + resident - 1) / resident;
     a.blocks = (uint32_t)((sets + rounds - 1) / rounds);
     wide_rows(a);
-    auto k = pick(mx4_blocks(a.cols) % 16 == 0, pf);
+    auto k = pick(mx4_blocks(a.cols) % 16 == 0);
     k<<<dim3(a.blocks, lists), dim3(64 * NW), lds, stream()>>>(a);
     return launch_ok(name);
 }
 typedef void (*MulKernel)(MulArgs);
-MulKernel few_kernel(bool full, uint32_t pf) {
-    return pf == 2 ? (full ? mx4_few_k<true, 2, 1, 4> : mx4_few_k<false, 2, 1, 4>)
-                   : (full ? mx4_few_k<true, 1, 1, 4> : mx4_few_k<false, 1, 1, 4>);
-}
-MulKernel sel_kernel(bool full, uint32_t pf) {
-    return pf == 2 ? (full ? mx4_sel_k<true, 2> : mx4_sel_k<false, 2>)
-                   : (full ? mx4_sel_k<true, 1> : mx4_sel_k<false, 1>);
-}
+MulKernel few_kernel(bool full) { return full ? mx4_few_k<true, 1, 4> : mx4_few_k<false, 1, 4>; }
+MulKernel sel_kernel(bool full) { return full ? mx4_sel_k<true> : mx4_sel_k<false>; }
 
 // Two groups: 17 to 32 activation rows, eight waves.
 bool few2_launch(MulArgs &a) {
@@ -825,7 +850,7 @@ bool few2_launch(MulArgs &a) {
     a.blocks = (uint32_t)std::min<uint64_t>((tiles + per - 1) / per, 2 * cu_count());
     wide_rows(a);
     const bool full = mx4_blocks(a.cols) % 16 == 0;
-    auto k = full ? mx4_few_k<true, 2, MT, NW> : mx4_few_k<false, 2, MT, NW>;
+    auto k = full ? mx4_few_k<true, MT, NW> : mx4_few_k<false, MT, NW>;
     static DynLds st[2];
     if (!dyn_lds_ok((const void *)k, lds, kMost, st[full], "mx4_few_k")) return false;
     k<<<dim3(a.blocks), dim3(64 * NW), lds, stream()>>>(a);

@@ -161,6 +161,34 @@ def test_mul_exact(gpu, n, rows, cols):
     assert (got[n:] == -7).all() and (got[:, rows:] == -7).all()
 
 
+@pytest.mark.parametrize("n,rows,cols", [
+    (700, 5000, 352), (700, 5000, 2080), (1300, 5000, 800), (1300, 5000, 256), (2100, 5000, 96),
+    (2100, 5000, 1056), (2309, 4609, 544), (20, 20000, 608), (32, 9000, 1024)])
+def test_mul_large_tiles(gpu, n, rows, cols):
+    """Sizes that fill the chip with each of the larger tiles, none of them
+    whole, with whole and partial stages of K; sums exact in fp32.  The torch
+    product in fp64 on the device is the reference."""
+    g = torch.Generator(device="cuda").manual_seed(n + cols)
+    nb = ref.blocks(cols)
+
+    def rand(r):
+        c = torch.randint(0, 256, (r, nb * 16), dtype=torch.uint8, device="cuda", generator=g)
+        s = torch.zeros((r, ref.scale_row(cols)), dtype=torch.uint8, device="cuda")
+        s[:, :nb] = torch.randint(126, 129, (r, nb), dtype=torch.uint8, device="cuda", generator=g)
+        t = torch.tensor(np.concatenate([ref.LEVELS, -ref.LEVELS]), device="cuda")
+        v = torch.stack([t[(c & 15).long()], t[(c >> 4).long()]], 2).view(r, nb, 32)
+        return c, s, (v * torch.exp2(s[:, :nb].double() - 127)[..., None]).view(r, nb * 32)
+
+    w, ws, wv = rand(rows)
+    x, xs, xv = rand(n)
+    want = xv @ wv.t()
+    y = torch.full((n + 1, rows + 4), -7.0, device="cuda")
+    q4mi.check(gpu.q4mi_mx4_mul(w.data_ptr(), ws.data_ptr(), rows, cols, x.data_ptr(),
+                                xs.data_ptr(), MX4, 0, n, y.data_ptr(), 0, rows + 4), "mul")
+    assert torch.equal(y[:n, :rows].double(), want)
+    assert bool((y[n:] == -7).all()) and bool((y[:, rows:] == -7).all())
+
+
 @pytest.mark.parametrize("n,rows,cols", [(1, 50, 16384), (8, 40, 8224), (16, 70, 9000),
                                          (16, 5000, 4128), (40, 64, 16000), (300, 260, 8192)])
 def test_mul_long_rows(gpu, n, rows, cols):
@@ -251,8 +279,8 @@ def test_mul_extreme_scales(gpu):
 
 # ------------------------------------------------------------ routed experts
 
-def arena(rng, experts, rows, cols):
-    w, ws = ref.random_rows(rng, experts * rows, cols, 126, 128)
+def arena(rng, experts, rows, cols, lo=126, hi=128):
+    w, ws = ref.random_rows(rng, experts * rows, cols, lo, hi)
     v = ref.values(w, ws, cols).reshape(experts, rows, cols)
     return dev(w), dev(ws), v, rows * w.shape[1], rows * ws.shape[1]
 
@@ -309,16 +337,20 @@ def test_mul_sel_float_rows(gpu, xt):
 @pytest.mark.parametrize("counts,rows,cols,spare", [
     ([0, 5, 0, 17], 64, 96, 3), ([40], 33, 32, 0), ([1] * 20, 100, 640, 0), ([0, 0], 16, 32, 4),
     ([130, 0, 300, 7, 64, 65], 272, 288, 9), ([500, 1], 1024, 512, 0), ([33, 260, 31], 520, 2048, 1),
-    ([3] * 64, 200, 1013, 2)])
+    ([3] * 64, 200, 1013, 2), ([32, 33, 31, 64, 16, 17], 90, 416, 0), ([1, 0, 2] * 341 + [5], 20, 64, 3),
+    ([20, 150], 50, 9000, 0), ([129] * 3, 600, 1056, 0)])
 @pytest.mark.parametrize("gather", [True, False])
 def test_mul_id_exact(gpu, counts, rows, cols, spare, gather):
     """Ragged stretches, empty experts, rows that no stretch covers."""
     rng = np.random.default_rng(sum(counts) + rows)
     experts, total = len(counts), sum(counts)
-    w, ws, wv, st, sst = arena(rng, experts, rows, cols)
+    # long rows keep one scale, so that their sums stay exact
+    w, ws, wv, st, sst = arena(rng, experts, rows, cols, 126 if cols <= 4096 else 127,
+                               128 if cols <= 4096 else 127)
     n = total + spare
     xrows = max(1, total // 3) if gather else max(n, 1)
-    x, xs = ref.random_rows(rng, xrows, cols, 126, 128)
+    x, xs = ref.random_rows(rng, xrows, cols, 126 if cols <= 4096 else 127,
+                            128 if cols <= 4096 else 127)
     xv = ref.values(x, xs, cols)
     bounds = np.concatenate([[0], np.cumsum(counts)]).astype(np.int32)
     act = rng.integers(0, xrows, n).astype(np.int32) if gather else np.arange(n, dtype=np.int32)
@@ -377,6 +409,106 @@ def test_mul_id_types(gpu, yt):
     want = np.einsum("prc,pc->pr", wv[e], xv)
     s = np.einsum("prc,pc->pr", np.abs(wv[e]), np.abs(xv))
     close(y, want, s, cols, TYPES[yt])
+
+
+# ---------------------------------------------------- a layer and its logits
+
+def test_layer_to_logits(gpu):
+    """The operators as an engine runs them: router, pack, 4-bit experts of a
+    prompt and of its last token alone, LM head, processed logits, top-k.  Each
+    step is checked against 64 bits on what the step before it gave."""
+    L, rng = gpu, np.random.default_rng(31)
+    T, E, K, H, F, V = 150, 12, 3, 256, 96, 500
+    t = lambda *n, dtype=torch.float32: torch.zeros(n, dtype=dtype, device="cuda")  # noqa: E731
+    i32, u8 = torch.int32, torch.uint8
+    x = dev(rng.standard_normal((T, H)).astype(np.float32))
+    wr = dev(rng.standard_normal((E, H)).astype(np.float32) / 16)
+    gu = [dev(a) for a in ref.quant(rng.standard_normal((E * 2 * F, H)) / 16)]
+    dn = [dev(a) for a in ref.quant(rng.standard_normal((E * H, F)) / 10)]
+    lm = [dev(a) for a in ref.quant(rng.standard_normal((V, H)) / 16)]
+    guv = ref.values(*map(host, gu), H).reshape(E, 2 * F, H)
+    dnv = ref.values(*map(host, dn), F).reshape(E, H, F)
+    lmv = ref.values(*map(host, lm), H)
+
+    def experts(w, rows, cols):
+        return (w[0].data_ptr(), w[1].data_ptr(), rows, cols, rows * w[0].shape[1],
+                rows * w[1].shape[1], E)
+
+    logits, ids, wts = t(T, E), t(T, K, dtype=i32), t(T, K)
+    q4mi.check(L.q4mi_moe_route(wr.data_ptr(), 0, None, x.data_ptr(), T, H, E, K,
+                                logits.data_ptr(), ids.data_ptr(), wts.data_ptr(), None, K, -1,
+                                None), "route")
+    R = T * K
+    atok, rsrc, rw, bounds = t(R, dtype=i32), t(R, dtype=i32), t(R), t(E + 1, dtype=i32)
+    stg, stgn, ek = t(512, dtype=i32), t(1, dtype=i32), t(512, dtype=i32)
+    q4mi.check(L.q4mi_assign(ids.data_ptr(), wts.data_ptr(), atok.data_ptr(), rsrc.data_ptr(),
+                             rw.data_ptr(), stg.data_ptr(), stgn.data_ptr(), ek.data_ptr(),
+                             bounds.data_ptr(), T, K, E, T), "pack")
+    xq, xs = quant(L, x, 0, H, T, H)
+    g, h, pd, y = t(R, 2 * F), t(R, F), t(R, H), t(T, H)
+    q4mi.check(L.q4mi_mx4_mul_id(*experts(gu, 2 * F, H), xq.data_ptr(), xs.data_ptr(), T,
+                                 atok.data_ptr(), bounds.data_ptr(), R, g.data_ptr(), 0, 2 * F),
+               "gate/up")
+    q4mi.check(L.q4_mmq_swiglu(g.data_ptr(), h.data_ptr(), R, F), "swiglu")
+    hq, hs = quant(L, h, 0, F, R, F)
+    q4mi.check(L.q4mi_mx4_mul_id(*experts(dn, H, F), hq.data_ptr(), hs.data_ptr(), R, None,
+                                 bounds.data_ptr(), R, pd.data_ptr(), 0, H), "down")
+    q4mi.check(L.q4_hip_expert_reduce(y.data_ptr(), pd.data_ptr(), rsrc.data_ptr(), rw.data_ptr(),
+                                      T, K, H), "reduce")
+    e = np.repeat(np.arange(E), np.diff(host(bounds)))
+    xv = ref.values(*ref.quant(host(x)), H)[host(atok)]
+    close(g, np.einsum("prc,pc->pr", guv[e], xv), np.einsum("prc,pc->pr", abs(guv[e]), abs(xv)), H,
+          torch.float32)
+    want = ref.quant(host(h))
+    assert np.array_equal(host(hq), want[0]) and np.array_equal(host(hs), want[1])
+    hv = ref.values(*want, F)
+    close(pd, np.einsum("prc,pc->pr", dnv[e], hv), np.einsum("prc,pc->pr", abs(dnv[e]), abs(hv)),
+          F, torch.float32)
+
+    # the last token alone, as a decode step: float rows in, the router's list
+    one = x[T - 1:]
+    g1, h1, d1 = t(K, 2 * F), t(K, F), t(K, H)
+    q4mi.check(L.q4mi_mx4_mul_sel(*experts(gu, 2 * F, H), one.data_ptr(), None, 0, H, K,
+                                  ids[T - 1].data_ptr(), K, g1.data_ptr(), 0, 2 * F), "gate/up")
+    q4mi.check(L.q4_mmq_swiglu(g1.data_ptr(), h1.data_ptr(), K, F), "swiglu")
+    q4mi.check(L.q4mi_mx4_mul_sel(*experts(dn, H, F), h1.data_ptr(), None, 0, F, 1,
+                                  ids[T - 1].data_ptr(), K, d1.data_ptr(), 0, H), "down")
+    pick = host(ids)[T - 1]
+    xv1 = ref.values(*ref.quant(host(one)), H)[0]
+    close(g1, guv[pick] @ xv1, abs(guv[pick]) @ abs(xv1), H, torch.float32)
+    hv1 = ref.values(*ref.quant(host(h1)), F)
+    close(d1, np.einsum("prc,pc->pr", dnv[pick], hv1),
+          np.einsum("prc,pc->pr", abs(dnv[pick]), abs(hv1)), F, torch.float32)
+    at = host(rsrc).reshape(T, K)[T - 1]
+    # the same rows of the prompt's pass, where no sum came out another way
+    same = np.array_equal(host(g)[at], host(g1))
+    if same:
+        assert np.array_equal(ref.quant(host(h)[at])[0], ref.quant(host(h1))[0])
+
+    # LM head on the last two tokens, penalties and a mask, then the best token
+    z, out = t(2, V), t(2, V)
+    q4mi.check(L.q4mi_mx4_mul(lm[0].data_ptr(), lm[1].data_ptr(), V, H, y[T - 2:].data_ptr(), None,
+                              0, H, 2, z.data_ptr(), 0, V), "LM head")
+    yv = ref.values(*ref.quant(host(y[T - 2:])), H)
+    close(z, yv @ lmv.T, abs(yv) @ abs(lmv).T, H, torch.float32)
+    best = host(z).argmax(1)
+    hist, off = dev(best.astype(np.int32)), dev(np.array([0, 1, 2], np.int64))
+    pen = dev(np.array([[1.0, 100.0, 0.0], [1.0, 0.0, 0.0]], np.float32))
+    mask = np.full((1, (V + 31) // 32), 0xffffffff, np.uint32)
+    mask[0, best[1] // 32] &= ~np.uint32(1 << (best[1] % 32))
+    dm, dr = dev(mask.view(np.int32)), dev(np.array([-1, 0], np.int32))
+    q4mi.check(L.q4mi_logits_process(z.data_ptr(), 0, V, 2, V, hist.data_ptr(), off.data_ptr(),
+                                     None, pen.data_ptr(), None, None, None, dm.data_ptr(),
+                                     mask.shape[1], 1, dr.data_ptr(), out.data_ptr(), V), "logits")
+    zh, got = host(z), host(out)
+    # tokens the model wrote count from the start of the history without gen
+    want = zh.copy()
+    want[0, best[0]] = np.float32(zh[0, best[0]] - np.float32(100))
+    want[1, best[1]] = -np.inf
+    assert np.array_equal(got, want)
+    top, tw = t(2, 1, dtype=i32), t(2, 1)
+    q4mi.check(L.q4_hip_route_pf(out.data_ptr(), top.data_ptr(), tw.data_ptr(), 2, V, 1), "top-k")
+    assert np.array_equal(host(top)[:, 0], want.argmax(1))
 
 
 # ---------------------------------------------------------- streams and graphs
