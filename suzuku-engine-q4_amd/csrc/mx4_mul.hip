@@ -13,6 +13,7 @@ namespace {
 
 typedef int v8i __attribute__((ext_vector_type(8)));
 typedef float v4f __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef u32x4 u32x4_a4 __attribute__((aligned(4)));   // in memory at any dword
 
@@ -35,15 +36,22 @@ __device__ inline v8i widen(u32x4 q) {
     return a;
 }
 
-// Four adjacent outputs, rounded once; `at` a multiple of 4.
+// Four adjacent outputs, rounded once; `at` a multiple of 4.  STREAM: past the
+// caches.
+template <bool STREAM = false>
 __device__ inline void store4(void *y, uint32_t yt, uint64_t at, v4f v) {
-    if (yt == kTypeF32) {
-        *(v4f *)((float *)y + at) = v;
-    } else {
-        const uint32_t lo = f32_to_16(v[0], yt) | (uint32_t)f32_to_16(v[1], yt) << 16;
-        const uint32_t hi = f32_to_16(v[2], yt) | (uint32_t)f32_to_16(v[3], yt) << 16;
-        *(uint2 *)((uint16_t *)y + at) = make_uint2(lo, hi);
-    }
+    auto put = [](auto *p, auto q) __attribute__((always_inline)) {
+        if constexpr (STREAM)
+            __builtin_nontemporal_store(q, p);
+        else
+            *p = q;
+    };
+    if (yt == kTypeF32)
+        put((v4f *)((float *)y + at), v);
+    else
+        put((u32x2 *)((uint16_t *)y + at),
+            (u32x2){f32_to_16(v[0], yt) | (uint32_t)f32_to_16(v[1], yt) << 16,
+                    f32_to_16(v[2], yt) | (uint32_t)f32_to_16(v[3], yt) << 16});
 }
 
 // ---------------------------------------------------------------- few rows
@@ -561,9 +569,16 @@ __device__ inline void tile(const MulArgs &a, const uint8_t *w, const uint8_t *w
     // so that a wave stores whole stretches of an output row: lane (row lr, h)
     // holds weight rows 8q + 4h + 0..3 of its fragments.
     constexpr uint32_t kRow = FN * 32 + 4, kLanes = FN * 8;   // floats a row, lanes that store one
+    // The largest tile is for outputs that the caches do not hold (16384 x 2048
+    // over 8192 rows, bf16 out: 215 us through them, 210 past them).
+    constexpr bool kStream = BM * BN >= 65536;
     static_assert(NW * 32 * kRow * 4 <= tile_lds<BM, BN>(), "sums fit the stages");
     float *sums = (float *)lds + wave * 32 * kRow;
     const uint64_t rw = r0 + wn * FN * 32 + lane % kLanes * 4;   // weight row of this lane's stores
+    const bool whole = a.y_wide && r0 + (wn + 1) * FN * 32 <= a.w_rows;
+    auto listed = [&](int64_t p) {      // whether row p has an activation row
+        return !GATHER || !a.act || (a.act[p] >= 0 && (int64_t)a.act[p] < (int64_t)a.xrows);
+    };
     __syncthreads();
 #pragma unroll
     for (uint32_t i = 0; i < FM; i++) {
@@ -575,18 +590,28 @@ __device__ inline void tile(const MulArgs &a, const uint8_t *w, const uint8_t *w
                     (v4f){acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2],
                           acc[i][j][4 * q + 3]};
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        const int64_t p1 = p0 + (wm * FM + i) * 32;
+        if (whole && p1 + 32 <= phi) {
+            constexpr uint32_t kStep = 64 / kLanes;
+#pragma unroll
+            for (uint32_t u = 0; u < 32 / kStep; u++) {
+                const uint32_t m = u * kStep + lane / kLanes;
+                const v4f v = *(const v4f *)(sums + m * kRow + lane % kLanes * 4);
+                if (listed(p1 + m)) store4<kStream>(a.y, a.y_type, (p1 + m) * a.ldy + rw, v);
+            }
+        } else {
 #pragma unroll 1
-        for (uint32_t m = lane / kLanes; m < 32; m += 64 / kLanes) {
-            const int64_t p = p0 + (wm * FM + i) * 32 + m;
-            if (p >= phi) break;
-            if (GATHER && a.act && (a.act[p] < 0 || (int64_t)a.act[p] >= (int64_t)a.xrows)) continue;
-            const v4f v = *(const v4f *)(sums + m * kRow + lane % kLanes * 4);
-            const uint64_t at = p * a.ldy + rw;
-            if (a.y_wide && rw + 4 <= a.w_rows)
-                store4(a.y, a.y_type, at, v);
-            else
-                for (uint32_t n = 0; n < 4; n++)
-                    if (rw + n < a.w_rows) store_from_f32(a.y, a.y_type, at + n, v[n]);
+            for (uint32_t m = lane / kLanes; m < 32 && p1 + m < phi; m += 64 / kLanes) {
+                const int64_t p = p1 + m;
+                if (!listed(p)) continue;
+                const v4f v = *(const v4f *)(sums + m * kRow + lane % kLanes * 4);
+                const uint64_t at = p * a.ldy + rw;
+                if (a.y_wide && rw + 4 <= a.w_rows)
+                    store4(a.y, a.y_type, at, v);
+                else
+                    for (uint32_t n = 0; n < 4; n++)
+                        if (rw + n < a.w_rows) store_from_f32(a.y, a.y_type, at + n, v[n]);
+            }
         }
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     }
@@ -766,7 +791,7 @@ bool mul_ok(const char *who, const MulArgs &a) {
     return true;
 }
 
-// Whether float and output rows can move 16 bytes at a time.
+// How float and output rows move.
 void wide_rows(MulArgs &a) {
     a.x_wide = is_float_type(a.x_type) && !((uintptr_t)a.x & 15) &&
                a.ldx * type_bytes(a.x_type) % 16 == 0;
