@@ -428,8 +428,9 @@ bool q4mi_mx4_mul_sel(const uint8_t *d_w, const uint8_t *d_ws, uint64_t w_rows, 
                       uint64_t ld_y);
 /* Routed experts of a prompt: packed rows bounds[e] .. bounds[e+1] go through
  * expert e, packed row p reading x row act_row ? act_row[p] : p (of xrows);
- * bounds and act_row as q4mi_assign writes them.  Rows outside every stretch,
- * past total_rows or with act_row outside 0..xrows-1 are left as they were. */
+ * bounds (ascending) and act_row as q4mi_assign writes them; n_expert <= 1024.
+ * Rows outside every stretch, past total_rows or with act_row outside
+ * 0..xrows-1 are left as they were. */
 bool q4mi_mx4_mul_id(const uint8_t *d_w, const uint8_t *d_ws, uint64_t w_rows, uint64_t cols,
                      uint64_t w_stride, uint64_t ws_stride, uint32_t n_expert, const uint8_t *d_xq,
                      const uint8_t *d_xs, uint64_t xrows, const int32_t *d_act_row,

@@ -184,7 +184,8 @@ __global__ __launch_bounds__(kThreads) void logits_k(LogitsArgs a) {
     };
     float z[NG][4];
 #pragma unroll
-    for (uint32_t n = 0; n < NG; n++) z[n][0] = x[n].x, z[n][1] = x[n].y, z[n][2] = x[n].z, z[n][3] = x[n].w;
+    for (uint32_t n = 0; n < NG; n++)
+        z[n][0] = x[n].x, z[n][1] = x[n].y, z[n][2] = x[n].z, z[n][3] = x[n].w;
     if (counted) {
         clear();
         count_history(a, b, v0, nv, lds);

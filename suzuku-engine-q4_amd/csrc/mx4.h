@@ -21,7 +21,9 @@ constexpr bool is_float_type(uint32_t t) {
 }
 constexpr uint32_t type_bytes(uint32_t t) { return t == kTypeF32 ? 4u : 2u; }
 
-__host__ __device__ inline uint32_t mx4_blocks(uint64_t cols) { return (uint32_t)((cols + 31) / 32); }
+__host__ __device__ inline uint32_t mx4_blocks(uint64_t cols) {
+    return (uint32_t)((cols + 31) / 32);
+}
 __host__ __device__ inline uint32_t mx4_scale_row(uint32_t nb) { return (nb + 3u) & ~3u; }
 
 __device__ inline float bits_f32(uint32_t u) { return __builtin_bit_cast(float, u); }
@@ -65,7 +67,9 @@ __device__ inline uint32_t mx4_scale_of(uint32_t top) {
 // Factor that takes the block's values to the codes' range: 2^(127 - s), a
 // normal fp32 for every scale byte that mx4_scale_of gives; 0 for a block
 // without finite values, whose codes are 0.
-__device__ inline float mx4_factor(uint32_t s) { return s == 255u ? 0.f : bits_f32((254u - s) << 23); }
+__device__ inline float mx4_factor(uint32_t s) {
+    return s == 255u ? 0.f : bits_f32((254u - s) << 23);
+}
 
 // Two scaled values as codes, in byte `SEL` of `old`: to nearest, ties to the
 // even code, at most 6 in magnitude.
@@ -119,16 +123,15 @@ __device__ inline void load_row8(const void *x, uint32_t xt, uint64_t row, uint3
     }
 }
 
-// Codes of this lane's eight values of a block that four adjacent lanes hold,
-// and the block's scale byte.
-__device__ inline uint32_t mx4_quant8(const float *v, uint32_t *s) {
+// Scale byte of a block of which 32 / N adjacent lanes hold N values each.
+template <uint32_t N>
+__device__ inline uint32_t mx4_block_scale(const float *v) {
     uint32_t top = 0;
 #pragma unroll
-    for (int i = 0; i < 8; i++) top = max(top, f32_bits(v[i]) & 0x7fffffffu);
-    top = max(top, (uint32_t)__shfl_xor((int)top, 1, 64));
-    top = max(top, (uint32_t)__shfl_xor((int)top, 2, 64));
-    *s = mx4_scale_of(top);
-    return mx4_pack8(v, *s);
+    for (uint32_t i = 0; i < N; i++) top = max(top, f32_bits(v[i]) & 0x7fffffffu);
+#pragma unroll
+    for (uint32_t d = 1; d < 32 / N; d *= 2) top = max(top, (uint32_t)__shfl_xor((int)top, d, 64));
+    return mx4_scale_of(top);
 }
 
 // 2^(s - 127) as fp32 (a subnormal for s = 0), NaN for 255.

@@ -1,7 +1,13 @@
 // Products of microscaled 4-bit rows (mx4.h has the format):
 //   y[t][r] = sum over blocks b of 2^(sw + sx - 254) * sum_i w[r][32b+i] x[t][32b+i]
-// on v_mfma_scale_f32_16x16x128_f8f6f4, whose lane (row m, group g) takes one
-// block of 32 codes and its scale byte, and which adds in fp32.
+// on v_mfma_scale_f32_16x16x128_f8f6f4 and _32x32x64_f8f6f4: a lane holds one
+// row's block of 32 codes and its scale byte, the sums are fp32.  Weight rows
+// are the first operand, so a lane's sums are four adjacent outputs of one
+// activation row.
+//
+// Three kernels: few rows (weights straight to registers), rows in tiles (both
+// sides through LDS) and packed rows (both of these, per expert).
+#include <algorithm>
 #include <type_traits>
 
 #include "mx4.h"
@@ -26,7 +32,7 @@ struct MulArgs {
     void *y;
     uint64_t w_rows, cols, w_stride, ws_stride, ldx, xrows, n, ldy;
     uint32_t n_expert, x_type, y_type, x_div;
-    uint32_t ks, seg, blocks;       // waves a tile, blocks of K in LDS, workgroups along the weights
+    uint32_t ks, seg, blocks;       // waves a tile, blocks of K in LDS, workgroups
     uint32_t m_tiles;               // tiles along the activations
     bool x_wide, y_wide;            // whether rows can move 16 bytes at a time
 };
@@ -61,12 +67,14 @@ __device__ inline void store4(void *y, uint32_t yt, uint64_t at, v4f v) {
 // registers; lane (m, g) of it holds row m's blocks 4s + g of a chunk of 16
 // blocks (s = 0..3), so four lanes read 64 adjacent bytes and a chunk's 16
 // scales are one 16-byte load, of which step s uses byte g of dword s.  PF
-// chunks (4 KB each with 16 rows) are multiplied while PF more are in flight.  The activation rows
-// sit in LDS, as codes, in groups of 16 for one instruction each: float rows
-// are quantised on the way there, once a workgroup.  ks waves share a tile
-// along K and their sums are joined in LDS in wave order, so a short matrix
-// still occupies the chip; a workgroup goes over several tiles, so a tall one
-// pays the LDS fill once.
+// chunks (4 KB each with 16 rows) are multiplied while PF more are in flight.
+// The activation rows sit in LDS, as codes, in groups of 16 for one instruction
+// each: float rows are quantised on the way there, once a workgroup.  ks waves
+// share a tile along K and their sums are joined in LDS in wave order, so a
+// short matrix still occupies the chip; a workgroup goes over several tiles, so
+// a tall one pays the LDS fill once.  LM head 151936 x 2048, one row: 30 us,
+// 5.6 TB/s with part of the weights in the last cache; from memory alone 4.4
+// TB/s for 16 rows (a large copy: 4.8).
 
 // LDS strides of a row's codes and scales, seg blocks: 16 bytes more than a
 // power of two, so that the rows of a fragment start in different banks.
@@ -117,7 +125,8 @@ __device__ inline void few_stage(const MulArgs &a, const FewRange &f, uint32_t b
             float v[8];
             load_row8(a.x, a.x_type, (uint64_t)f.x_row(t, a.xrows) * a.ldx,
                       32u * (b0 + b) + 8u * sub, (uint32_t)a.cols, a.x_wide, v);
-            code = mx4_quant8(v, &s);
+            s = mx4_block_scale<8>(v);
+            code = mx4_pack8(v, s);
         }
         *(uint32_t *)(codes + t * cld + 16u * b + 4u * sub) = code;
         if (sub == 0) scales[t * scld + b] = (uint8_t)s;
@@ -392,7 +401,8 @@ __device__ inline void tile(const MulArgs &a, const uint8_t *w, const uint8_t *w
     const uint32_t c0 = (lane & 7u) ^ (l8 >> 1);        // chunk of an even copy; c0 ^ 4 of an odd
     auto fetch = [&](uint32_t k, uint32_t i) __attribute__((always_inline)) {
         const uint32_t to = base + (k & 1u) * kStage;
-        const uint32_t at[2] = {16u * min(8 * k + c0, nb - 1), 16u * min(8 * k + (c0 ^ 4u), nb - 1)};
+        const uint32_t at[2] = {16u * min(8 * k + c0, nb - 1),
+                                16u * min(8 * k + (c0 ^ 4u), nb - 1)};
 #pragma unroll
         for (uint32_t j = 0; j < RA; j++) {
             if (j % FM != i) continue;
@@ -475,7 +485,8 @@ __device__ inline void tile(const MulArgs &a, const uint8_t *w, const uint8_t *w
 #pragma unroll
         for (uint32_t j = 0; j < FN; j++) sw[j] = one(BM + rb + 32 * j, rb + 32 * j);
     };
-    auto read_codes = [&](uint32_t k, uint32_t s, u32x4 *xq, u32x4 *wq) __attribute__((always_inline)) {
+    auto read_codes = [&](uint32_t k, uint32_t s, u32x4 *xq, u32x4 *wq)
+        __attribute__((always_inline)) {
         const uint8_t *st = lds + (k & 1u) * kStage + off[s];
 #pragma unroll
         for (uint32_t i = 0; i < FM; i++) xq[i] = *(const u32x4 *)(st + (ra + 32 * i) * 128);
@@ -632,23 +643,27 @@ __global__ __launch_bounds__(64 * WM * WN, WAVES) void mx4_dense_k(MulArgs a) {
     const uint32_t group = t / (kGroup * n_tiles), in = t - group * kGroup * n_tiles;
     const uint32_t gm = min(kGroup, a.m_tiles - group * kGroup);
     const uint32_t mt = group * kGroup + in % gm, nt = in / gm;
-    tile<BM, BN, WM, WN, false>(a, a.w, a.ws, (uint64_t)nt * BN, (int64_t)mt * BM, (int64_t)a.n, lds);
+    tile<BM, BN, WM, WN, false>(a, a.w, a.ws, (uint64_t)nt * BN, (int64_t)mt * BM, (int64_t)a.n,
+                                lds);
 }
 
 // ------------------------------------------------------------- packed rows
 //
 // Experts differ: of a prompt's, a few take most of the rows and many take a
-// handful.  One persistent workgroup a CU goes over a list of items: first
-// tiles of kIdM rows x kIdN weight rows of the experts with more than kIdFew
-// rows (bound by the matrix units), then the others' 16-row weight tiles, each
-// streamed once past all of its expert's rows (bound by memory).  Of the list
-// of those, expert by expert, a workgroup takes one stretch, so it stages few
-// experts' rows, and one shorter by kIdCost tiles for each of its large tiles.
-// Half of the workgroups begin with those, so that memory and matrix units work
-// at the same time.
-// Every workgroup makes the list by itself, as prefix sums over the experts'
-// stretches in LDS: no scratch in memory, no launch before, and no workgroups
-// that find nothing to do.
+// handful.  One persistent workgroup a CU goes over two lists: tiles of kIdM
+// rows x kIdN weight rows of the experts with more than kIdFew rows (bound by
+// the matrix units), and the other experts' 16-row weight tiles, each streamed
+// once past all of its expert's rows (bound by memory).  Of the second list a
+// workgroup takes one stretch, so that it stages few experts' rows, shorter by
+// kIdCost tiles for each large tile that it has (22 of them take as long as
+// one; 512 experts' 1024 x 2048 over 2048 tokens: 188 us at 11, 180 at 22).
+// Every second workgroup begins with the streamed tiles, so that memory and
+// matrix units work at the same time (192 us all alike, 185 so).
+//
+// Every workgroup makes the lists by itself, as prefix sums over the experts'
+// stretches in LDS (under 5 us with nothing to do): no scratch in memory, no
+// launch before, and no workgroups that find nothing to do, of which a grid
+// over experts, slices and tiles has tens of thousands (347 us).
 constexpr uint32_t kIdM = 128, kIdN = 256, kIdWM = 2, kIdWN = 4, kIdWaves = kIdWM * kIdWN;
 constexpr uint32_t kIdFew = 32, kIdExperts = 1024, kIdCost = 22;
 constexpr size_t kIdLists = 2 * (kIdExperts + 1) * 4;

@@ -4,79 +4,113 @@
 // RNE(x / 2^s) capped at 6.  The scale is a power of two, so x / 2^s is exact
 // wherever a code other than 0 can come of it, and the codes depend on
 // nothing but the 32 values.
+#include <algorithm>
+
 #include "mx4.h"
 #include "q4mi_internal.h"
 
 using namespace q4mi;
 
-// Four lanes a block, eight values a lane; a 256-thread workgroup takes 64
-// successive blocks of the row-major block order.  VEC: rows are 16-byte
-// aligned and whole, so a lane's values come in 16-byte loads.
-template <bool VEC>
+// Place of a thread's block: `off` blocks past the first of the `each` (64 or
+// 128) that the workgroup takes in the row-major order of all rows' blocks,
+// off < each.  Workgroups
+// with one blockIdx.y share a group of whole rows with fewer than 2^31 blocks,
+// so that the divisions stay in 32 bits.
+struct Place {
+    uint64_t r;
+    uint32_t b;
+    __device__ Place(uint32_t each, uint64_t group, uint32_t off, uint32_t nb) {
+        const uint32_t base = blockIdx.x * each, r0 = base / nb;
+        b = base - r0 * nb + off;
+        // a row of `each` blocks or more: at most one row further
+        const uint32_t q = nb >= each ? (b >= nb ? 1u : 0u) : b / nb;
+        b -= q * nb;
+        const uint32_t in = r0 + q;
+        r = in < group ? blockIdx.y * group + in : ~0ull;
+    }
+};
+
+// N values a lane, 32 / N lanes a block: 32 bytes of input, eight fp32 or
+// sixteen 16-bit values.  VEC: rows are 16-byte aligned, so they come in
+// 16-byte loads.
+template <bool VEC, uint32_t N>
 __global__ __launch_bounds__(256) void mx4_quant_k(const void *__restrict__ x, uint32_t xt,
                                                    uint64_t ld, const int32_t *__restrict__ ids,
-                                                   uint64_t rows, uint32_t cols,
+                                                   uint64_t rows, uint64_t group, uint32_t cols,
                                                    uint8_t *__restrict__ codes,
                                                    uint8_t *__restrict__ scales) {
-    const uint32_t nb = mx4_blocks(cols), sld = mx4_scale_row(nb);
-    const uint64_t base = (uint64_t)blockIdx.x * 64;
-    const uint32_t off = (uint32_t)(base % nb) + (threadIdx.x >> 2);
-    const uint64_t r = base / nb + off / nb;
-    if (r >= rows) return;
-    const uint32_t b = off % nb, sub = threadIdx.x & 3u;
-    const uint64_t src = ids ? (uint64_t)(int64_t)ids[r] : r;
-    const uint32_t c0 = b * 32 + sub * 8;
-    float v[8];
-    load_row8(x, xt, src * ld, c0, cols, VEC, v);
-    uint32_t s;
-    const uint32_t q = mx4_quant8(v, &s);
-    *(uint32_t *)(codes + r * (16ull * nb) + b * 16u + sub * 4u) = q;
+    constexpr uint32_t L = 32 / N;
+    const uint32_t nb = mx4_blocks(cols), sld = mx4_scale_row(nb), sub = threadIdx.x % L;
+    const Place p(256 / L, group, threadIdx.x / L, nb);
+    if (p.r >= rows) return;
+    const uint64_t src = ids ? (uint64_t)(int64_t)ids[p.r] : p.r;
+    float v[N];
+#pragma unroll
+    for (uint32_t i = 0; i < N; i += 8)
+        load_row8(x, xt, src * ld, p.b * 32 + sub * N + i, cols, VEC, v + i);
+    const uint32_t s = mx4_block_scale<N>(v);
+    uint32_t *c = (uint32_t *)(codes + p.r * (16ull * nb) + p.b * 16u + sub * (N / 2));
+    if constexpr (N == 16)
+        *(uint2 *)c = make_uint2(mx4_pack8(v, s), mx4_pack8(v + 8, s));
+    else
+        *c = mx4_pack8(v, s);
     if (sub == 0) {
-        uint8_t *p = scales + r * sld;
-        p[b] = (uint8_t)s;
-        if (b == nb - 1)
-            for (uint32_t i = nb; i < sld; i++) p[i] = 0;
+        uint8_t *d = scales + p.r * sld;
+        d[p.b] = (uint8_t)s;
+        if (p.b == nb - 1)
+            for (uint32_t i = nb; i < sld; i++) d[i] = 0;
     }
 }
 
-// The mirror: four lanes a block, eight values a lane.
-template <bool VEC>
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
+// The mirror, G values a lane (32 / G lanes a block), so that a lane's values
+// are 16 bytes of output and a wave's one stretch: eight for 16-bit outputs,
+// four for fp32.  Past the caches, which the values would only pass through
+// (8192 x 8192 to bf16: 47 us through them, 33 past them).
+template <bool VEC, uint32_t G>
 __global__ __launch_bounds__(256) void mx4_dequant_k(const uint8_t *__restrict__ codes,
                                                      const uint8_t *__restrict__ scales,
                                                      const int32_t *__restrict__ ids,
-                                                     uint64_t rows, uint32_t cols,
-                                                     void *__restrict__ y, uint32_t yt,
-                                                     uint64_t ld) {
-    const uint32_t nb = mx4_blocks(cols), sld = mx4_scale_row(nb);
-    const uint64_t base = (uint64_t)blockIdx.x * 64;
-    const uint32_t off = (uint32_t)(base % nb) + (threadIdx.x >> 2);
-    const uint64_t r = base / nb + off / nb;
-    if (r >= rows) return;
-    const uint32_t b = off % nb, sub = threadIdx.x & 3u;
-    const uint64_t src = ids ? (uint64_t)(int64_t)ids[r] : r;
-    const uint32_t q = *(const uint32_t *)(codes + src * (16ull * nb) + b * 16u + sub * 4u);
-    const float f = mx4_scale_value(scales[src * sld + b]);
-    const mx4_f2 p0 = mx4_unpack2<0>(q), p1 = mx4_unpack2<1>(q), p2 = mx4_unpack2<2>(q),
-                 p3 = mx4_unpack2<3>(q);
-    const float v[8] = {p0.x * f, p0.y * f, p1.x * f, p1.y * f,
-                        p2.x * f, p2.y * f, p3.x * f, p3.y * f};
-    const uint32_t c0 = b * 32 + sub * 8;
-    const uint64_t at = r * ld + c0;
-    if (VEC && c0 + 8 <= cols) {
-        if (yt == kTypeF32) {
-            *(float4 *)((float *)y + at) = make_float4(v[0], v[1], v[2], v[3]);
-            *(float4 *)((float *)y + at + 4) = make_float4(v[4], v[5], v[6], v[7]);
-        } else {
-            uint32_t w[4];
+                                                     uint64_t rows, uint64_t group,
+                                                     uint32_t cols, void *__restrict__ y,
+                                                     uint32_t yt, uint64_t ld) {
+    constexpr uint32_t L = 32 / G, U = 8 / G;       // lanes a block; sets of blocks a workgroup
+    const uint32_t nb = mx4_blocks(cols), sld = mx4_scale_row(nb), sub = threadIdx.x % L;
 #pragma unroll
-            for (int i = 0; i < 4; i++)
-                w[i] = f32_to_16(v[2 * i], yt) | (uint32_t)f32_to_16(v[2 * i + 1], yt) << 16;
-            *(uint4 *)((uint16_t *)y + at) = make_uint4(w[0], w[1], w[2], w[3]);
+    for (uint32_t u = 0; u < U; u++) {
+        const Place p(64, group, 256 / L * u + threadIdx.x / L, nb);
+        if (p.r >= rows) continue;
+        const uint64_t src = ids ? (uint64_t)(int64_t)ids[p.r] : p.r;
+        const uint8_t *c = codes + src * (16ull * nb) + p.b * 16u + sub * (G / 2);
+        const float f = mx4_scale_value(scales[src * sld + p.b]);
+        const uint32_t c0 = p.b * 32 + sub * G;
+        const uint64_t at = p.r * ld + c0;
+        float v[G];
+        const uint32_t q = G == 8 ? *(const uint32_t *)c : (uint32_t)*(const uint16_t *)c;
+        const mx4_f2 p0 = mx4_unpack2<0>(q), p1 = mx4_unpack2<1>(q);
+        v[0] = p0.x * f, v[1] = p0.y * f, v[2] = p1.x * f, v[3] = p1.y * f;
+        if constexpr (G == 8) {
+            const mx4_f2 p2 = mx4_unpack2<2>(q), p3 = mx4_unpack2<3>(q);
+            v[4] = p2.x * f, v[5] = p2.y * f, v[6] = p3.x * f, v[7] = p3.y * f;
         }
-    } else {
+        if (VEC && c0 + G <= cols) {
+            if constexpr (G == 4) {
+                __builtin_nontemporal_store((f32x4){v[0], v[1], v[2], v[3]},
+                                            (f32x4 *)((float *)y + at));
+            } else {
+                u32x4 w;
 #pragma unroll
-        for (uint32_t i = 0; i < 8; i++)
-            if (c0 + i < cols) store_from_f32(y, yt, at + i, v[i]);
+                for (int i = 0; i < 4; i++)
+                    w[i] = f32_to_16(v[2 * i], yt) | (uint32_t)f32_to_16(v[2 * i + 1], yt) << 16;
+                __builtin_nontemporal_store(w, (u32x4 *)((uint16_t *)y + at));
+            }
+        } else {
+#pragma unroll
+            for (uint32_t i = 0; i < G; i++)
+                if (c0 + i < cols) store_from_f32(y, yt, at + i, v[i]);
+        }
     }
 }
 
@@ -93,7 +127,7 @@ bool rows_ok(const char *who, const void *f, uint32_t type, uint64_t ld, uint64_
         set_error("%s: type %u not covered (F32, F16, BF16)", who, type);
         return false;
     }
-    if (cols > (1u << 30) || rows > (1ull << 32) || rows * mx4_blocks(cols) > (uint64_t)0x7fffffffu * 64) {
+    if (cols > (1u << 30) || rows > (1ull << 32) || rows * mx4_blocks(cols) > (1ull << 45)) {
         set_error("%s: %llu x %llu too large", who, (unsigned long long)rows,
                   (unsigned long long)cols);
         return false;
@@ -117,6 +151,14 @@ bool wide(const void *f, uint32_t type, uint64_t ld) {
     return !((uintptr_t)f & 15) && ld * type_bytes(type) % 16 == 0;
 }
 
+// `each` blocks a workgroup over groups of whole rows (see Place).
+dim3 block_grid(uint32_t each, uint64_t rows, uint64_t cols, uint64_t *group) {
+    const uint32_t nb = mx4_blocks(cols);
+    *group = std::min<uint64_t>(rows, ((1u << 31) - each) / nb);
+    return dim3((uint32_t)((*group * nb + each - 1) / each),
+                (uint32_t)((rows + *group - 1) / *group));
+}
+
 }  // namespace
 
 extern "C" {
@@ -134,10 +176,13 @@ bool q4mi_mx4_quant(const void *d_x, uint32_t x_type, uint64_t ld_x, const int32
                     uint64_t rows, uint64_t cols, uint8_t *d_codes, uint8_t *d_scales) {
     if (!rows_ok("q4mi_mx4_quant", d_x, x_type, ld_x, rows, cols, d_codes, d_scales)) return false;
     if (!rows) return true;
-    const uint32_t grid = (uint32_t)((rows * mx4_blocks(cols) + 63) / 64);
-    auto k = wide(d_x, x_type, ld_x) ? mx4_quant_k<true> : mx4_quant_k<false>;
-    k<<<dim3(grid), dim3(256), 0, stream()>>>(d_x, x_type, ld_x, d_ids, rows, (uint32_t)cols,
-                                              d_codes, d_scales);
+    uint64_t group;
+    const bool f32 = x_type == kTypeF32;
+    const dim3 grid = block_grid(f32 ? 64 : 128, rows, cols, &group);
+    auto k = f32 ? (wide(d_x, x_type, ld_x) ? mx4_quant_k<true, 8> : mx4_quant_k<false, 8>)
+                 : (wide(d_x, x_type, ld_x) ? mx4_quant_k<true, 16> : mx4_quant_k<false, 16>);
+    k<<<grid, dim3(256), 0, stream()>>>(d_x, x_type, ld_x, d_ids, rows, group, (uint32_t)cols,
+                                        d_codes, d_scales);
     return launch_ok("mx4_quant_k");
 }
 
@@ -147,10 +192,13 @@ bool q4mi_mx4_dequant(const uint8_t *d_codes, const uint8_t *d_scales, const int
     if (!rows_ok("q4mi_mx4_dequant", d_y, y_type, ld_y, rows, cols, d_codes, d_scales))
         return false;
     if (!rows) return true;
-    const uint32_t grid = (uint32_t)((rows * mx4_blocks(cols) + 63) / 64);
-    auto k = wide(d_y, y_type, ld_y) ? mx4_dequant_k<true> : mx4_dequant_k<false>;
-    k<<<dim3(grid), dim3(256), 0, stream()>>>(d_codes, d_scales, d_ids, rows, (uint32_t)cols, d_y,
-                                              y_type, ld_y);
+    uint64_t group;
+    const dim3 grid = block_grid(64, rows, cols, &group);
+    auto k = y_type == kTypeF32
+                 ? (wide(d_y, y_type, ld_y) ? mx4_dequant_k<true, 4> : mx4_dequant_k<false, 4>)
+                 : (wide(d_y, y_type, ld_y) ? mx4_dequant_k<true, 8> : mx4_dequant_k<false, 8>);
+    k<<<grid, dim3(256), 0, stream()>>>(d_codes, d_scales, d_ids, rows, group, (uint32_t)cols, d_y,
+                                        y_type, ld_y);
     return launch_ok("mx4_dequant_k");
 }
 

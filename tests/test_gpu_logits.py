@@ -120,7 +120,8 @@ def make(rng, b, v, hmax, bmax, masks):
 @pytest.mark.parametrize("xt", sorted(TYPES))
 @pytest.mark.parametrize("b,v,pad,hmax,bmax", [
     (1, 1, 0, 5, 3), (1, 100, 0, 50, 10), (3, 32003, 5, 4000, 100), (5, 4096, 0, 300, 0),
-    (2, 4097, 7, 0, 700), (9, 1000, 24, 2000, 2000), (1, 151936, 0, 3000, 50)])
+    (2, 4097, 7, 0, 700), (9, 1000, 24, 2000, 2000), (1, 151936, 0, 3000, 50),
+    (3, 5001, 0, 600, 60), (4, 2047, 2, 100, 9), (130, 10000, 1, 300, 20), (40, 60001, 0, 900, 30)])
 def test_all_three(gpu, xt, b, v, pad, hmax, bmax):
     rng = np.random.default_rng(b * 100 + v)
     hist, gen, pen, bias, ms, rows = make(rng, b, v, hmax, bmax, 3)

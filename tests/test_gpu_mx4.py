@@ -336,8 +336,9 @@ def test_mul_sel_float_rows(gpu, xt):
 
 @pytest.mark.parametrize("counts,rows,cols,spare", [
     ([0, 5, 0, 17], 64, 96, 3), ([40], 33, 32, 0), ([1] * 20, 100, 640, 0), ([0, 0], 16, 32, 4),
-    ([130, 0, 300, 7, 64, 65], 272, 288, 9), ([500, 1], 1024, 512, 0), ([33, 260, 31], 520, 2048, 1),
-    ([3] * 64, 200, 1013, 2), ([32, 33, 31, 64, 16, 17], 90, 416, 0), ([1, 0, 2] * 341 + [5], 20, 64, 3),
+    ([130, 0, 300, 7, 64, 65], 272, 288, 9), ([500, 1], 1024, 512, 0),
+    ([33, 260, 31], 520, 2048, 1), ([3] * 64, 200, 1013, 2),
+    ([32, 33, 31, 64, 16, 17], 90, 416, 0), ([1, 0, 2] * 341 + [5], 20, 64, 3),
     ([20, 150], 50, 9000, 0), ([129] * 3, 600, 1056, 0)])
 @pytest.mark.parametrize("gather", [True, False])
 def test_mul_id_exact(gpu, counts, rows, cols, spare, gather):

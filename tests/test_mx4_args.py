@@ -25,7 +25,8 @@ def test_sizes():
 def test_reference_format():
     """Every code's value, the ties, the cap and the scale of known blocks."""
     x = np.zeros((1, 32))
-    x[0, :15] = [4, 0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5, 7.99, -0.25, -6, 0.2500001, 0.7499, 6.5, -5]
+    x[0, :15] = [4, 0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5, 7.99, -0.25, -6, 0.2500001, 0.7499, 6.5,
+                 -5]
     c, s = ref.quant(x)
     v = ref.values(c, s, 32)[0]
     assert s[0, 0] == 127
