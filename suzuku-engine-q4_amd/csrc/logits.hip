@@ -111,12 +111,13 @@ __device__ inline void count_history(const LogitsArgs &a, uint32_t b, uint32_t v
     }
 }
 
-// Sums of the row's biases in list order, by one wave: entries of one token
-// among 64 are taken in turn.
+// Sums of the row's biases in list order: every wave goes through the list and
+// adds those of the tokens that are its own (v modulo the waves), entries of
+// one token among 64 in turn.
 __device__ inline void sum_biases(const LogitsArgs &a, int64_t lo, int64_t hi, uint32_t v0,
                                   uint32_t nv, float *add) {
-    constexpr uint32_t U = 4;
-    const uint32_t lane = threadIdx.x & 63u;
+    constexpr uint32_t U = 4, W = kThreads / 64;
+    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
     for (int64_t i0 = lo; i0 < hi; i0 += 64 * U) {
         uint32_t t[U];
         float v[U];
@@ -129,7 +130,7 @@ __device__ inline void sum_biases(const LogitsArgs &a, int64_t lo, int64_t hi, u
 #pragma unroll
         for (uint32_t u = 0; u < U; u++) {
             const uint32_t at = t[u] - v0;
-            const bool in = at < nv;        // else another slice's, or no token
+            const bool in = at < nv && at % W == wave;  // else another's, or no token
             uint32_t turn = 0;
             for (uint64_t m = __ballot(in); m; m &= m - 1) {
                 const uint32_t l = (uint32_t)__builtin_ctzll(m);
@@ -207,7 +208,7 @@ __global__ __launch_bounds__(kThreads) void logits_k(LogitsArgs a) {
     }
     if (biased) {
         clear();    // each thread clears what it alone has read
-        if (tid < 64) sum_biases(a, blo, bhi, v0, nv, (float *)lds);
+        sum_biases(a, blo, bhi, v0, nv, (float *)lds);
         __syncthreads();
 #pragma unroll
         for (uint32_t n = 0; n < NG; n++) {

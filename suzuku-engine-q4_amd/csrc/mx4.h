@@ -91,20 +91,29 @@ __device__ inline uint32_t mx4_pack8(const float *v, uint32_t s) {
     return s == 255u ? 0u : q;
 }
 
-// Eight values of a float row from column c0 on (0 past cols); wide: the row
-// moves 16 bytes at a time.  row: index of the row's first element.
+// Vectors in memory at any address of their elements (global loads and stores
+// take 16 bytes at any of them).
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef f32x4 f32x4_a4 __attribute__((aligned(4)));
+typedef u32x4 u32x4_a4 __attribute__((aligned(4)));
+typedef u32x4 u32x4_a2 __attribute__((aligned(2)));
+typedef u32x2 u32x2_a2 __attribute__((aligned(2)));
+
+// Eight values of a float row from column c0 on (0 past cols).  row: index of
+// the row's first element.
 __device__ inline void load_row8(const void *x, uint32_t xt, uint64_t row, uint32_t c0,
-                                 uint32_t cols, bool wide, float *v) {
+                                 uint32_t cols, float *v) {
     const uint64_t at = row + c0;
-    if (wide && c0 + 8 <= cols) {
+    if (c0 + 8 <= cols) {
         if (xt == kTypeF32) {
-            const float4 lo = *(const float4 *)((const float *)x + at);
-            const float4 hi = *(const float4 *)((const float *)x + at + 4);
-            v[0] = lo.x, v[1] = lo.y, v[2] = lo.z, v[3] = lo.w;
-            v[4] = hi.x, v[5] = hi.y, v[6] = hi.z, v[7] = hi.w;
+            const f32x4 lo = *(const f32x4_a4 *)((const float *)x + at);
+            const f32x4 hi = *(const f32x4_a4 *)((const float *)x + at + 4);
+#pragma unroll
+            for (int i = 0; i < 4; i++) v[i] = lo[i], v[4 + i] = hi[i];
         } else {
-            const uint4 h = *(const uint4 *)((const uint16_t *)x + at);
-            const uint32_t w[4] = {h.x, h.y, h.z, h.w};
+            const u32x4 w = *(const u32x4_a2 *)((const uint16_t *)x + at);
 #pragma unroll
             for (int i = 0; i < 4; i++) {
                 if (xt == kTypeBF16) {

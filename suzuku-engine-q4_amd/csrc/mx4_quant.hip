@@ -31,9 +31,8 @@ struct Place {
 };
 
 // N values a lane, 32 / N lanes a block: 32 bytes of input, eight fp32 or
-// sixteen 16-bit values.  VEC: rows are 16-byte aligned, so they come in
-// 16-byte loads.
-template <bool VEC, uint32_t N>
+// sixteen 16-bit values.
+template <uint32_t N>
 __global__ __launch_bounds__(256) void mx4_quant_k(const void *__restrict__ x, uint32_t xt,
                                                    uint64_t ld, const int32_t *__restrict__ ids,
                                                    uint64_t rows, uint64_t group, uint32_t cols,
@@ -47,7 +46,7 @@ __global__ __launch_bounds__(256) void mx4_quant_k(const void *__restrict__ x, u
     float v[N];
 #pragma unroll
     for (uint32_t i = 0; i < N; i += 8)
-        load_row8(x, xt, src * ld, p.b * 32 + sub * N + i, cols, VEC, v + i);
+        load_row8(x, xt, src * ld, p.b * 32 + sub * N + i, cols, v + i);
     const uint32_t s = mx4_block_scale<N>(v);
     uint32_t *c = (uint32_t *)(codes + p.r * (16ull * nb) + p.b * 16u + sub * (N / 2));
     if constexpr (N == 16)
@@ -62,14 +61,11 @@ __global__ __launch_bounds__(256) void mx4_quant_k(const void *__restrict__ x, u
     }
 }
 
-typedef float f32x4 __attribute__((ext_vector_type(4)));
-typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
-
 // The mirror, G values a lane (32 / G lanes a block), so that a lane's values
 // are 16 bytes of output and a wave's one stretch: eight for 16-bit outputs,
 // four for fp32.  Past the caches, which the values would only pass through
 // (8192 x 8192 to bf16: 47 us through them, 33 past them).
-template <bool VEC, uint32_t G>
+template <uint32_t G>
 __global__ __launch_bounds__(256) void mx4_dequant_k(const uint8_t *__restrict__ codes,
                                                      const uint8_t *__restrict__ scales,
                                                      const int32_t *__restrict__ ids,
@@ -95,16 +91,16 @@ __global__ __launch_bounds__(256) void mx4_dequant_k(const uint8_t *__restrict__
             const mx4_f2 p2 = mx4_unpack2<2>(q), p3 = mx4_unpack2<3>(q);
             v[4] = p2.x * f, v[5] = p2.y * f, v[6] = p3.x * f, v[7] = p3.y * f;
         }
-        if (VEC && c0 + G <= cols) {
+        if (c0 + G <= cols) {
             if constexpr (G == 4) {
                 __builtin_nontemporal_store((f32x4){v[0], v[1], v[2], v[3]},
-                                            (f32x4 *)((float *)y + at));
+                                            (f32x4_a4 *)((float *)y + at));
             } else {
                 u32x4 w;
 #pragma unroll
                 for (int i = 0; i < 4; i++)
                     w[i] = f32_to_16(v[2 * i], yt) | (uint32_t)f32_to_16(v[2 * i + 1], yt) << 16;
-                __builtin_nontemporal_store(w, (u32x4 *)((uint16_t *)y + at));
+                __builtin_nontemporal_store(w, (u32x4_a2 *)((uint16_t *)y + at));
             }
         } else {
 #pragma unroll
@@ -146,11 +142,6 @@ bool rows_ok(const char *who, const void *f, uint32_t type, uint64_t ld, uint64_
     return true;
 }
 
-// Whether a lane's eight values can move 16 bytes at a time.
-bool wide(const void *f, uint32_t type, uint64_t ld) {
-    return !((uintptr_t)f & 15) && ld * type_bytes(type) % 16 == 0;
-}
-
 // `each` blocks a workgroup over groups of whole rows (see Place).
 dim3 block_grid(uint32_t each, uint64_t rows, uint64_t cols, uint64_t *group) {
     const uint32_t nb = mx4_blocks(cols);
@@ -179,8 +170,7 @@ bool q4mi_mx4_quant(const void *d_x, uint32_t x_type, uint64_t ld_x, const int32
     uint64_t group;
     const bool f32 = x_type == kTypeF32;
     const dim3 grid = block_grid(f32 ? 64 : 128, rows, cols, &group);
-    auto k = f32 ? (wide(d_x, x_type, ld_x) ? mx4_quant_k<true, 8> : mx4_quant_k<false, 8>)
-                 : (wide(d_x, x_type, ld_x) ? mx4_quant_k<true, 16> : mx4_quant_k<false, 16>);
+    auto k = f32 ? mx4_quant_k<8> : mx4_quant_k<16>;
     k<<<grid, dim3(256), 0, stream()>>>(d_x, x_type, ld_x, d_ids, rows, group, (uint32_t)cols,
                                         d_codes, d_scales);
     return launch_ok("mx4_quant_k");
@@ -194,9 +184,7 @@ bool q4mi_mx4_dequant(const uint8_t *d_codes, const uint8_t *d_scales, const int
     if (!rows) return true;
     uint64_t group;
     const dim3 grid = block_grid(64, rows, cols, &group);
-    auto k = y_type == kTypeF32
-                 ? (wide(d_y, y_type, ld_y) ? mx4_dequant_k<true, 4> : mx4_dequant_k<false, 4>)
-                 : (wide(d_y, y_type, ld_y) ? mx4_dequant_k<true, 8> : mx4_dequant_k<false, 8>);
+    auto k = y_type == kTypeF32 ? mx4_dequant_k<4> : mx4_dequant_k<8>;
     k<<<grid, dim3(256), 0, stream()>>>(d_codes, d_scales, d_ids, rows, group, (uint32_t)cols, d_y,
                                         y_type, ld_y);
     return launch_ok("mx4_dequant_k");
