@@ -87,7 +87,7 @@ struct FewRange {
     const uint32_t *list;
     __device__ uint64_t row(uint32_t t) const { return p0 + (list ? list[t] : t); }
     __device__ int64_t x_row(uint32_t t, uint64_t xrows) const {
-        if (!act) return (int64_t)(row(t) / x_div);
+        if (!act) return x_div == 1 ? (int64_t)row(t) : (int64_t)((uint32_t)row(t) / x_div);
         const int64_t r = act[row(t)];
         return r < (int64_t)xrows ? r : -1;
     }
