@@ -392,7 +392,8 @@ bool q4mi_expert_reduce_x(float *d_y, const float *d_pd, const int32_t *d_rsrc,
  * Codes are 16-byte and scales 4-byte aligned.  Float rows are F32 (type 0),
  * F16 (1) or BF16 (30), aligned to their type, `ld` elements apart.  Launches
  * keep no state and no scratch, so calls on different streams (through
- * q4mi_set_stream) and captured graphs are independent of each other.  The
+ * q4mi_set_stream) and captured graphs are independent of each other.  A call
+ * without rows succeeds; its pointers to rows and lists of rows may be NULL.  The
  * reference has no such format. */
 uint64_t q4mi_mx4_code_bytes(uint64_t rows, uint64_t cols);
 uint64_t q4mi_mx4_scale_bytes(uint64_t rows, uint64_t cols);
@@ -455,7 +456,8 @@ bool q4mi_mx4_mul_id(const uint8_t *d_w, const uint8_t *d_ws, uint64_t w_rows, u
  * pen and hist_off, NULL bias_off, NULL mask (a list without entries may be
  * NULL with its offsets given).  Ids outside 0..n_vocab-1 are skipped.  fp32
  * throughout, rounded once.  A row that a mask leaves without tokens is all
- * -inf.  Keeps no state and no scratch.  The reference samples on the host
+ * -inf.  At most 2^23 workgroups of 2048 to 8192 tokens of a row.  n_rows 0
+ * succeeds, with any lists.  Keeps no state and no scratch.  The reference samples on the host
  * (src/q4_tok.c:1901). */
 bool q4mi_logits_process(const void *d_logits, uint32_t type, uint64_t ld, uint32_t n_rows,
                          uint32_t n_vocab, const int32_t *d_hist, const int64_t *d_hist_off,

@@ -237,7 +237,7 @@ bool q4mi_logits_process(const void *d_logits, uint32_t type, uint64_t ld, uint3
                          uint64_t mask_ld, uint32_t n_mask, const int32_t *d_mask_row,
                          void *d_out, uint64_t ld_out) {
     const char *who = "q4mi_logits_process";
-    if (!d_logits || !d_out || !n_vocab || n_vocab > (1u << 30)) {
+    if ((n_rows && (!d_logits || !d_out)) || !n_vocab || n_vocab > (1u << 30)) {
         set_error("%s: bad arguments", who);
         return false;
     }
@@ -245,7 +245,7 @@ bool q4mi_logits_process(const void *d_logits, uint32_t type, uint64_t ld, uint3
         set_error("%s: type %u not covered (F32, F16, BF16)", who, type);
         return false;
     }
-    if (ld < n_vocab || ld_out < n_vocab || (d_out == d_logits && ld != ld_out)) {
+    if (ld < n_vocab || ld_out < n_vocab || (n_rows && d_out == d_logits && ld != ld_out)) {
         set_error("%s: row strides must cover the vocabulary, and agree in place", who);
         return false;
     }
@@ -253,6 +253,7 @@ bool q4mi_logits_process(const void *d_logits, uint32_t type, uint64_t ld, uint3
         set_error("%s: logits must be aligned to their type", who);
         return false;
     }
+    if (!n_rows) return true;
     if (!d_pen != !d_hist_off || ((d_hist || d_gen) && !d_pen)) {
         set_error("%s: penalties need their values and the history's offsets", who);
         return false;
@@ -277,11 +278,10 @@ bool q4mi_logits_process(const void *d_logits, uint32_t type, uint64_t ld, uint3
     const uint32_t ng = least <= fill ? 1 : least <= 2 * fill ? 2 : 4;
     const uint32_t slice = ng * kThreads * 4;
     a.slices = (n_vocab + slice - 1) / slice;
-    if ((uint64_t)a.slices * n_rows > 0x7fffffffu) {
+    if ((uint64_t)a.slices * n_rows > UINT32_MAX / kThreads) {     // threads of a launch
         set_error("%s: %u rows of %u logits too large", who, n_rows, n_vocab);
         return false;
     }
-    if (!n_rows) return true;
     const size_t lds = d_hist || d_bias ? (size_t)slice * 4 : 0;
     auto k = ng == 1 ? logits_k<1> : ng == 2 ? logits_k<2> : logits_k<4>;
     k<<<dim3(a.slices * n_rows), dim3(kThreads), lds, stream()>>>(a);

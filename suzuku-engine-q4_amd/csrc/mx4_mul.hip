@@ -827,8 +827,9 @@ __global__ __launch_bounds__(64 * kIdWaves, 2) void mx4_id_k(MulArgs a) {
     }
 }
 
-bool mul_ok(const char *who, const MulArgs &a) {
-    if (!a.w || !a.ws || !a.x || !a.y || !a.w_rows || !a.cols) {
+// rows: whether the call has any; without, their pointers may be NULL.
+bool mul_ok(const char *who, const MulArgs &a, bool rows) {
+    if (!a.w || !a.ws || (rows && (!a.x || !a.y)) || !a.w_rows || !a.cols) {
         set_error("%s: bad arguments", who);
         return false;
     }
@@ -841,7 +842,7 @@ bool mul_ok(const char *who, const MulArgs &a) {
                   a.x_type, a.y_type);
         return false;
     }
-    if (a.x_type == kTypeMx4 ? !a.xs || ((uintptr_t)a.x & 15) || ((uintptr_t)a.xs & 3)
+    if (a.x_type == kTypeMx4 ? (rows && !a.xs) || ((uintptr_t)a.x & 15) || ((uintptr_t)a.xs & 3)
                              : a.xs || a.ldx < a.cols ||
                                    ((uintptr_t)a.x & (type_bytes(a.x_type) - 1))) {
         set_error("%s: 4-bit inputs need scales, codes aligned to 16 bytes and scales to 4; float "
@@ -1015,7 +1016,7 @@ bool q4mi_mx4_mul(const uint8_t *d_w, const uint8_t *d_ws, uint64_t w_rows, uint
     a.w = d_w, a.ws = d_ws, a.w_rows = w_rows, a.cols = cols;
     a.x = d_x, a.xs = d_xs, a.x_type = x_type, a.ldx = ld_x, a.n = a.xrows = n;
     a.y = d_y, a.y_type = y_type, a.ldy = ld_y;
-    if (!mul_ok("q4mi_mx4_mul", a)) return false;
+    if (!mul_ok("q4mi_mx4_mul", a, n > 0)) return false;
     if (x_type != kTypeMx4 && n > kFloatRows) {
         set_error("q4mi_mx4_mul: %llu float rows not covered (<= %llu; quantise them first)",
                   (unsigned long long)n, (unsigned long long)kFloatRows);
@@ -1035,8 +1036,8 @@ bool q4mi_mx4_mul_sel(const uint8_t *d_w, const uint8_t *d_ws, uint64_t w_rows, 
     a.w_stride = w_stride, a.ws_stride = ws_stride, a.n_expert = n_expert;
     a.x = d_x, a.xs = d_xs, a.x_type = x_type, a.ldx = ld_x, a.x_div = x_div, a.eid = d_eid;
     a.n = n, a.y = d_y, a.y_type = y_type, a.ldy = ld_y;
-    if (!mul_ok("q4mi_mx4_mul_sel", a)) return false;
-    if (!d_eid || !n_expert || !x_div || n > 65535) {
+    if (!mul_ok("q4mi_mx4_mul_sel", a, n > 0)) return false;
+    if ((n && !d_eid) || !n_expert || !x_div || n > 65535) {
         set_error("q4mi_mx4_mul_sel: needs a list, experts, x_div >= 1 and at most 65535 rows");
         return false;
     }
@@ -1062,7 +1063,7 @@ bool q4mi_mx4_mul_id(const uint8_t *d_w, const uint8_t *d_ws, uint64_t w_rows, u
     a.w_stride = w_stride, a.ws_stride = ws_stride, a.n_expert = n_expert;
     a.x = d_xq, a.xs = d_xs, a.x_type = kTypeMx4, a.xrows = xrows, a.act = d_act_row;
     a.bounds = d_bounds, a.n = total_rows, a.y = d_y, a.y_type = y_type, a.ldy = ld_y;
-    if (!mul_ok("q4mi_mx4_mul_id", a)) return false;
+    if (!mul_ok("q4mi_mx4_mul_id", a, total_rows && xrows)) return false;
     if (!d_bounds || !n_expert || n_expert > kIdExperts) {
         set_error("q4mi_mx4_mul_id: needs bounds of 1 to %u experts", kIdExperts);
         return false;

@@ -14,7 +14,7 @@ using namespace q4mi;
 // Place of a thread's block: `off` blocks past the first of the `each` (64 or
 // 128) that the workgroup takes in the row-major order of all rows' blocks,
 // off < each.  Workgroups
-// with one blockIdx.y share a group of whole rows with fewer than 2^31 blocks,
+// with one blockIdx.y share a group of whole rows with fewer than 2^29 blocks,
 // so that the divisions stay in 32 bits.
 struct Place {
     uint64_t r;
@@ -115,7 +115,7 @@ namespace {
 // What both directions ask of their arguments.
 bool rows_ok(const char *who, const void *f, uint32_t type, uint64_t ld, uint64_t rows,
              uint64_t cols, const uint8_t *codes, const uint8_t *scales) {
-    if (!f || !codes || !scales || !cols) {
+    if ((rows && (!f || !codes || !scales)) || !cols) {
         set_error("%s: bad arguments", who);
         return false;
     }
@@ -142,10 +142,11 @@ bool rows_ok(const char *who, const void *f, uint32_t type, uint64_t ld, uint64_
     return true;
 }
 
-// `each` blocks a workgroup over groups of whole rows (see Place).
+// `each` blocks a workgroup over groups of whole rows (see Place), of fewer
+// than 2^29 blocks: a launch has fewer than 2^32 threads along x.
 dim3 block_grid(uint32_t each, uint64_t rows, uint64_t cols, uint64_t *group) {
     const uint32_t nb = mx4_blocks(cols);
-    *group = std::min<uint64_t>(rows, ((1u << 31) - each) / nb);
+    *group = std::min<uint64_t>(rows, ((1u << 29) - each) / nb);
     return dim3((uint32_t)((*group * nb + each - 1) / each),
                 (uint32_t)((rows + *group - 1) / *group));
 }

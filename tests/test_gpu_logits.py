@@ -162,6 +162,26 @@ def test_defaults_of_gen_and_mask_rows(gpu):
           torch.float32)
 
 
+@pytest.mark.parametrize("v", [1, 7, 100, 538])
+def test_biases_of_few_tokens(gpu, v):
+    """Many biases a token: their fp32 sum in list order, to the bit."""
+    rng = np.random.default_rng(v)
+    b = 3
+    x = rng.standard_normal((b, v)).astype(np.float32)
+    bias = [(rng.integers(-1, v + 1, n), rng.uniform(-5, 5, n).astype(np.float32))
+            for n in (1461, 64, 1000)]
+    bias[1][0][:] = v - 1               # a whole wave's entries of one token
+    want = np.empty_like(x)
+    for i, (ids, val) in enumerate(bias):
+        add = np.zeros(v, np.float32)
+        for t, d in zip(ids, val):
+            if 0 <= t < v:
+                add[t] = add[t] + d
+        want[i] = x[i] + add
+    got = call(gpu, 0, dev(x), v, bias=bias).cpu().numpy()
+    assert np.array_equal(got, want)
+
+
 def test_special_values(gpu):
     """Infinities and NaN in the logits, masked and not; infinite biases; a
     mask row out of range masks everything; the same id listed often."""

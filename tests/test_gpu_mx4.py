@@ -102,6 +102,21 @@ def test_quant_gather_and_repeat(gpu):
     assert np.array_equal(host(c), want[0]) and np.array_equal(host(s), want[1])
 
 
+def test_quant_past_one_group(gpu):
+    """More than 2^29 blocks, 8.6 GB of codes: past one group of rows and past
+    32-bit offsets."""
+    cols, few = 16384, 64
+    rows = (1 << 29) // (cols // 32) + 300
+    g = torch.Generator(device="cuda").manual_seed(3)
+    x = torch.randn((few, cols), device="cuda", generator=g).to(torch.bfloat16)
+    ids = torch.randint(0, few, (rows,), dtype=torch.int32, device="cuda", generator=g)
+    c0, s0 = quant(gpu, x, q4mi.T_BF16, cols, few, cols)
+    c, s = quant(gpu, x, q4mi.T_BF16, cols, rows, cols, ids)
+    for r in range(0, rows, 1 << 16):
+        i = ids[r:r + (1 << 16)].long()
+        assert torch.equal(c[r:r + (1 << 16)], c0[i]) and torch.equal(s[r:r + (1 << 16)], s0[i]), r
+
+
 @pytest.mark.parametrize("yt", sorted(TYPES))
 @pytest.mark.parametrize("rows,cols,pad,shift", [
     (1, 1, 0, 0), (3, 40, 0, 0), (17, 257, 7, 1), (64, 2048, 8, 0), (5, 96, 1, 0)])
@@ -334,6 +349,38 @@ def test_mul_sel_float_rows(gpu, xt):
     assert np.array_equal(y[0], y[1])
 
 
+@pytest.mark.parametrize("n,experts,rows,cols,div", [
+    (600, 3, 40, 96, 1), (40, 1, 50, 352, 1), (257, 2, 33, 32, 4), (300, 1000, 20, 64, 1),
+    (17, 4, 64, 4096, 17), (256, 1, 16, 512, 8)])
+def test_mul_sel_shared_experts(gpu, n, experts, rows, cols, div):
+    """Lists past 256 rows, many rows of one expert, rows of none between
+    them: codes give the 64-bit result, float rows the bits of their codes."""
+    rng = np.random.default_rng(n + experts)
+    w, ws, wv, st, sst = arena(rng, experts, rows, cols)
+    xr = (n + div - 1) // div
+    x, xs = ref.random_rows(rng, xr, cols, 126, 128)
+    xv = ref.values(x, xs, cols)
+    eid = rng.integers(0, experts, n).astype(np.int32)
+    eid[::7] = -1
+    eid[3] = experts
+    want = np.full((n, rows + 1), -7.0)
+    for p in range(n):
+        if 0 <= eid[p] < experts:
+            want[p, :rows] = wv[eid[p]] @ xv[p // div]
+    de = dev(eid)
+    f = dev(rng.standard_normal((xr, cols))).to(torch.bfloat16)
+    c, s = quant(gpu, f, q4mi.T_BF16, cols, xr, cols)
+    y = torch.full((3, n, rows + 1), -7.0, device="cuda")
+    sides = ((dev(x), dev(xs), MX4), (f, None, q4mi.T_BF16), (c, s, MX4))
+    for i, (a, b, t) in enumerate(sides):
+        q4mi.check(gpu.q4mi_mx4_mul_sel(w.data_ptr(), ws.data_ptr(), rows, cols, st, sst, experts,
+                                        a.data_ptr(), q4mi.ptr(b), t, cols, div, de.data_ptr(), n,
+                                        y[i].data_ptr(), 0, rows + 1), "sel")
+    y = host(y)
+    assert np.array_equal(y[0], want)
+    assert np.array_equal(y[1], y[2])
+
+
 @pytest.mark.parametrize("counts,rows,cols,spare", [
     ([0, 5, 0, 17], 64, 96, 3), ([40], 33, 32, 0), ([1] * 20, 100, 640, 0), ([0, 0], 16, 32, 4),
     ([130, 0, 300, 7, 64, 65], 272, 288, 9), ([500, 1], 1024, 512, 0),
@@ -513,6 +560,58 @@ def test_layer_to_logits(gpu):
 
 
 # ---------------------------------------------------------- streams and graphs
+
+def test_two_streams_and_graphs(gpu):
+    """Two captured sequences replayed on two streams at once, over and over:
+    each gives what it gives alone."""
+    rng = np.random.default_rng(9)
+    n, rows, cols, experts = 64, 500, 1056, 5
+    w, ws, _, st, sst = arena(rng, experts, rows, cols)
+    bounds = dev(np.array([0, 3, 40, 40, 41, 64], np.int32))
+    eid = dev(rng.integers(0, experts, n).astype(np.int32))
+    x = [dev(rng.standard_normal((n, cols)).astype(np.float32)) for _ in range(2)]
+    c = torch.empty((2, n, ref.blocks(cols) * 16), dtype=torch.uint8, device="cuda")
+    s = torch.empty((2, n, ref.scale_row(cols)), dtype=torch.uint8, device="cuda")
+    y = torch.zeros((2, 3, n, rows), device="cuda")
+
+    def calls(i):
+        q4mi.use_torch_stream()
+        q4mi.check(gpu.q4mi_mx4_quant(x[i].data_ptr(), 0, cols, None, n, cols, c[i].data_ptr(),
+                                      s[i].data_ptr()), "quant")
+        q4mi.check(gpu.q4mi_mx4_mul(w.data_ptr(), ws.data_ptr(), rows, cols, c[i].data_ptr(),
+                                    s[i].data_ptr(), MX4, 0, n, y[i, 0].data_ptr(), 0, rows), "mul")
+        q4mi.check(gpu.q4mi_mx4_mul_sel(w.data_ptr(), ws.data_ptr(), rows, cols, st, sst, experts,
+                                        x[i].data_ptr(), None, 0, cols, 1, eid.data_ptr(), n,
+                                        y[i, 1].data_ptr(), 0, rows), "sel")
+        q4mi.check(gpu.q4mi_mx4_mul_id(w.data_ptr(), ws.data_ptr(), rows, cols, st, sst, experts,
+                                       c[i].data_ptr(), s[i].data_ptr(), n, None,
+                                       bounds.data_ptr(), n, y[i, 2].data_ptr(), 0, rows), "id")
+
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    graphs = [torch.cuda.CUDAGraph() for _ in range(2)]
+    calls(0), calls(1)
+    torch.cuda.synchronize()
+    want = y.clone()
+    assert not torch.equal(want[0], want[1])
+    try:
+        for i in range(2):
+            with torch.cuda.graph(graphs[i], stream=streams[i]):
+                calls(i)
+        for eager in (False, True, False):
+            y.zero_()
+            torch.cuda.synchronize()
+            for _ in range(4):
+                for i in range(2):
+                    with torch.cuda.stream(streams[i]):
+                        if eager:
+                            calls(i)
+                        else:
+                            graphs[i].replay()
+            torch.cuda.synchronize()
+            assert torch.equal(y, want), eager
+    finally:
+        q4mi.use_torch_stream()
+
 
 def test_mx4_graph_and_stream(gpu):
     """Captured on a stream of its own and replayed with other inputs, eager

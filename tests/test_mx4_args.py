@@ -110,6 +110,23 @@ def test_product_refusals(which):
         refused(call(xt=F32, xs=None, n=9), "float rows")
 
 
+def test_calls_without_rows():
+    """An empty batch's pointers may be NULL, as an empty tensor's are."""
+    L = q4mi.lib()
+    assert L.q4mi_mx4_quant(None, F32, 64, None, 0, 64, None, None), q4mi.last_error()
+    assert L.q4mi_mx4_dequant(None, None, None, 0, 64, None, F32, 64), q4mi.last_error()
+    for x_type in (MX4, F32):
+        assert L.q4mi_mx4_mul(A, A, 64, 64, None, None, x_type, 64, 0, None, F32, 64), \
+            q4mi.last_error()
+        assert L.q4mi_mx4_mul_sel(A, A, 64, 64, 4096, 256, 4, None, None, x_type, 64, 1, None, 0,
+                                  None, F32, 64), q4mi.last_error()
+    for n, xrows in ((0, 0), (0, 4), (4, 0)):
+        assert L.q4mi_mx4_mul_id(A, A, 64, 64, 4096, 256, 4, None, None, xrows, None, A, n, None,
+                                 F32, 64), q4mi.last_error()
+    assert L.q4mi_logits_process(None, F32, 100, 0, 100, None, A, None, None, None, None, A, None,
+                                 0, 0, None, None, 100), q4mi.last_error()
+
+
 def test_logits_refusals():
     L = q4mi.lib()
 
@@ -141,4 +158,5 @@ def test_logits_refusals():
     refused(call(mask=None, mrow=A), "masks")
     refused(call(n=(1 << 32) - 1, v=1 << 20, ld=1 << 20, ldo=1 << 20, mld=1 << 15, mrow=A),
             "too large")
+    refused(call(n=1 << 24, mrow=A), "too large")         # 2^24 workgroups of 512 threads
     assert call(n=0)
