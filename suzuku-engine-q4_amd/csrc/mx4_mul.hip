@@ -41,18 +41,21 @@ __device__ inline v8i widen(u32x4 q) {
 // Four adjacent outputs, rounded once.  STREAM: past the caches.
 template <bool STREAM = false>
 __device__ inline void store4(void *y, uint32_t yt, uint64_t at, v4f v) {
-    auto put = [](auto *p, auto q) __attribute__((always_inline)) {
+    if (yt == kTypeF32) {
+        f32x4_a4 *p = (f32x4_a4 *)((float *)y + at);
+        if constexpr (STREAM)
+            __builtin_nontemporal_store((f32x4)v, p);
+        else
+            *p = v;
+    } else {
+        const u32x2 q = {f32_to_16(v[0], yt) | (uint32_t)f32_to_16(v[1], yt) << 16,
+                         f32_to_16(v[2], yt) | (uint32_t)f32_to_16(v[3], yt) << 16};
+        u32x2_a2 *p = (u32x2_a2 *)((uint16_t *)y + at);
         if constexpr (STREAM)
             __builtin_nontemporal_store(q, p);
         else
             *p = q;
-    };
-    if (yt == kTypeF32)
-        put((f32x4_a4 *)((float *)y + at), (f32x4)v);
-    else
-        put((u32x2_a2 *)((uint16_t *)y + at),
-            (u32x2){f32_to_16(v[0], yt) | (uint32_t)f32_to_16(v[1], yt) << 16,
-                    f32_to_16(v[2], yt) | (uint32_t)f32_to_16(v[3], yt) << 16});
+    }
 }
 
 // ---------------------------------------------------------------- few rows
