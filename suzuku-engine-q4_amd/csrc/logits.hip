@@ -70,8 +70,7 @@ __device__ inline void store_four(const LogitsArgs &a, uint64_t i, uint32_t left
                 (u32x4){f32_bits(z[0]), f32_bits(z[1]), f32_bits(z[2]), f32_bits(z[3])};
         } else {
             *(u32x2_a2 *)((uint16_t *)a.out + i) =
-                (u32x2){f32_to_16(z[0], a.type) | (uint32_t)f32_to_16(z[1], a.type) << 16,
-                        f32_to_16(z[2], a.type) | (uint32_t)f32_to_16(z[3], a.type) << 16};
+                (u32x2){f32_to_16x2(z[0], z[1], a.type), f32_to_16x2(z[2], z[3], a.type)};
         }
     } else {
         for (uint32_t k = 0; k < left; k++) store_from_f32(a.out, a.type, i + k, z[k]);

@@ -48,8 +48,7 @@ __device__ inline void store4(void *y, uint32_t yt, uint64_t at, v4f v) {
         else
             *p = v;
     } else {
-        const u32x2 q = {f32_to_16(v[0], yt) | (uint32_t)f32_to_16(v[1], yt) << 16,
-                         f32_to_16(v[2], yt) | (uint32_t)f32_to_16(v[3], yt) << 16};
+        const u32x2 q = {f32_to_16x2(v[0], v[1], yt), f32_to_16x2(v[2], v[3], yt)};
         u32x2_a2 *p = (u32x2_a2 *)((uint16_t *)y + at);
         if constexpr (STREAM)
             __builtin_nontemporal_store(q, p);

@@ -99,7 +99,7 @@ __global__ __launch_bounds__(256) void mx4_dequant_k(const uint8_t *__restrict__
                 u32x4 w;
 #pragma unroll
                 for (int i = 0; i < 4; i++)
-                    w[i] = f32_to_16(v[2 * i], yt) | (uint32_t)f32_to_16(v[2 * i + 1], yt) << 16;
+                    w[i] = f32_to_16x2(v[2 * i], v[2 * i + 1], yt);
                 __builtin_nontemporal_store(w, (u32x4_a2 *)((uint16_t *)y + at));
             }
         } else {

@@ -182,6 +182,36 @@ def test_biases_of_few_tokens(gpu, v):
     assert np.array_equal(got, want)
 
 
+@pytest.mark.parametrize("v", [4096, 4093])
+@pytest.mark.parametrize("xt", [q4mi.T_F16, q4mi.T_BF16])
+def test_rounding_to_16_bits(gpu, xt, v):
+    """Every kind of fp32 value, given as a bias of logits 0, is stored as its
+    nearest 16-bit value, ties to even: halves between neighbours and the
+    values beside them, subnormals, overflow, infinities, NaN."""
+    rng = np.random.default_rng(v)
+    t = TYPES[xt]
+    step = 1 << (13 if xt == q4mi.T_F16 else 16)        # of the 16-bit type, in fp32 bits
+    top = 0x47800000 if xt == q4mi.T_F16 else 0x7f800000
+    bits = (rng.integers(0, top // step, (v, ), dtype=np.int64) * step + step // 2
+            + rng.integers(-1, 2, v)).astype(np.uint32)
+    small = np.arange(0, 600) * step // 2 + rng.integers(-1, 2, 600)
+    bits[:600] = np.maximum(small, 0).astype(np.uint32)
+    if xt == q4mi.T_F16:                                # halves of its subnormal step, 2^-24
+        half = (np.arange(600) * 2.0 ** -25).astype(np.float32).view(np.uint32).astype(np.int64)
+        bits[600:1200] = np.maximum(half + rng.integers(-1, 2, 600), 0).astype(np.uint32)
+    edge = torch.finfo(t).max
+    last = np.array([edge, np.inf, np.nan], np.float32).view(np.uint32)
+    bits[1200:1209] = [last[0], last[0] + step // 2 - 1, last[0] + step // 2, last[0] + step // 2 + 1,
+                       last[1], last[2], 0x7fffffff, 0, 1]
+    val = (bits ^ (rng.integers(0, 2, v).astype(np.uint32) << np.uint32(31))).view(np.float32)
+    x = torch.zeros((1, v), dtype=t, device="cuda")
+    got = call(gpu, xt, x, v, bias=[(np.arange(v), val)]).cpu()
+    want = torch.from_numpy(val).reshape(1, v).to(t)
+    nan = torch.isnan(want)
+    assert torch.equal(torch.isnan(got), nan) and int(nan.sum()) >= 2
+    assert torch.equal(got[~nan], want[~nan])
+
+
 def test_special_values(gpu):
     """Infinities and NaN in the logits, masked and not; infinite biases; a
     mask row out of range masks everything; the same id listed often."""
