@@ -617,8 +617,9 @@ __device__ inline void tile(const MulArgs &a, const uint8_t *w, const uint8_t *w
     // so that a wave stores whole stretches of an output row: lane (row lr, h)
     // holds weight rows 8q + 4h + 0..3 of its fragments.
     constexpr uint32_t kRow = FN * 32 + 4, kLanes = FN * 8;   // floats a row, lanes that store one
-    // The largest tile is for outputs that the caches do not hold (16384 x 2048
-    // over 8192 rows, bf16 out: 215 us through them, 210 past them).
+    // The largest tile is for outputs that the caches may not hold (bf16 out,
+    // through them against past them: 16384 rows x 16384 x 1024, 512 MiB, 262
+    // against 222 us; 8192 rows x 16384 x 2048, 256 MiB, 191 against 194).
     constexpr bool kStream = BM * BN >= 65536;
     static_assert(NW * 32 * kRow * 4 <= tile_lds<BM, BN>(), "sums fit the stages");
     float *sums = (float *)lds + wave * 32 * kRow;
@@ -692,17 +693,19 @@ __global__ __launch_bounds__(64 * WM * WN, WAVES) void mx4_dense_k(MulArgs a) {
 // the matrix units), and the other experts' 16-row weight tiles, each streamed
 // once past all of its expert's rows (bound by memory).  Of the second list a
 // workgroup takes one stretch, so that it stages few experts' rows, shorter by
-// kIdCost tiles for each large tile that it has (22 of them take as long as
-// one; 512 experts' 1024 x 2048 over 2048 tokens: 188 us at 11, 180 at 22).
+// kIdCost tiles for each large tile that it has (18 of them take as long as
+// one; 512 experts' 1024 x 2048 over 4096 tokens, 256 experts' 1280 x 2560 over
+// 333: 234 and 122 us at 14, 226 and 118 at 18, 226 and 121 at 22, 230 and 120
+// at 26).
 // Every second workgroup begins with the streamed tiles, so that memory and
-// matrix units work at the same time (192 us all alike, 185 so).
+// matrix units work at the same time (188 us all alike, 175 so).
 //
 // Every workgroup makes the lists by itself, as prefix sums over the experts'
 // stretches in LDS (under 5 us with nothing to do): no scratch in memory, no
 // launch before, and no workgroups that find nothing to do, of which a grid
-// over experts, slices and tiles has tens of thousands (347 us).
+// over experts, slices and tiles has tens of thousands (347 us, then 191).
 constexpr uint32_t kIdM = 128, kIdN = 256, kIdWM = 2, kIdWN = 4, kIdWaves = kIdWM * kIdWN;
-constexpr uint32_t kIdFew = 32, kIdExperts = 1024, kIdCost = 22;
+constexpr uint32_t kIdFew = 32, kIdExperts = 1024, kIdCost = 18;
 constexpr size_t kIdLists = 2 * (kIdExperts + 1) * 4;
 
 // Sums over a workgroup's threads, before this one and over all.
@@ -955,14 +958,14 @@ bool few2_launch(MulArgs &a) {
 // its tile while the chip has room for all of them, so the smallest tile wins
 // that still gives at most two workgroups a CU (64 x 64: two and a half);
 // measured in us, bf16 out (rows x cols, activation rows):
-//   few rows    against 64 x 64:   1024 x 2048, 128: 5.7 / 6.8; 4096 x 4096, 32: 7.6 / 10.1;
-//                                  2560 x 2560, 77: 9.3 / 7.7
-//   two groups  against 64 x 64:   8192 x 8192, 32: 17.3 / 20.2; 64: 22.0 / 20.5
-//   64 x 64     against 64 x 128:  4096 x 4096, 512: 13.6 / 14.1; 1024: 22.0 / 19.8
-//   64 x 128    against 128 x 128: 8192 x 8192, 512: 33.4 / 34.2; 1024: 63.6 / 50.5
-//   128 x 128   against 256 x 256: 8192 x 8192, 1024: 50.5 / 63.8; 2048: 96.8 / 83.3
-// Past that the two largest are compared by their full rounds: 50 us for two
-// 128 x 128 a CU, 83 us for one 256 x 256 (8192 columns).
+//   few rows    against 64 x 64:   1024 x 2048, 64: 4.7 / 5.6; 128: 5.5 / 5.7; 192: 6.3 / 5.8;
+//                                  4096 x 4096, 32: 7.4 / 8.9; 64: 9.5 / 8.9
+//   two groups  against 64 x 64:   8192 x 8192, 17: 13.4 / 20.9; 32: 17.3 / 19.1
+//   64 x 64     against 64 x 128:  4096 x 4096, 512: 12.0 / 11.8; 1024: 20.0 / 16.9
+//   64 x 128    against 128 x 128: 8192 x 8192, 512: 29.2 / 29.8; 1024: 59.6 / 43.5
+//   128 x 128   against 256 x 256: 8192 x 8192, 1024: 43.5 / 54.0; 2048: 86.7 / 71.2
+// Past that the two largest are compared by their full rounds: 43 us for two
+// 128 x 128 a CU, 71 us for one 256 x 256 (8192 columns).
 bool mul_pick(MulArgs &a) {
     const uint64_t cus = cu_count();
     auto tiles = [&](uint64_t bm, uint64_t bn) {

@@ -64,7 +64,7 @@ __global__ __launch_bounds__(256) void mx4_quant_k(const void *__restrict__ x, u
 // The mirror, G values a lane (32 / G lanes a block), so that a lane's values
 // are 16 bytes of output and a wave's one stretch: eight for 16-bit outputs,
 // four for fp32.  Past the caches, which the values would only pass through
-// (8192 x 8192 to bf16: 47 us through them, 33 past them).
+// (8192 x 8192 to bf16: 36 us through them, 25 past them; to fp32 63 and 44).
 template <uint32_t G>
 __global__ __launch_bounds__(256) void mx4_dequant_k(const uint8_t *__restrict__ codes,
                                                      const uint8_t *__restrict__ scales,
