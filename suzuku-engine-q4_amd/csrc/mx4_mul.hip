@@ -365,22 +365,22 @@ __device__ inline uint32_t tile_swz(uint32_t row) { return (row >> 1) & 7u; }
 __device__ inline void copy16(const void *g, uint32_t lds) {
     asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(g),
                  "s"(lds)
-                 : "memory");
+                 : "memory", "m0");
 }
 __device__ inline void copy16(const void *base, uint32_t off, uint32_t lds) {
     asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off),
                  "s"(base), "s"(lds)
-                 : "memory");
+                 : "memory", "m0");
 }
 __device__ inline void copy4(const void *g, uint32_t lds) {
     asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off" ::"v"(g),
                  "s"(lds)
-                 : "memory");
+                 : "memory", "m0");
 }
 __device__ inline void copy4(const void *base, uint32_t off, uint32_t lds) {
     asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dword %0, %1" ::"v"(off),
                  "s"(base), "s"(lds)
-                 : "memory");
+                 : "memory", "m0");
 }
 // This wave's copies have landed and its LDS reads are done; then the
 // workgroup meets.
