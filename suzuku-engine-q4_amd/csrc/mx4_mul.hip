@@ -361,14 +361,16 @@ __device__ inline uint32_t tile_swz(uint32_t row) { return (row >> 1) & 7u; }
 
 // Lane i's 16 (4) bytes land at LDS address lds + 16 i (4 i); from a pointer,
 // or from a uniform base and a 32-bit offset.  Inline asm, so that the
-// compiler adds no wait before the next LDS read.
+// compiler adds no wait before the next LDS read.  Nor does it see that a base
+// is read: one that a vector instruction wrote (a spilled one read back) needs
+// five wait states, which the move and the s_nop 3 are.
 __device__ inline void copy16(const void *g, uint32_t lds) {
     asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(g),
                  "s"(lds)
                  : "memory", "m0");
 }
 __device__ inline void copy16(const void *base, uint32_t off, uint32_t lds) {
-    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off),
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 3\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off),
                  "s"(base), "s"(lds)
                  : "memory", "m0");
 }
@@ -378,7 +380,7 @@ __device__ inline void copy4(const void *g, uint32_t lds) {
                  : "memory", "m0");
 }
 __device__ inline void copy4(const void *base, uint32_t off, uint32_t lds) {
-    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dword %0, %1" ::"v"(off),
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 3\n\tglobal_load_lds_dword %0, %1" ::"v"(off),
                  "s"(base), "s"(lds)
                  : "memory", "m0");
 }

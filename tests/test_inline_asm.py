@@ -47,3 +47,19 @@ def test_finds_the_copies():
     n = sum("lds" in line for p in SOURCES for code, _ in statements(open(p).read())
             for line in code)
     assert n >= 8
+
+
+@pytest.mark.parametrize("path", SOURCES, ids=os.path.basename)
+def test_a_base_from_a_vector_instruction_can_be_read(path):
+    """A memory instruction may read a scalar register that a vector
+    instruction wrote (readfirstlane, or readlane of a spilled one) only five
+    wait states later; inside asm the compiler does not see the reader and
+    counts none of them."""
+    for code, _ in statements(open(path).read()):
+        states = 0
+        for line in code:
+            if m := re.match(r"(global|buffer|scratch)_\w+\s+(.*)", line):
+                vector_only = re.fullmatch(r"%\d+, off", m.group(2))
+                assert vector_only or states >= 5, code
+            nop = re.match(r"s_nop (\d+)", line)
+            states += int(nop.group(1)) + 1 if nop else 1
