@@ -446,7 +446,8 @@ bool q4mi_mx4_mul_id(const uint8_t *d_w, const uint8_t *d_ws, uint64_t w_rows, u
  *   n_all, n_gen = occurrences of v in hist[hist_off[b] .. hist_off[b+1]) and
  *     in its part from entry gen[b] on (the tokens the model wrote; gen NULL: 0)
  *   z = z > 0 ? z / rep : z * rep                   when n_all > 0
- *   z = z - freq * n_gen - pres * (n_gen > 0)
+ *   z = z - freq * n_gen - pres                   when n_gen > 0 (so that either
+ *     may be infinite: a token that was written is forbidden, the others stay)
  *   z = z + the row's biases of v, summed in list order
  *   z = -inf                                        when the mask's bit v is 0
  * pen[b] = {rep, freq, pres}.  Biases of row b: bias_ids / bias[bias_off[b] ..

@@ -4,7 +4,7 @@
 // that the model wrote:
 //   z = logits[b][v]
 //   z = z > 0 ? z / rep : z * rep            where n_all > 0
-//   z = z - freq * n_gen - pres * (n_gen > 0)
+//   z = z - freq * n_gen - pres               where n_gen > 0
 //   z = z + sum of the row's biases of v, in list order
 //   z = -inf                                  where the mask's bit v is 0
 //
@@ -200,8 +200,7 @@ __global__ __launch_bounds__(kThreads) void logits_k(LogitsArgs a) {
                 if (!c[k]) continue;
                 const float m = (float)(c[k] & ~kPrompt);
                 z[n][k] = z[n][k] > 0.f ? z[n][k] / rep : z[n][k] * rep;
-                z[n][k] = z[n][k] - freq * m;
-                if (m > 0.f) z[n][k] = z[n][k] - pres;
+                if (m > 0.f) z[n][k] = z[n][k] - freq * m - pres;   // both may be infinite
             }
         }
     }

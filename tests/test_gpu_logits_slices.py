@@ -1,6 +1,6 @@
 """q4mi_logits_process where test_gpu_logits does not reach: every slice size
 in every type, in place and out of place, at the most workgroups, past 32-bit
-offsets.  The choice of slice is restated here and
+offsets; penalties without a bound.  The choice of slice is restated here and
 asserted.  Formula and tolerance are test_gpu_logits'."""
 import numpy as np
 import pytest
@@ -81,3 +81,25 @@ def test_rows_past_32_bits(gpu):
     assert torch.equal(x, near)
     del flat, x
     torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("xt", sorted(TYPES))
+def test_penalties_without_a_bound(gpu, xt):
+    """A token that the model has written may be forbidden by an infinite
+    frequency or presence penalty, or forced by a negative one; the others,
+    those of the prompt among them, keep their logits (no infinity times
+    zero)."""
+    v, inf = 3000, np.inf
+    prompt, wrote = np.array([5, 6, 7, 2999, 0]), np.array([6, 8, 8, 2048, 0])
+    hist = np.concatenate([prompt, wrote]).astype(np.int32)
+    pen = np.array([[1, inf, 0], [1, 0, inf], [2, inf, inf], [1, -inf, 0], [1, 0, -inf]],
+                   np.float32)
+    b = len(pen)
+    x = dev(np.random.default_rng(1).standard_normal((b, v)), TYPES[xt])
+    out = call(gpu, xt, x, v, [hist] * b, [len(prompt)] * b, pen)
+    want = x.clone()
+    seen = dev(prompt.astype(np.int64))
+    want[2, seen] = torch.where(x[2, seen] > 0, x[2, seen] / 2, x[2, seen] * 2)
+    for i in range(b):
+        want[i, dev(wrote.astype(np.int64))] = -inf if i < 3 else inf
+    assert torch.equal(out, want)
