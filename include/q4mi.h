@@ -457,9 +457,9 @@ bool q4mi_mx4_mul_id(const uint8_t *d_w, const uint8_t *d_ws, uint64_t w_rows, u
  * pen and hist_off, NULL bias_off, NULL mask (a list without entries may be
  * NULL with its offsets given).  Ids outside 0..n_vocab-1 are skipped.  fp32
  * throughout, rounded once.  A row that a mask leaves without tokens is all
- * -inf.  At most 2^23 workgroups of 2048 to 8192 tokens of a row.  n_rows 0
- * succeeds, with any lists.  Keeps no state and no scratch.  The reference samples on the host
- * (src/q4_tok.c:1901). */
+ * -inf.  Fewer than 2^23 workgroups of 2048 to 8192 tokens of a row.  n_rows 0
+ * succeeds, with any lists.  Keeps no state and no scratch.  The reference
+ * samples on the host (src/q4_tok.c:1901). */
 bool q4mi_logits_process(const void *d_logits, uint32_t type, uint64_t ld, uint32_t n_rows,
                          uint32_t n_vocab, const int32_t *d_hist, const int64_t *d_hist_off,
                          const int32_t *d_gen, const float *d_pen, const int32_t *d_bias_ids,
