@@ -390,7 +390,9 @@ bool q4mi_expert_reduce_x(float *d_y, const float *d_pd, const int32_t *d_rsrc,
  * Scales: one byte s a block for 2^(s - 127), 255 for NaN; a row's scales take
  * nb bytes rounded up to a whole dword.  Rows follow each other without gaps.
  * Codes are 16-byte and scales 4-byte aligned.  Float rows are F32 (type 0),
- * F16 (1) or BF16 (30), aligned to their type, `ld` elements apart.  Launches
+ * F16 (1) or BF16 (30), aligned to their type, `ld` elements apart.  ggml's own
+ * blocks of type 39 hold the same codes and scales in another order (a scale
+ * byte, then values j and j + 16 in byte j): no call here takes them.  Launches
  * keep no state and no scratch, so calls on different streams (through
  * q4mi_set_stream) and captured graphs are independent of each other.  A call
  * without rows succeeds; its pointers to rows and lists of rows may be NULL.  The

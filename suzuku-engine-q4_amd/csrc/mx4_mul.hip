@@ -619,9 +619,13 @@ __device__ inline void tile(const MulArgs &a, const uint8_t *w, const uint8_t *w
     // so that a wave stores whole stretches of an output row: lane (row lr, h)
     // holds weight rows 8q + 4h + 0..3 of its fragments.
     constexpr uint32_t kRow = FN * 32 + 4, kLanes = FN * 8;   // floats a row, lanes that store one
-    // The largest tile is for outputs that the caches may not hold (bf16 out,
-    // through them against past them: 16384 rows x 16384 x 1024, 512 MiB, 262
-    // against 222 us; 8192 rows x 16384 x 2048, 256 MiB, 191 against 194).
+    // The largest tile stores past the caches, whatever its output's size.  That
+    // pays for outputs that the caches cannot hold and costs below (us through
+    // them / past them, bf16 out, alone and with a quantiser that reads it:
+    // 16384 rows x 16384 x 1024, 512 MiB, 259 / 222 and 397 / 383; 8192 x 16384
+    // x 2048, 256 MiB, 169 / 171 and 253 / 234; 8192 x 8192 x 2048, 128 MiB,
+    // 85 / 93 and 113 / 126; 4096 x 8192 x 4096, 64 MiB, 76 / 79 and 91 / 97;
+    // 2048 x 8192 x 8192, 32 MiB, 80 / 80 and 83 / 83).
     constexpr bool kStream = BM * BN >= 65536;
     static_assert(NW * 32 * kRow * 4 <= tile_lds<BM, BN>(), "sums fit the stages");
     float *sums = (float *)lds + wave * 32 * kRow;

@@ -63,8 +63,11 @@ __global__ __launch_bounds__(256) void mx4_quant_k(const void *__restrict__ x, u
 
 // The mirror, G values a lane (32 / G lanes a block), so that a lane's values
 // are 16 bytes of output and a wave's one stretch: eight for 16-bit outputs,
-// four for fp32.  Past the caches, which the values would only pass through
-// (8192 x 8192 to bf16: 36 us through them, 25 past them; to fp32 63 and 44).
+// four for fp32.  Stored past the caches, whatever the size: alone that is the
+// faster way from 2 MiB on (us through / past them, bf16: 16 MiB 5.8 / 4.7, 64
+// MiB 14.5 / 11.4, 128 MiB 26.1 / 24.9, 256 MiB 67 / 47), while a quantiser that
+// reads the values next has 64 and 128 MiB sooner through them (33 / 35 and
+// 55 / 59 together; 16 MiB 15.5 / 15.2, 256 MiB 140 / 124).
 template <uint32_t G>
 __global__ __launch_bounds__(256) void mx4_dequant_k(const uint8_t *__restrict__ codes,
                                                      const uint8_t *__restrict__ scales,
