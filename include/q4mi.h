@@ -469,6 +469,122 @@ bool q4mi_logits_process(const void *d_logits, uint32_t type, uint64_t ld, uint3
                          uint64_t mask_ld, uint32_t n_mask, const int32_t *d_mask_row,
                          void *d_out, uint64_t ld_out);
 
+/* --------------------------- 8-bit floating point rows in blocks of 128 (type 248)
+ *
+ * A row of `cols` values is nb = ceil(cols/128) blocks and 128*nb bytes of e4m3
+ * codes (sign, four exponent bits of bias 7, three mantissa bits; no infinity,
+ * 0x7f and 0xff are NaN), 0 past cols; rows follow each other without gaps.  A
+ * value is its code times its block's fp32 scale, any fp32.  Activations have a
+ * scale for each block of a row ([rows][nb]), weights one for each 128 x 128
+ * values ([ceil(rows/128)][nb]).  Codes are 16-byte and scales 4-byte aligned.
+ * Float rows are F32 (type 0), F16 (1) or BF16 (30), aligned to their type, `ld`
+ * elements apart.  248 is this library's own number; ggml has no such type.
+ * Launches keep no state and no scratch, so calls on different streams (through
+ * q4mi_set_stream) and captured graphs are independent of each other.  A call
+ * without rows succeeds; its pointers to rows and lists of rows may be NULL.  The
+ * reference has no such format. */
+uint64_t q4mi_f8_code_bytes(uint64_t rows, uint64_t cols);
+/* block_rows: 1 (activations) or 128 (weights). */
+uint64_t q4mi_f8_scale_bytes(uint64_t rows, uint64_t cols, uint32_t block_rows);
+/* rows (row r = x[ids ? ids[r] : r]) to codes and scales, block_rows (1, 128)
+ * rows to a scale: the least power of two, at least 2^-120, that takes the
+ * block's largest magnitude to at most 448; codes to nearest, ties to the even
+ * code.  A block that holds an infinity or a NaN becomes all NaN (its scale).
+ * ids are not checked. */
+bool q4mi_f8_quant(const void *d_x, uint32_t x_type, uint64_t ld_x, const int32_t *d_ids,
+                   uint64_t rows, uint64_t cols, uint32_t block_rows, uint8_t *d_codes,
+                   float *d_scales);
+/* Row r = code times scale in fp32 of row ids ? ids[r] : r, rounded to y_type;
+ * columns past cols of y are left as they were. */
+bool q4mi_f8_dequant(const uint8_t *d_codes, const float *d_scales, const int32_t *d_ids,
+                     uint64_t rows, uint64_t cols, uint32_t block_rows, void *d_y,
+                     uint32_t y_type, uint64_t ld_y);
+/* y[t][r] = W_r . x_t for t < n, r < w_rows, both sides in 8 bits: sums of a
+ * block, both scales and the sum over blocks in fp32, rounded once to y_type.
+ * x_type 248: x and xs are codes and scales (ld_x unused).  x_type 0 / 1 / 30:
+ * float rows, at most 16, quantised as by q4mi_f8_quant on the way in (the same
+ * bits in y), xs NULL.  Blocks are taken whole: codes past cols must be 0 in W
+ * or in x and not NaN in either, as the quantiser leaves them. */
+bool q4mi_f8_mul(const uint8_t *d_w, const float *d_ws, uint64_t w_rows, uint64_t cols,
+                 const void *d_x, const float *d_xs, uint32_t x_type, uint64_t ld_x, uint64_t n,
+                 void *d_y, uint32_t y_type, uint64_t ld_y);
+/* Routed experts of a decode step: row p < n (n <= 65535) is expert eid[p]
+ * (codes at w + e*w_stride, scales at ws + e*ws_stride, both in bytes) times x
+ * row p / x_div (x_div = topk: the token's hidden state; 1: a row each).  x as
+ * for q4mi_f8_mul, any number of float rows.  A row whose eid is outside
+ * 0..n_expert-1 is left as it was.  eid is what q4mi_route_scored and
+ * q4mi_moe_route write (ostride topk). */
+bool q4mi_f8_mul_sel(const uint8_t *d_w, const float *d_ws, uint64_t w_rows, uint64_t cols,
+                     uint64_t w_stride, uint64_t ws_stride, uint32_t n_expert, const void *d_x,
+                     const float *d_xs, uint32_t x_type, uint64_t ld_x, uint32_t x_div,
+                     const int32_t *d_eid, uint64_t n, void *d_y, uint32_t y_type,
+                     uint64_t ld_y);
+/* Routed experts of a prompt: packed rows bounds[e] .. bounds[e+1] go through
+ * expert e, packed row p reading x row act_row ? act_row[p] : p (of xrows);
+ * bounds (ascending) and act_row as q4mi_assign writes them; n_expert <= 1024.
+ * Rows outside every stretch, past total_rows or with act_row outside
+ * 0..xrows-1 are left as they were. */
+bool q4mi_f8_mul_id(const uint8_t *d_w, const float *d_ws, uint64_t w_rows, uint64_t cols,
+                    uint64_t w_stride, uint64_t ws_stride, uint32_t n_expert, const uint8_t *d_xq,
+                    const float *d_xs, uint64_t xrows, const int32_t *d_act_row,
+                    const int32_t *d_bounds, uint64_t total_rows, void *d_y, uint32_t y_type,
+                    uint64_t ld_y);
+
+/* ------------------------------------------------- norm and scored routing */
+
+/* Root-mean-square norm of rows with the residual's addition:
+ *   h = x + res, rounded to r_type        (res and sum NULL: h = x)
+ *   y = (h * fp32(1 / sqrt(sum h^2 / cols + eps))) * w, the sum in 64 bits
+ * h goes to d_sum (optional; it may be d_res, or d_x of the same type and
+ * stride), y to d_y rounded to y_type (optional; it may be d_x of the same type
+ * and stride) and / or in 8 bits to d_codes and d_scales, from y in fp32: q_type
+ * 248, the blocks of 128 of q4mi_f8_quant; q_type 8, the groups of 32 of
+ * q4mi_quant8 (int8 codes [rows][cols], fp32 scales [rows][cols/32], cols % 32
+ * == 0), what q4mi_mmvq reads.  No codes: both NULL.  Types F32 (0), F16 (1) or
+ * BF16 (30), rows aligned to their type and ld elements apart (res and sum
+ * both ld_r), d_w [cols] of w_type or NULL (1), codes 16-byte and scales 4-byte
+ * aligned.  cols <= 2^24, fewer than 2^30 rows.  Columns past cols stay as they
+ * were; rows 0 succeeds.  Keeps no state and no scratch.  The reference
+ * norms on its own side (src/q4_quant.c); this stands ahead of q4mi_moe_route /
+ * q4mi_moe_route_scored (y) and the 8-bit products (codes). */
+bool q4mi_rms_norm(const void *d_x, uint32_t x_type, uint64_t ld_x, const void *d_res, void *d_sum,
+                   uint32_t r_type, uint64_t ld_r, const void *d_w, uint32_t w_type, float eps,
+                   uint64_t rows, uint64_t cols, void *d_y, uint32_t y_type, uint64_t ld_y,
+                   uint32_t q_type, void *d_codes, float *d_scales);
+/* Routing by scores, of logits [n_tok][n_exp] (F32, F16 or BF16, `ld` apart):
+ *   s_e = softmax over the token's experts (sigmoid 0) or 1 / (1 + exp(-z_e)) (1)
+ *   c_e = s_e + bias[e]                            (bias NULL: s_e)
+ * Of n_group equal groups of adjacent experts (1 to 64) the topk_group stay
+ * whose group_top (1 or 2) best c have the largest sum; of the experts that
+ * stay, the topk with the largest c are picked, in that order, ties to the
+ * lowest index (without a bias by the logit: the same order, and of scores that
+ * round alike too).  Weight of a pick: s (without the bias), with renorm divided by
+ * the picks' sum (all 0 where that is 0), times scale.  An expert whose logit
+ * or c is -inf or NaN is never picked (a group without others never stays; a
+ * logit of +inf counts as the largest finite one); places that find no expert
+ * have id -1 and weight 0, which q4mi_assign and the _sel products skip.
+ * Scores, sums and comparisons in 64 bits, weights rounded once.  Rows of
+ * ostride entries: topk, and with shared_slot >= 0 one more; the shared expert
+ * stands after the picks that were found (weight d_sg[t], 1 without), d_nh
+ * (optional) receives how many entries that makes, so that the device lists of
+ * q4_hip_moe_exec_win / _dev end there.  n_exp <= 1024, topk <= 64, n_tok <=
+ * 2^24.  Keeps no state and no scratch; n_tok 0 succeeds.  The reference routes by softmax alone
+ * (src/q4_quant.c:715-755: q4_hip_route_pf). */
+bool q4mi_route_scored(const void *d_logits, uint32_t type, uint64_t ld, uint32_t n_tok,
+                       uint32_t n_exp, const float *d_bias, uint32_t sigmoid, uint32_t n_group,
+                       uint32_t topk_group, uint32_t group_top, uint32_t topk, bool renorm,
+                       float scale, int32_t *d_ids, float *d_wts, int32_t *d_nh,
+                       uint32_t ostride, int32_t shared_slot, const float *d_sg);
+/* q4mi_moe_route with q4mi_route_scored's choice: the router GEMV (d_logits, and
+ * d_sg with a gate vector) and then the scored routing of its logits.  Arguments
+ * and limits as both (n_exp <= 512, n_tok >= 1). */
+bool q4mi_moe_route_scored(const void *d_wr, uint32_t wr_type, const float *d_sgw,
+                           const float *d_x, uint32_t n_tok, uint32_t n_embd, uint32_t n_exp,
+                           const float *d_bias, uint32_t sigmoid, uint32_t n_group,
+                           uint32_t topk_group, uint32_t group_top, uint32_t topk, bool renorm,
+                           float scale, float *d_logits, int32_t *d_ids, float *d_wts,
+                           int32_t *d_nh, uint32_t ostride, int32_t shared_slot, float *d_sg);
+
 #ifdef __cplusplus
 }
 #endif

@@ -28,6 +28,7 @@ T_Q8_0 = 8
 T_IQ3_S = 21
 T_BF16 = 30
 T_MXFP4 = 39
+T_F8 = 248      # e4m3 in blocks of 128, this library's own number
 
 _c = ctypes
 _vp = _c.c_void_p
@@ -127,6 +128,22 @@ _SIGS = {
                               _vp, _u64, _vp, _u32, _u64]),
     "q4mi_mx4_mul_id": (_b, [_vp, _vp, _u64, _u64, _u64, _u64, _u32, _vp, _vp, _u64, _vp, _vp,
                              _u64, _vp, _u32, _u64]),
+    "q4mi_f8_code_bytes": (_u64, [_u64, _u64]),
+    "q4mi_f8_scale_bytes": (_u64, [_u64, _u64, _u32]),
+    "q4mi_f8_quant": (_b, [_vp, _u32, _u64, _vp, _u64, _u64, _u32, _vp, _vp]),
+    "q4mi_f8_dequant": (_b, [_vp, _vp, _vp, _u64, _u64, _u32, _vp, _u32, _u64]),
+    "q4mi_f8_mul": (_b, [_vp, _vp, _u64, _u64, _vp, _vp, _u32, _u64, _u64, _vp, _u32, _u64]),
+    "q4mi_f8_mul_sel": (_b, [_vp, _vp, _u64, _u64, _u64, _u64, _u32, _vp, _vp, _u32, _u64, _u32,
+                             _vp, _u64, _vp, _u32, _u64]),
+    "q4mi_f8_mul_id": (_b, [_vp, _vp, _u64, _u64, _u64, _u64, _u32, _vp, _vp, _u64, _vp, _vp,
+                            _u64, _vp, _u32, _u64]),
+    "q4mi_rms_norm": (_b, [_vp, _u32, _u64, _vp, _vp, _u32, _u64, _vp, _u32, _f32, _u64, _u64,
+                           _vp, _u32, _u64, _u32, _vp, _vp]),
+    "q4mi_route_scored": (_b, [_vp, _u32, _u64, _u32, _u32, _vp, _u32, _u32, _u32, _u32, _u32, _b,
+                               _f32, _vp, _vp, _vp, _u32, _c.c_int32, _vp]),
+    "q4mi_moe_route_scored": (_b, [_vp, _u32, _vp, _vp, _u32, _u32, _u32, _vp, _u32, _u32, _u32,
+                                   _u32, _u32, _b, _f32, _vp, _vp, _vp, _vp, _u32, _c.c_int32,
+                                   _vp]),
     "q4mi_logits_process": (_b, [_vp, _u32, _u64, _u32, _u32, _vp, _vp, _vp, _vp, _vp, _vp, _vp,
                                  _vp, _u64, _u32, _vp, _vp, _u64]),
 }
