@@ -33,6 +33,7 @@ struct F8Args {
     uint64_t w_rows, cols, w_stride, ws_stride, ldx, xrows, n, ldy;
     uint32_t n_expert, x_type, y_type, x_div;
     uint32_t ks, seg, blocks;       // waves a tile, blocks of K in LDS, workgroups
+    uint32_t m_tiles;               // tiles along the activations
 };
 
 // Four adjacent outputs, rounded once.
@@ -43,11 +44,6 @@ __device__ inline void store4(void *y, uint32_t yt, uint64_t at, v4f v) {
         const u32x2 q = {f32_to_16x2(v[0], v[1], yt), f32_to_16x2(v[2], v[3], yt)};
         *(u32x2_a2 *)((uint16_t *)y + at) = q;
     }
-}
-
-__device__ inline v8i join(u32x4 a, u32x4 b) {
-    const v8i r = {(int)a.x, (int)a.y, (int)a.z, (int)a.w, (int)b.x, (int)b.y, (int)b.z, (int)b.w};
-    return r;
 }
 
 // Eight codes as bf16, exact.
@@ -61,16 +57,45 @@ __device__ inline v8b widen(uint32_t lo, uint32_t hi) {
     return r;
 }
 
-// Sixteen rows against sixteen over one block, from zero.  Which of the block's
-// values a lane holds is free as long as both sides agree: lane (row, g) has
-// bytes 16g .. and 64 + 16g .. of its row, so that four lanes read 64 bytes.
-__device__ inline v4f block_sums(v8i w, v8i x) {
+// A lane's part of a block of sixteen rows.  Which of the block's values that is
+// is free as long as both sides agree: lane (row, g) has bytes 16g .. and 64 +
+// 16g .. of its row, so that four lanes read 64 bytes.
+template <bool WIDE>
+struct Frag;
+template <>
+struct Frag<true> {
+    v8b v[4];
+    __device__ Frag() {}
+    __device__ Frag(u32x4 a, u32x4 b)
+        : v{widen(a.x, a.y), widen(a.z, a.w), widen(b.x, b.y), widen(b.z, b.w)} {}
+};
+template <>
+struct Frag<false> {
+    v8i v;
+    __device__ Frag() {}
+    __device__ Frag(u32x4 a, u32x4 b)
+        : v{(int)a.x, (int)a.y, (int)a.z, (int)a.w, (int)b.x, (int)b.y, (int)b.z, (int)b.w} {}
+};
+
+// Sixteen rows against sixteen over one block, from zero.
+__device__ inline v4f block_sums(const Frag<true> &w, const Frag<true> &x) {
     v4f d = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int i = 0; i < 8; i += 2)
-        d = __builtin_amdgcn_mfma_f32_16x16x32_bf16(widen(w[i], w[i + 1]), widen(x[i], x[i + 1]),
-                                                    d, 0, 0, 0);
+    for (int i = 0; i < 4; i++)
+        d = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w.v[i], x.v[i], d, 0, 0, 0);
     return d;
+}
+__device__ inline v4f block_sums(const Frag<false> &w, const Frag<false> &x) {
+    const v4f zero = {0.f, 0.f, 0.f, 0.f};
+    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w.v, x.v, zero, 0, 0, 0, 0, 0, 0);
+}
+
+// acc += d * s, here: the compiler would rather keep every block's sums in
+// registers and add them after the loop's last product.
+__device__ inline void add_scaled(v4f &acc, v4f d, float s) {
+#pragma unroll
+    for (int i = 0; i < 4; i++) acc[i] = fmaf(d[i], s, acc[i]);
+    asm volatile("" : "+v"(acc));
 }
 
 // ---------------------------------------------------------------- few rows
@@ -188,8 +213,9 @@ __device__ inline void few_rows(const F8Args &a, const uint8_t *w, const float *
         for (uint32_t h = 0; h < 2; h++) {
             if (!FULL && h == 1 && sg * seg + 2 * c + 1 >= nb) break;
             const uint8_t *xp = codes + xc + 256u * c + 128u * h;
-            const v4f d = block_sums(join(q.codes[2 * h], q.codes[2 * h + 1]),
-                                     join(*(const u32x4 *)xp, *(const u32x4 *)(xp + 64)));
+            const v4f d = block_sums(
+                Frag<true>(q.codes[2 * h], q.codes[2 * h + 1]),
+                Frag<true>(*(const u32x4 *)xp, *(const u32x4 *)(xp + 64)));
             const float s = q.s[h] * xs[h];
 #pragma unroll
             for (int k = 0; k < 4; k++) acc[k] = fmaf(d[k], s, acc[k]);
@@ -299,81 +325,351 @@ __global__ __launch_bounds__(64 * kFewWaves) void f8_sel_k(F8Args a) {
     few_rows<FULL>(a, w, ws, f, blockIdx.x, lds + kSelList);
 }
 
-// Activation rows p0 .. p0 + rows (<= 16) of expert weights w against weight
-// rows 16 * tile ..: a wave, both sides straight from memory.
-__device__ inline void plain_tile(const F8Args &a, const uint8_t *w, const float *ws,
-                                  uint64_t tile, uint64_t p0, uint32_t rows) {
-    const uint32_t lane = threadIdx.x & 63u, m = lane & 15u, g = lane >> 4;
+// ------------------------------------------------------------ rows in tiles
+//
+// BM activation rows x BN weight rows a workgroup of WM x WN waves.  K goes in
+// stages of one block: 128 bytes a row, a whole cache line, come by global -> LDS
+// copies into a ring of S stages, spread over the products of S - 1 stages
+// before.  The activations' scales come for eight stages at once, 32 bytes a row;
+// a wave's weight rows share one scale a stage.  A wave holds all its weight
+// fragments of a stage, and the next stage's as it is read, over its activation
+// fragments one by one.
+//
+// LDS places: chunk c (16 bytes) of row r at c ^ ((r >> 1) & 7), dword d of a
+// row's scales at d ^ ((r >> 3) & 7), so that a fragment's reads spread over all
+// 64 banks; the copies fill LDS in lane order, so the lanes permute their source
+// addresses instead.
+
+__device__ inline uint32_t tile_swz(uint32_t row) { return (row >> 1) & 7u; }
+
+// Lane i's 16 (4) bytes land at LDS address lds + 16 i (4 i); from a pointer, or
+// from a uniform base and a 32-bit offset.  Inline asm, so that the compiler adds
+// no wait before the next LDS read.  Nor does it see that
+// a base is read: one that a vector instruction wrote (a spilled one read back)
+// needs five wait states, which the move and the s_nop 3 are.
+__device__ inline void copy16(const void *base, uint32_t off, uint32_t lds) {
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 3\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off),
+                 "s"(base), "s"(lds)
+                 : "memory", "m0");
+}
+__device__ inline void copy16(const void *g, uint32_t lds) {
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(g),
+                 "s"(lds)
+                 : "memory", "m0");
+}
+__device__ inline void copy4(const void *g, uint32_t lds) {
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off" ::"v"(g),
+                 "s"(lds)
+                 : "memory", "m0");
+}
+__device__ inline void copy4(const void *base, uint32_t off, uint32_t lds) {
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 3\n\tglobal_load_lds_dword %0, %1" ::"v"(off),
+                 "s"(base), "s"(lds)
+                 : "memory", "m0");
+}
+// All but this wave's last `LEFT` memory operations have landed; then the
+// workgroup meets.  Later operations of the compiler's make it wait for more.
+template <int LEFT>
+__device__ inline void landed_barrier() {
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(LEFT) : "memory");
+}
+
+// LDS: S stages of codes, two windows (eight stages) of scales.
+template <uint32_t BM, uint32_t BN, uint32_t S>
+constexpr uint32_t tile_lds() { return (BM + BN) * S * 128 + BM * 2 * 32; }
+
+// Weight rows [r0, r0 + BN) of w against activation rows [p0, p0 + BM), of which
+// those below phi exist; the row read for p is act[p] with GATHER, else p.  Rows
+// past either end are read as the last one and not stored.
+template <uint32_t BM, uint32_t BN, uint32_t WM, uint32_t WN, uint32_t S, bool WIDE, bool GATHER>
+__device__ inline void tile(const F8Args &a, const uint8_t *w, const float *ws, uint64_t r0,
+                            uint64_t p0, uint64_t phi, uint8_t *lds) {
+    constexpr uint32_t NW = WM * WN;
+    constexpr uint32_t FM = BM / (16 * WM), FN = BN / (16 * WN);
+    constexpr uint32_t RA = BM / 8 / NW, RB = BN / 8 / NW;   // 8-row copies of each side a wave
+    constexpr uint32_t kLeft = (S - 2) * (RA + RB);     // copies on their way past the next stage's
+    static_assert(FM && FN && RA && RB && 16 * FN <= 128 && kLeft < 64, "tile and waves");
+    static_assert(S - 2 + RA <= 8, "a window's scales land in time");
+    constexpr uint32_t kX = BM * 128, kW = BN * 128, kWin = BM * 32;
+    constexpr uint32_t kWeights = S * kX, kScales = S * (kX + kW);
+    const uint32_t lane = threadIdx.x & 63u, l8 = lane >> 3;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t nb = f8_blocks(a.cols);
-    const uint64_t p = p0 + min(m, rows - 1);
-    int64_t xr = a.act ? (int64_t)a.act[p] : (int64_t)((uint32_t)p / a.x_div);
-    if (xr >= (int64_t)a.xrows) xr = -1;
-    const uint64_t xrow = (uint64_t)max(xr, (int64_t)0);
-    const uint8_t *wp = w + min(tile * 16 + m, a.w_rows - 1) * (128ull * nb) + 16 * g;
-    const float *wsp = ws + tile / 8 * nb;
-    const uint8_t *xp = (const uint8_t *)a.x + xrow * (128ull * nb) + 16 * g;
-    v4f acc = {0.f, 0.f, 0.f, 0.f};
-    for (uint32_t b = 0; b < nb; b++) {
-        const v8i wq = join(*(const u32x4 *)(wp + 128ull * b), *(const u32x4 *)(wp + 128ull * b + 64));
-        v8i xq;
-        float s;
-        if (a.x_type == kTypeF8) {
-            xq = join(*(const u32x4 *)(xp + 128ull * b), *(const u32x4 *)(xp + 128ull * b + 64));
-            s = a.xs[xrow * nb + b];
-        } else {
-            float v[32];
+    const uint32_t base = (uint32_t)(uintptr_t)lds;     // LDS offset: low half of the address
+    const uint32_t row_bytes = 128 * nb;
+
+    // sources of this lane's part of every copy, without the place in K: offsets
+    // from the tile's first row, or numbers of rows with GATHER
+    const uint8_t *xc = (const uint8_t *)a.x;
+    const float *xs = a.xs;
+    if (!GATHER) xc += p0 * row_bytes, xs += p0 * nb;
+    const uint32_t xlast = (uint32_t)min((uint64_t)BM, phi - p0) - 1;
+    const uint32_t wlast = (uint32_t)min((uint64_t)BN, a.w_rows - r0) - 1;
+    w += r0 * row_bytes;
+    auto gathered = [&](uint32_t t) -> uint32_t {
+        const int64_t r = a.act ? (int64_t)a.act[p0 + t] : (int64_t)(p0 + t);
+        return r < 0 || r >= (int64_t)a.xrows ? 0u : (uint32_t)r;
+    };
+    const uint32_t c0 = 16 * ((lane & 7u) ^ (l8 >> 1));     // chunk of an even copy; ^ 64 of an odd
+    uint32_t xo[RA], wo[RB];
 #pragma unroll
-            for (uint32_t i = 0; i < 32; i += 8)
-                load_row8(a.x, a.x_type, xrow * a.ldx, 128 * b + 64 * (i / 16) + 16 * g + i % 16,
-                          (uint32_t)a.cols, v + i);
-            uint32_t top = f8_top<32>(v), q[8];
-            top = max(top, (uint32_t)__shfl_xor((int)top, 16, 64));
-            top = max(top, (uint32_t)__shfl_xor((int)top, 32, 64));
-            const uint32_t bits = f8_scale_of(top);
-            f8_pack<32>(v, bits, q);
-#pragma unroll
-            for (int i = 0; i < 8; i++) xq[i] = (int)q[i];
-            s = bits_f32(bits);
-        }
-        s *= wsp[b];
-        const v4f d = block_sums(wq, xq);
-#pragma unroll
-        for (int i = 0; i < 4; i++) acc[i] = fmaf(d[i], s, acc[i]);
+    for (uint32_t j = 0; j < RA; j++) {
+        const uint32_t c = wave * RA + j, t = min(c * 8 + l8, xlast);
+        xo[j] = GATHER ? gathered(t) : t * row_bytes + (c0 ^ 64 * (c & 1u));
     }
-    if (m >= rows || xr < 0) return;
-    const uint64_t r = tile * 16 + 4 * g, at = p * a.ldy + r;
-    if (r + 4 <= a.w_rows)
-        store4(a.y, a.y_type, at, acc);
-    else
-        for (uint32_t k = 0; k < 4; k++)
-            if (r + k < a.w_rows) store_from_f32(a.y, a.y_type, at + k, acc[k]);
-}
-
-// Dense: grid (weight tiles / 4, sets of 16 activation rows).
-__global__ __launch_bounds__(256) void f8_dense_k(F8Args a) {
-    const uint64_t tile = (uint64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    const uint64_t p0 = (uint64_t)blockIdx.y * 16;
-    if (tile * 16 >= a.w_rows) return;
-    plain_tile(a, a.w, a.ws, tile, p0, (uint32_t)min((uint64_t)16, a.n - p0));
-}
-
-// Packed rows: grid (weight tiles / 4, an upper bound of the experts' sets of 16).
-__global__ __launch_bounds__(256) void f8_id_k(F8Args a) {
-    const uint64_t tile = (uint64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (tile * 16 >= a.w_rows) return;
-    const int64_t end = (int64_t)(a.act ? a.n : min(a.n, a.xrows));
-    uint32_t set = blockIdx.y;
-    for (uint32_t e = 0; e < a.n_expert; e++) {
-        const int64_t lo = max(a.bounds[e], 0), hi = min((int64_t)a.bounds[e + 1], end);
-        const uint32_t sets = hi > lo ? (uint32_t)((hi - lo + 15) / 16) : 0u;
-        if (set < sets) {
-            const int64_t p0 = lo + 16 * (int64_t)set;
-            plain_tile(a, a.w + e * a.w_stride,
-                       (const float *)((const uint8_t *)a.ws + e * a.ws_stride), tile,
-                       (uint64_t)p0, (uint32_t)min((int64_t)16, hi - p0));
-            return;
+#pragma unroll
+    for (uint32_t j = 0; j < RB; j++) {
+        const uint32_t c = wave * RB + j;
+        wo[j] = min(c * 8 + l8, wlast) * row_bytes + (c0 ^ 64 * (c & 1u));
+    }
+    // copy q (of RA + RB) of this wave's of stage k; stages past the last as the last
+    auto fetch = [&](uint32_t k, uint32_t q) __attribute__((always_inline)) {
+        const uint32_t at = 128u * min(k, nb - 1), c = wave * RA + q;
+        const uint32_t to = base + k % S * kX + c * 1024;
+        if (q >= RA)
+            copy16(w + at, wo[q - RA], base + kWeights + k % S * kW + (wave * RB + q - RA) * 1024);
+        else if (GATHER)
+            copy16(xc + at + (c0 ^ 64 * (c & 1u)) + (uint64_t)xo[q] * row_bytes, to);
+        else
+            copy16(xc + at, xo[q], to);
+    };
+    // Copy q (of RA; 8 rows each) of this wave's of window v's scales.
+    auto fetch_scales = [&](uint32_t v, uint32_t q) __attribute__((always_inline)) {
+        const uint32_t c = wave * RA + q, to = base + kScales + (v & 1u) * kWin + c * 256;
+        const uint32_t d = min(8 * v + ((lane & 7u) ^ (c & 7u)), nb - 1);
+        if (GATHER) {
+            uint32_t r = xo[0];
+#pragma unroll
+            for (uint32_t j = 1; j < RA; j++) r = q == j ? xo[j] : r;
+            copy4(xs + (uint64_t)r * nb + d, to);
+        } else {
+            copy4(xs, 4 * (min(c * 8 + l8, xlast) * nb + d), to);
         }
-        set -= sets;
+    };
+    const uint32_t wm = wave / WN, wn = wave % WN, m = lane & 15u, g = lane >> 4;
+    const uint32_t ra = wm * FM * 16 + m, rb = wn * FN * 16 + m;
+    const uint32_t lo = 16 * (g ^ tile_swz(m)), hi = lo ^ 64;
+    // read by scalar loads: one of the compiler's vector loads would wait for every copy
+    typedef const float __attribute__((address_space(4))) *Constant;
+    const Constant wsp = (Constant)(uintptr_t)(ws + (r0 + wn * FN * 16) / 128 * nb);
+
+    v4f acc[FN][FM];
+#pragma unroll
+    for (uint32_t j = 0; j < FN; j++)
+#pragma unroll
+        for (uint32_t i = 0; i < FM; i++) acc[j][i] = (v4f){0.f, 0.f, 0.f, 0.f};
+
+#pragma unroll
+    for (uint32_t q = 0; q < RA; q++) fetch_scales(0, q);
+#pragma unroll
+    for (uint32_t k = 0; k + 1 < S; k++)
+#pragma unroll
+        for (uint32_t q = 0; q < RA + RB; q++) fetch(k, q);
+    landed_barrier<kLeft>();
+    Frag<WIDE> wf[2][FN], xf[2];
+    float sx[2], s = wsp[0];
+    auto read_w = [&](uint32_t k, Frag<WIDE> *f, uint32_t j) __attribute__((always_inline)) {
+        const uint8_t *p = lds + kWeights + k % S * kW + rb * 128 + j * 2048;
+        f[j] = Frag<WIDE>(*(const u32x4 *)(p + lo), *(const u32x4 *)(p + hi));
+    };
+    auto read_x = [&](uint32_t k, uint32_t i) __attribute__((always_inline)) {
+        const uint8_t *p = lds + k % S * kX + ra * 128 + i * 2048;
+        xf[i & 1u] = Frag<WIDE>(*(const u32x4 *)(p + lo), *(const u32x4 *)(p + hi));
+        const uint32_t d = 4 * ((k & 7u) ^ ((ra + 16 * i) >> 3 & 7u));
+        sx[i & 1u] = *(const float *)(lds + kScales + (k >> 3 & 1u) * kWin + ra * 32 + i * 512 + d);
+    };
+#pragma unroll
+    for (uint32_t j = 0; j < FN; j++) read_w(0, wf[0], j);
+    read_x(0, 0);
+    // A stage begins with its weights and its first activations in registers.  The
+    // barrier that says that the next stage has landed and this one is read stands
+    // before the last activations' products, which cover the next stage's first
+    // reads.  Sums are added two products later.
+    auto stage = [&](uint32_t k, Frag<WIDE> *now, Frag<WIDE> *next) __attribute__((always_inline)) {
+        const float s_next = wsp[min(k + 1, nb - 1)];
+        constexpr uint32_t kPairs = FM * FN, kLag = 2;
+        constexpr uint32_t kFirst = FM > 1 ? FM - 1 : 1;
+        constexpr uint32_t kNeed = (RA + RB + kFirst - 1) / kFirst, kEach = kNeed > 3 ? kNeed : 3;
+        v4f d[kLag + 1];
+        float ds[kLag + 1];
+#pragma unroll
+        for (uint32_t t = 0; t < kPairs + kLag; t++) {
+            const uint32_t i = t / FN, j = t % FN;
+            if (t < kPairs) {
+                if (j == 0) {
+                    if (i + 1 < FM) read_x(k, i + 1);
+#pragma unroll
+                    for (uint32_t q = kEach * i; q < min(kEach * (i + 1), RA + RB); q++)
+                        fetch(k + S - 1, q);
+                    if (i + 1 == FM) {
+                        landed_barrier<kLeft>();
+                        // a window's copies spread over the stages of the one before it
+                        if ((k & 7u) < RA) fetch_scales((k >> 3) + 1, k & 7u);
+#pragma unroll
+                        for (uint32_t u = 0; u < FN; u++) read_w(k + 1, next, u);
+                    }
+                }
+                d[t % (kLag + 1)] = block_sums(now[j], xf[i & 1u]);
+                ds[t % (kLag + 1)] = sx[i & 1u];
+                if (t + 1 == kPairs) read_x(k + 1, 0);
+            }
+            if (t >= kLag) {
+                const uint32_t o = t - kLag;
+                add_scaled(acc[o % FN][o / FN], d[o % (kLag + 1)], s * ds[o % (kLag + 1)]);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        s = s_next;
+    };
+    for (uint32_t k = 0; k < nb; k += 2) {
+        stage(k, wf[0], wf[1]);
+        if (k + 1 < nb) stage(k + 1, wf[1], wf[0]);
+    }
+
+    // Sums of 16 activation rows at a time through LDS (the stages are read), so
+    // that a wave stores whole stretches of an output row: lane (m, g) holds
+    // weight rows 4g .. 4g + 3 of its fragments.
+    constexpr uint32_t kRow = FN * 16 + 4, kLanes = FN * 4;   // floats a row, lanes that store one
+    static_assert(NW * 16 * kRow * 4 <= tile_lds<BM, BN, S>(), "sums fit the stages");
+    static_assert(kLanes <= 64, "a row's stores");
+    landed_barrier<0>();
+    float *sums = (float *)lds + wave * 16 * kRow;
+    const uint64_t rw = r0 + wn * FN * 16 + lane % kLanes * 4;   // weight row of this lane's stores
+    auto listed = [&](uint64_t p) {     // whether row p has an activation row
+        return !GATHER || !a.act || (a.act[p] >= 0 && (int64_t)a.act[p] < (int64_t)a.xrows);
+    };
+#pragma unroll
+    for (uint32_t i = 0; i < FM; i++) {
+#pragma unroll
+        for (uint32_t j = 0; j < FN; j++)
+            *(v4f *)(sums + m * kRow + 16 * j + 4 * g) = acc[j][i];
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        const uint64_t p1 = p0 + (wm * FM + i) * 16;
+#pragma unroll
+        for (uint32_t u = 0; u < 16 * kLanes / 64; u++) {
+            const uint32_t t = u * (64 / kLanes) + lane / kLanes;
+            const v4f v = *(const v4f *)(sums + t * kRow + lane % kLanes * 4);
+            const uint64_t at = (p1 + t) * a.ldy + rw;
+            if (p1 + t >= phi || !listed(p1 + t)) continue;
+            if (rw + 4 <= a.w_rows)
+                store4(a.y, a.y_type, at, v);
+            else
+                for (uint32_t n = 0; n < 4; n++)
+                    if (rw + n < a.w_rows) store_from_f32(a.y, a.y_type, at + n, v[n]);
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    }
+}
+
+// Tiles of a dense product, `a.blocks` of them, a.m_tiles along the
+// activations.  Workgroups go to the eight dies in turn, each with an L2 of its
+// own: a die takes a contiguous run of tiles, in groups of kGroup activation
+// tiles, so that its L2 holds what its tiles share.
+constexpr uint32_t kGroup = 4;
+template <uint32_t BM, uint32_t BN, uint32_t WM, uint32_t WN, uint32_t S, bool WIDE>
+__global__ __launch_bounds__(64 * WM * WN, 2) void f8_tile_k(F8Args a) {
+    extern __shared__ __align__(16) uint8_t lds[];
+    const uint32_t die = blockIdx.x & 7u, i = blockIdx.x >> 3;
+    const uint32_t q = a.blocks >> 3, rem = a.blocks & 7u;
+    const uint32_t t = die * q + min(die, rem) + i;
+    const uint32_t n_tiles = a.blocks / a.m_tiles;
+    const uint32_t group = t / (kGroup * n_tiles), in = t - group * kGroup * n_tiles;
+    const uint32_t gm = min(kGroup, a.m_tiles - group * kGroup);
+    const uint32_t mt = group * kGroup + in % gm, nt = in / gm;
+    tile<BM, BN, WM, WN, S, WIDE, false>(a, a.w, a.ws, (uint64_t)nt * BN, (uint64_t)mt * BM, a.n, lds);
+}
+
+// ------------------------------------------------------------- packed rows
+//
+// Persistent workgroups, two a CU, go over the experts' sets of up to 128 rows x
+// 128 weight rows, each in the tile that its rows fill: mostly a few rows, so that
+// reading the weights bounds it, and one workgroup's first copies and last stores
+// are covered by the other's stages.  Every workgroup makes the list of sets by
+// itself, as prefix sums over the experts' stretches in LDS: no scratch in memory,
+// no launch before.
+constexpr uint32_t kIdExperts = 1024, kIdRows = 128, kIdCols = 128, kIdWaves = 4;
+constexpr size_t kIdLists = ((kIdExperts + 1) * 4 + 15) / 16 * 16;
+constexpr uint32_t kIdTiles = tile_lds<128, kIdCols, 2>();     // the largest of them
+static_assert(2 * (kIdLists + kIdTiles) <= 160 * 1024, "two workgroups a CU");
+
+// The last e with list[e] <= i, of n + 1 ascending sums.
+__device__ inline uint32_t owner(const uint32_t *list, uint32_t n, uint32_t i) {
+    uint32_t lo = 0, hi = n;
+    while (hi - lo > 1) {
+        const uint32_t mid = (lo + hi) / 2;
+        if (list[mid] <= i)
+            lo = mid;
+        else
+            hi = mid;
+    }
+    return __builtin_amdgcn_readfirstlane(lo);
+}
+
+template <bool WIDE>
+__global__ __launch_bounds__(64 * kIdWaves, 2) void f8_id_k(F8Args a) {
+    extern __shared__ __align__(16) uint8_t lds[];
+    uint32_t *sets = (uint32_t *)lds;
+    uint8_t *work = lds + kIdLists;
+    // without a row list, packed row p is activation row p: those past xrows do not exist
+    const int64_t end = (int64_t)(a.act ? a.n : min(a.n, a.xrows));
+    const uint32_t n = a.n_expert;
+    auto stretch = [&](uint32_t e, int64_t *lo) __attribute__((always_inline)) -> int64_t {
+        *lo = max(a.bounds[e], 0);
+        return min((int64_t)a.bounds[e + 1], end) - *lo;
+    };
+    // exclusive sums of the experts' sets
+    constexpr uint32_t kEach = kIdExperts / (64 * kIdWaves);
+    uint32_t mine[kEach], sum = 0;
+#pragma unroll
+    for (uint32_t i = 0; i < kEach; i++) {
+        const uint32_t e = threadIdx.x * kEach + i;
+        int64_t lo, rows = e < n ? stretch(e, &lo) : 0;
+        mine[i] = rows > 0 ? (uint32_t)((rows + kIdRows - 1) / kIdRows) : 0u;
+        sum += mine[i];
+    }
+    uint32_t *tmp = (uint32_t *)work, v = sum;
+    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
+#pragma unroll
+    for (uint32_t d = 1; d < 64; d *= 2) {
+        const uint32_t o = __shfl_up(v, d, 64);
+        if (lane >= d) v += o;
+    }
+    if (lane == 63) tmp[wave] = v;
+    __syncthreads();
+    uint32_t total = 0;
+    v -= sum;
+    for (uint32_t i = 0; i < kIdWaves; i++) {
+        if (i < wave) v += tmp[i];
+        total += tmp[i];
+    }
+#pragma unroll
+    for (uint32_t i = 0; i < kEach; i++) {
+        const uint32_t e = threadIdx.x * kEach + i;
+        if (e <= n) sets[e] = v;
+        v += mine[i];
+    }
+    if (threadIdx.x == 0) sets[n] = total;
+    __syncthreads();
+    const uint32_t slices = (uint32_t)((a.w_rows + kIdCols - 1) / kIdCols);
+    const uint64_t items = (uint64_t)__builtin_amdgcn_readfirstlane(total) * slices;
+    for (uint64_t i = blockIdx.x; i < items; i += a.blocks) {
+        const uint32_t unit = (uint32_t)(i / slices), part = (uint32_t)(i - (uint64_t)unit * slices);
+        const uint32_t e = owner(sets, n, unit);
+        const uint32_t first = __builtin_amdgcn_readfirstlane(sets[e]);
+        int64_t lo;
+        const int64_t all = stretch(e, &lo), skip = (int64_t)(unit - first) * kIdRows;
+        const uint32_t rows = (uint32_t)min((int64_t)kIdRows, all - skip);
+        const uint8_t *w = a.w + e * a.w_stride;
+        const float *ws = (const float *)((const uint8_t *)a.ws + e * a.ws_stride);
+        const uint64_t r0 = (uint64_t)part * kIdCols, p0 = (uint64_t)(lo + skip), phi = p0 + rows;
+        if (skip >= all) continue;      // never, with bounds that ascend
+        if (rows <= 32)
+            tile<32, kIdCols, 2, 2, 3, WIDE, true>(a, w, ws, r0, p0, phi, work);
+        else if (rows <= 64)
+            tile<64, kIdCols, 2, 2, 2, WIDE, true>(a, w, ws, r0, p0, phi, work);
+        else
+            tile<128, kIdCols, 2, 2, 2, WIDE, true>(a, w, ws, r0, p0, phi, work);
+        __syncthreads();    // the next item overwrites what slower waves may still read
     }
 }
 
@@ -416,7 +712,6 @@ bool mul_ok(const char *who, const F8Args &a, bool rows) {
 }
 
 constexpr uint64_t kFloatRows = 16;     // float rows that q4mi_f8_mul takes
-constexpr uint32_t kIdExperts = 1024;
 
 // K segment of the few-rows kernels for `rows` activation rows a workgroup:
 // whole rows where they fit in `room` bytes, else equal parts of whole chunks;
@@ -461,7 +756,55 @@ F8Kernel sel_group_kernel(bool full) {
     return full ? f8_sel_k<true, true> : f8_sel_k<false, true>;
 }
 
-uint32_t tiles4(const F8Args &a) { return (uint32_t)((a.w_rows + 63) / 64); }
+// fp32 outputs are summed in fp32 throughout, 16-bit ones on the 8-bit matrix
+// instruction, whose cut-off lies 2^-6 below their rounding.
+bool wide(const F8Args &a) { return a.y_type == kTypeF32; }
+
+template <uint32_t BM, uint32_t BN, uint32_t WM, uint32_t WN, uint32_t S, bool WIDE>
+bool tile_launch(F8Args &a) {
+    static DynLds st;
+    constexpr size_t lds = tile_lds<BM, BN, S>();
+    auto k = f8_tile_k<BM, BN, WM, WN, S, WIDE>;
+    if (!dyn_lds_ok((const void *)k, lds, lds, st, "f8_tile_k")) return false;
+    const uint64_t m = (a.n + BM - 1) / BM, n = (a.w_rows + BN - 1) / BN;
+    if (m * n > 0x7fffffu) {
+        set_error("q4mi_f8_mul: too many tiles");
+        return false;
+    }
+    a.m_tiles = (uint32_t)m, a.blocks = (uint32_t)(m * n);
+    k<<<dim3(a.blocks), dim3(64 * WM * WN), lds, stream()>>>(a);
+    return launch_ok("f8_tile_k");
+}
+
+template <uint32_t BM, uint32_t BN, uint32_t WM, uint32_t WN, uint32_t S>
+bool tile_pick(F8Args &a) {
+    return wide(a) ? tile_launch<BM, BN, WM, WN, S, true>(a)
+                   : tile_launch<BM, BN, WM, WN, S, false>(a);
+}
+
+// Which kernel a product of more than sixteen rows takes.
+bool mul_pick(F8Args &a) {
+    const uint64_t cus = cu_count();
+    auto tiles = [&](uint64_t bm, uint64_t bn) {
+        return ((a.n + bm - 1) / bm) * ((a.w_rows + bn - 1) / bn);
+    };
+    if (tiles(32, 32) <= 2 * cus) return tile_pick<32, 32, 2, 2, 8>(a);
+    if (tiles(64, 64) <= cus) return tile_pick<64, 64, 2, 2, 8>(a);
+    if (tiles(128, 64) <= cus) return tile_pick<128, 64, 2, 2, 6>(a);
+    if (tiles(128, 128) <= cus) return tile_pick<128, 128, 2, 2, 4>(a);
+    if (tiles(256, 128) <= cus) return tile_pick<256, 128, 4, 2, 3>(a);
+    return wide(a) ? tile_launch<128, 256, 2, 4, 2, true>(a) : tile_launch<256, 256, 2, 4, 2, false>(a);
+}
+
+bool id_launch(F8Args &a) {
+    constexpr size_t lds = kIdLists + kIdTiles;
+    a.blocks = 2 * (uint32_t)cu_count();
+    static DynLds st[2];
+    auto k = wide(a) ? f8_id_k<true> : f8_id_k<false>;
+    if (!dyn_lds_ok((const void *)k, lds, lds, st[wide(a)], "f8_id_k")) return false;
+    k<<<dim3(a.blocks), dim3(64 * kIdWaves), lds, stream()>>>(a);
+    return launch_ok("f8_id_k");
+}
 
 }  // namespace
 
@@ -484,12 +827,7 @@ bool q4mi_f8_mul(const uint8_t *d_w, const float *d_ws, uint64_t w_rows, uint64_
     if (!n) return true;
     if (n <= kFewRows)
         return few_launch(a, (uint32_t)n, 1, 1, 0, few_kernel, "f8_few_k");
-    if (n > 16 * 65535) {
-        set_error("q4mi_f8_mul: too many tiles");
-        return false;
-    }
-    f8_dense_k<<<dim3(tiles4(a), (uint32_t)((n + 15) / 16)), dim3(256), 0, stream()>>>(a);
-    return launch_ok("f8_dense_k");
+    return mul_pick(a);
 }
 
 /* Every row through its own expert (see include/q4mi.h). */
@@ -532,12 +870,7 @@ bool q4mi_f8_mul_id(const uint8_t *d_w, const float *d_ws, uint64_t w_rows, uint
         return false;
     }
     if (!total_rows || !xrows) return true;
-    if (total_rows > 16 * 64000) {
-        set_error("q4mi_f8_mul_id: too many tiles");
-        return false;
-    }
-    f8_id_k<<<dim3(tiles4(a), (uint32_t)(total_rows / 16 + n_expert)), dim3(256), 0, stream()>>>(a);
-    return launch_ok("f8_id_k");
+    return id_launch(a);
 }
 
 }  // extern "C"
