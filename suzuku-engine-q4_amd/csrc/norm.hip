@@ -54,20 +54,76 @@ __device__ inline void store_row8(void *p, uint32_t t, uint64_t row, uint32_t c0
     }
 }
 
-// h of eight columns.
-__device__ inline void norm_h(const NormArgs &a, uint64_t r, uint32_t c0, float *v) {
-    load_row8(a.x, a.x_type, r * a.ldx, c0, a.cols, v);
-    if (a.res) {
-        float u[8];
-        load_row8(a.res, a.r_type, r * a.ldr, c0, a.cols, u);
+// Eight columns as they are in memory (B bytes a value), so that a lane's loads
+// all go out before the first is converted.
+template <uint32_t B>
+struct Raw8 {
+    u32x4 q[B / 2];
+};
+template <uint32_t B>
+__device__ inline void load_raw8(const void *p, uint64_t row, uint32_t c0, uint32_t cols,
+                                 Raw8<B> &r) {
+    const uint8_t *at = (const uint8_t *)p + (row + c0) * B;
+    if (c0 + 8 <= cols) {
 #pragma unroll
-        for (int i = 0; i < 8; i++) v[i] += u[i];
-    }
-    if (a.res || a.sum) {
+        for (uint32_t i = 0; i < B / 2; i++) {
+            if constexpr (B == 4)
+                r.q[i] = *(const u32x4_a4 *)(at + 16 * i);
+            else
+                r.q[i] = *(const u32x4_a2 *)(at + 16 * i);
+        }
+    } else {
 #pragma unroll
-        for (int i = 0; i < 8; i++) v[i] = round_to(v[i], a.r_type);
+        for (uint32_t i = 0; i < B / 2; i++) r.q[i] = (u32x4){0, 0, 0, 0};
+        // columns past the last are 0
+#pragma unroll
+        for (uint32_t i = 0; i < 8; i++) {
+            if (c0 + i >= cols) continue;
+            if constexpr (B == 4)
+                r.q[i / 4][i % 4] = ((const uint32_t *)at)[i];
+            else
+                r.q[0][i / 2] |= (uint32_t)((const uint16_t *)at)[i] << (16 * (i % 2));
+        }
     }
 }
+template <uint32_t B>
+__device__ inline void raw8_to_f32(const Raw8<B> &r, uint32_t t, float *v) {
+    if constexpr (B == 4) {
+#pragma unroll
+        for (int i = 0; i < 8; i++) v[i] = bits_f32(r.q[i / 4][i % 4]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            const uint32_t h = i % 2 ? r.q[0][i / 2] >> 16 : r.q[0][i / 2] & 0xffffu;
+            v[i] = t == kTypeF16 ? (float)__builtin_bit_cast(_Float16, (uint16_t)h)
+                                 : bits_f32(h << 16);
+        }
+    }
+}
+
+// A lane's eight columns of x and of the residual.
+template <uint32_t XB, uint32_t RB>
+struct NormIn {
+    Raw8<XB> x;
+    Raw8<RB> r;
+    __device__ void load(const NormArgs &a, uint64_t row, uint32_t c0) {
+        load_raw8<XB>(a.x, row * a.ldx, c0, a.cols, x);
+        if (a.res) load_raw8<RB>(a.res, row * a.ldr, c0, a.cols, r);
+    }
+    __device__ void h(const NormArgs &a, float *v) const {
+        raw8_to_f32<XB>(x, a.x_type, v);
+        if (a.res) {
+            float u[8];
+            raw8_to_f32<RB>(r, a.r_type, u);
+#pragma unroll
+            for (int i = 0; i < 8; i++) v[i] += u[i];
+        }
+        if (RB == 2 && (a.res || a.sum)) {
+#pragma unroll
+            for (int i = 0; i < 8; i++) v[i] = round_to(v[i], a.r_type);
+        }
+    }
+};
 
 // Outputs of eight columns of row r from y; every lane of the wave is here.
 __device__ inline void norm_out(const NormArgs &a, uint64_t r, uint32_t c0, const float *y) {
@@ -98,8 +154,9 @@ __device__ inline void norm_out(const NormArgs &a, uint64_t r, uint32_t c0, cons
 constexpr uint32_t kNormGridX = 1u << 20;   // fewer than 2^32 threads along x
 
 // L lanes a row, I chunks of eight columns a lane in registers (lane l has
-// chunks l, l + L, ..); I = 0: any length, h read again after the sum.
-template <uint32_t L, uint32_t I>
+// chunks l, l + L, ..); I = 0: any length, h read again after the sum.  XB, RB:
+// bytes of x's values and the residual's.
+template <uint32_t L, uint32_t I, uint32_t XB, uint32_t RB>
 __global__ __launch_bounds__(L < 256 ? 256 : L) void rms_norm_k(NormArgs a) {
     constexpr uint32_t T = L < 256 ? 256 : L, NW = L / 64;
     const uint64_t r = ((uint64_t)blockIdx.y * kNormGridX + blockIdx.x) * (T / L) + threadIdx.x / L;
@@ -119,16 +176,21 @@ __global__ __launch_bounds__(L < 256 ? 256 : L) void rms_norm_k(NormArgs a) {
             for (int i = 0; i < 8; i++) u[i] = 1.f;
         }
     };
+    NormIn<XB, RB> in[I ? I : 1];
     if constexpr (I > 0) {
 #pragma unroll
-        for (uint32_t i = 0; i < I; i++) norm_h(a, r, 8 * (l + L * i), v[i]);
+        for (uint32_t i = 0; i < I; i++) in[i].load(a, r, 8 * (l + L * i));
 #pragma unroll
         for (uint32_t i = 0; i < I; i++) weights(8 * (l + L * i), w[i]);
 #pragma unroll
-        for (uint32_t i = 0; i < I; i++) add(v[i]);
+        for (uint32_t i = 0; i < I; i++) {
+            in[i].h(a, v[i]);
+            add(v[i]);
+        }
     } else {
         for (uint32_t c0 = 8 * l; c0 < a.cols; c0 += 8 * L) {
-            norm_h(a, r, c0, v[0]);
+            in[0].load(a, r, c0);
+            in[0].h(a, v[0]);
             add(v[0]);
         }
     }
@@ -159,7 +221,8 @@ __global__ __launch_bounds__(L < 256 ? 256 : L) void rms_norm_k(NormArgs a) {
     } else {
         // whole waves to the end of the last block
         for (uint32_t c0 = 8 * l; c0 - 8 * (l & 63u) < a.cols; c0 += 8 * L) {
-            norm_h(a, r, c0, v[0]);
+            in[0].load(a, r, c0);
+            in[0].h(a, v[0]);
             weights(c0, w[0]);
             out(c0, v[0], w[0]);
         }
@@ -215,7 +278,10 @@ bool norm_launch(const NormArgs &a) {
     const uint64_t blocks = (a.rows + per - 1) / per;
     const dim3 grid((uint32_t)std::min<uint64_t>(blocks, kNormGridX),
                     (uint32_t)((blocks + kNormGridX - 1) / kNormGridX));
-    rms_norm_k<L, I><<<grid, dim3(T), 0, stream()>>>(a);
+    const bool x4 = a.x_type == kTypeF32, r4 = !(a.res || a.sum) || a.r_type == kTypeF32;
+    auto k = x4 ? (r4 ? rms_norm_k<L, I, 4, 4> : rms_norm_k<L, I, 4, 2>)
+                : (r4 ? rms_norm_k<L, I, 2, 4> : rms_norm_k<L, I, 2, 2>);
+    k<<<grid, dim3(T), 0, stream()>>>(a);
     return launch_ok("rms_norm_k");
 }
 
@@ -234,7 +300,9 @@ bool q4mi_rms_norm(const void *d_x, uint32_t x_type, uint64_t ld_x, const void *
     if (!rows) return true;
     if (cols <= 512) return norm_launch<64, 1>(a);
     if (cols <= 2048) return norm_launch<256, 1>(a);
+    if (cols <= 4096) return norm_launch<256, 2>(a);
     if (cols <= 8192) return norm_launch<256, 4>(a);
+    if (cols <= 16384) return norm_launch<1024, 2>(a);
     if (cols <= 32768) return norm_launch<1024, 4>(a);
     return norm_launch<1024, 0>(a);
 }
