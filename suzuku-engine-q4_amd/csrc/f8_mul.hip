@@ -32,7 +32,7 @@ struct F8Args {
     void *y;
     uint64_t w_rows, cols, w_stride, ws_stride, ldx, xrows, n, ldy;
     uint32_t n_expert, x_type, y_type, x_div;
-    uint32_t ks, seg, blocks;       // waves a tile, blocks of K in LDS, workgroups
+    uint32_t ks, waves, seg, blocks;    // waves a tile, a workgroup; blocks of K in LDS; workgroups
     uint32_t m_tiles;               // tiles along the activations
 };
 
@@ -110,7 +110,12 @@ __device__ inline void add_scaled(v4f &acc, v4f d, float s) {
 // and their sums are joined in LDS in wave order, so a short matrix still
 // occupies the chip; a workgroup goes over several tiles, so a tall one pays the
 // LDS fill once.
-constexpr uint32_t kFewRows = 16, kFewWaves = 4;
+//
+// Measured, codes to BF16: one row through 151936 x 2048 58 us (5.4 TB/s), 8192 x
+// 8192 14.6 us (4.6 TB/s), 2560 x 2560 4.7 us (an empty launch: 2 us); sixteen rows
+// 66.5, 20.5 and 5.8 us.  What bounds the middle ones is how much a CU can have on
+// its way with loads to registers, 30 KB/us.
+constexpr uint32_t kFewRows = 16, kFewWaves = 8;     // at most
 
 // LDS strides of a row's codes and scales, seg blocks: 16 bytes more than a
 // multiple of 128, so that the rows of a fragment start in different banks.
@@ -130,39 +135,56 @@ struct FewRange {
 };
 
 // Blocks [b0, b0 + seg) of the rows into LDS; blocks from nb on get codes and
-// scales of 0.
+// scales of 0.  Four loads a lane are on their way at once (of float rows, two
+// blocks).
 __device__ inline void few_stage(const F8Args &a, const FewRange &f, uint32_t b0, uint32_t seg,
                                  uint32_t nb, uint8_t *codes, uint8_t *scales) {
-    constexpr uint32_t T = kFewWaves * 64;
     const uint32_t cld = few_code_ld(seg), sld = few_scale_ld(seg);
     if (a.x_type == kTypeF8) {
-        const uint32_t lane = threadIdx.x & 63u;
-#pragma unroll 2
-        for (uint32_t t = threadIdx.x >> 6; t < f.rows; t += kFewWaves) {
+        const uint32_t lane = threadIdx.x & 63u, here = min(seg, nb - b0);
+        for (uint32_t t = threadIdx.x >> 6; t < f.rows; t += a.waves) {
             const uint64_t xr = f.x_row(t);
-            const u32x4 *c = (const u32x4 *)((const uint8_t *)a.x + xr * (128ull * nb));
-            const float *s = a.xs + xr * nb;
-            for (uint32_t i = lane; i < seg * 8; i += 64)
-                *(u32x4 *)(codes + t * cld + 16u * i) =
-                    b0 + i / 8 < nb ? c[8 * b0 + i] : (u32x4){0, 0, 0, 0};
+            const u32x4 *c = (const u32x4 *)((const uint8_t *)a.x + xr * (128ull * nb)) + 8 * b0;
+            const float *s = a.xs + xr * nb + b0;
             for (uint32_t i = lane; i < seg; i += 64)
-                *(float *)(scales + t * sld + 4u * i) = b0 + i < nb ? s[b0 + i] : 0.f;
+                *(float *)(scales + t * sld + 4u * i) = i < here ? s[i] : 0.f;
+            for (uint32_t i = lane; i < seg * 8; i += 256) {
+                u32x4 v[4];
+#pragma unroll
+                for (uint32_t u = 0; u < 4; u++)
+                    v[u] = i + 64 * u < here * 8 ? c[i + 64 * u] : (u32x4){0, 0, 0, 0};
+#pragma unroll
+                for (uint32_t u = 0; u < 4; u++)
+                    if (i + 64 * u < seg * 8) *(u32x4 *)(codes + t * cld + 16u * (i + 64 * u)) = v[u];
+            }
         }
         return;
     }
     // sixteen lanes a block, eight values each
-    for (uint32_t i = threadIdx.x; i < f.rows * seg * 16; i += T) {
-        const uint32_t sub = i & 15u, q = i >> 4, t = q / seg, b = q - t * seg;
-        uint32_t code[2] = {0, 0}, s = 0;
-        if (b0 + b < nb) {
-            float v[8];
-            load_row8(a.x, a.x_type, f.x_row(t) * a.ldx, 128u * (b0 + b) + 8u * sub,
-                      (uint32_t)a.cols, v);
-            s = f8_scale_of(f8_max_lanes<16>(f8_top<8>(v)));
-            f8_pack<8>(v, s, code);
+    const uint32_t step = 64 * a.waves, end = f.rows * seg * 16;
+    for (uint32_t i = threadIdx.x; i < end; i += 2 * step) {
+        float v[2][8];
+        uint32_t t[2], b[2];
+#pragma unroll
+        for (uint32_t u = 0; u < 2; u++) {
+            const uint32_t q = (i + u * step) >> 4;
+            t[u] = q / seg, b[u] = q - t[u] * seg;
+#pragma unroll
+            for (int k = 0; k < 8; k++) v[u][k] = 0.f;
+            if (i + u * step < end && b0 + b[u] < nb)
+                load_row8(a.x, a.x_type, f.x_row(t[u]) * a.ldx, 128u * (b0 + b[u]) + 8u * (i & 15u),
+                          (uint32_t)a.cols, v[u]);
         }
-        *(u32x2 *)(codes + t * cld + 128u * b + 8u * sub) = (u32x2){code[0], code[1]};
-        if (sub == 0) *(uint32_t *)(scales + t * sld + 4u * b) = s;
+#pragma unroll
+        for (uint32_t u = 0; u < 2; u++) {
+            if (i + u * step >= end) break;
+            uint32_t code[2], s = f8_scale_of(f8_max_lanes<16>(f8_top<8>(v[u])));
+            f8_pack<8>(v[u], s, code);
+            if (b0 + b[u] >= nb) s = 0;
+            *(u32x2 *)(codes + t[u] * cld + 128u * b[u] + 8u * (i & 15u)) =
+                (u32x2){code[0], code[1]};
+            if ((i & 15u) == 0) *(uint32_t *)(scales + t[u] * sld + 4u * b[u]) = s;
+        }
     }
 }
 
@@ -174,7 +196,7 @@ __device__ inline void few_rows(const F8Args &a, const uint8_t *w, const float *
     const uint32_t lane = threadIdx.x & 63u;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t m = lane & 15u, g = lane >> 4;
-    const uint32_t ks = a.ks, kw = wave & (ks - 1), sub = wave / ks, per = kFewWaves / ks;
+    const uint32_t ks = a.ks, kw = wave & (ks - 1), sub = wave / ks, per = a.waves / ks;
     const uint32_t nb = f8_blocks(a.cols), last = (uint32_t)((a.w_rows + 15) / 16);
     const uint32_t seg = a.seg, nseg = (nb + seg - 1) / seg;
     const uint32_t cld = few_code_ld(seg), sld = few_scale_ld(seg);
@@ -280,16 +302,17 @@ __global__ __launch_bounds__(64 * kFewWaves) void f8_few_k(F8Args a) {
 }
 
 // Rows through the experts that the list names; grid (blocks, rows).  GROUP:
-// rows of one expert among 256 go together, sixteen at a time, so that its
+// rows of one expert among kSelRows go together, sixteen at a time, so that its
 // weights are read once: the first of them does the work, the others'
 // workgroups end.
-constexpr size_t kSelList = 4 * 8 + kFewRows * 4;
+constexpr uint32_t kSelRows = 256, kSelSets = kSelRows / 64;
+constexpr size_t kSelList = kSelSets * 8 + kFewRows * 4;
 template <bool FULL, bool GROUP>
 __global__ __launch_bounds__(64 * kFewWaves) void f8_sel_k(F8Args a) {
     extern __shared__ __align__(16) uint8_t lds[];
-    uint64_t *same = (uint64_t *)lds;           // which of the 256 rows are of this expert
-    uint32_t *list = (uint32_t *)(same + 4);
-    const uint32_t p = blockIdx.y, p0 = p & ~255u, q = p0 + threadIdx.x;
+    uint64_t *same = (uint64_t *)lds;           // which of the rows are of this expert
+    uint32_t *list = (uint32_t *)(same + kSelSets);
+    const uint32_t p = blockIdx.y, p0 = p & ~(kSelRows - 1), q = p0 + threadIdx.x;
     const int32_t e = a.eid[p];
     if (e < 0 || (uint32_t)e >= a.n_expert) return;
     const uint8_t *w = a.w + e * a.w_stride;
@@ -299,25 +322,25 @@ __global__ __launch_bounds__(64 * kFewWaves) void f8_sel_k(F8Args a) {
         few_rows<FULL>(a, w, ws, f, blockIdx.x, lds);
         return;
     }
-    const uint64_t bits = __ballot(q < a.n && a.eid[q] == e);
-    if ((threadIdx.x & 63u) == 0) same[threadIdx.x >> 6] = bits;
+    const uint64_t bits = __ballot(threadIdx.x < kSelRows && q < a.n && a.eid[q] == e);
+    if ((threadIdx.x & 63u) == 0 && threadIdx.x < kSelRows) same[threadIdx.x >> 6] = bits;
     __syncthreads();
     // how many of them lie before place i
     auto before = [&](uint32_t i) {
         uint32_t c = 0;
 #pragma unroll
-        for (uint32_t w = 0; w < 4; w++)
+        for (uint32_t w = 0; w < kSelSets; w++)
             c += i >= 64 * w + 64 ? (uint32_t)__popcll(same[w])
                  : i > 64 * w     ? (uint32_t)__popcll(same[w] & ((1ull << (i - 64 * w)) - 1))
                                   : 0u;
         return c;
     };
-    const uint32_t rank = before(p - p0), rows = min(before(256) - rank, kFewRows);
+    const uint32_t rank = before(p - p0), rows = min(before(kSelRows) - rank, kFewRows);
     if (rank % kFewRows) return;
     FewRange f = {p, rows, a.x_div, nullptr};
     if (rows > 1) {
         const uint32_t mine = before(threadIdx.x) - rank;
-        if ((same[threadIdx.x >> 6] >> (threadIdx.x & 63u) & 1u) && mine < rows)
+        if (threadIdx.x < kSelRows && (same[threadIdx.x >> 6] >> (threadIdx.x & 63u) & 1u) && mine < rows)
             list[mine] = threadIdx.x;
         __syncthreads();
         f.p0 = p0, f.list = list;
@@ -713,49 +736,59 @@ bool mul_ok(const char *who, const F8Args &a, bool rows) {
 
 constexpr uint64_t kFloatRows = 16;     // float rows that q4mi_f8_mul takes
 
-// K segment of the few-rows kernels for `rows` activation rows a workgroup:
-// whole rows where they fit in `room` bytes, else equal parts of whole chunks;
-// returns the LDS bytes.
-size_t few_fit(F8Args &a, uint32_t rows, size_t room) {
-    const uint32_t nb = f8_blocks(a.cols);
-    uint32_t parts = 1;
-    size_t need;
+constexpr uint32_t kFewLds = 76 * 1024;     // of activation rows: two workgroups a CU
+constexpr uint32_t kFewFour = 48 * 1024;    // three
+inline uint64_t few_lds(uint32_t rows, uint32_t seg) {
+    return (uint64_t)rows * (few_code_ld(seg) + few_scale_ld(seg));
+}
+// Blocks of K at a time of `rows` activation rows a workgroup: all where they fit,
+// else equal parts of whole chunks.
+uint32_t few_seg(uint64_t cols, uint32_t rows) {
+    const uint32_t nb = f8_blocks(cols);
+    uint32_t parts = 1, seg;
     do {
-        a.seg = ((nb + parts - 1) / parts + 1) / 2 * 2;
-        need = (size_t)rows * (few_code_ld(a.seg) + few_scale_ld(a.seg));
+        seg = ((nb + parts - 1) / parts + 1) / 2 * 2;
         parts++;
-    } while (need > room && a.seg > 2);
-    return (need + 15) / 16 * 16 + (a.ks > 1 ? kFewWaves * 64 * sizeof(v4f) : 0);
+    } while (few_lds(rows, seg) > kFewLds && seg > 2);
+    return seg;
 }
 
 // One set of `rows` (<= 16) activation rows a workgroup, `lists` of them, of
-// which about `busy` have work.  As many workgroups as are resident at once, each
-// with the same number of rounds.  Waves a tile: as many as there are chunks,
-// while the whole launch has fewer than 8 waves a CU.
-template <class F>
-bool few_launch(F8Args &a, uint32_t rows, uint32_t lists, uint32_t busy, size_t extra, F pick,
+// which about `busy` have work.
+//
+// Waves a tile: as many as there are chunks, up to eight, while the whole launch
+// has fewer than 8 waves a CU.  Workgroups have eight waves where a tile has, or
+// where the rows leave LDS for no more than two of them, which then share them;
+// else four (one row, us, four / eight: 2048 x 8192 11.6 / 9.8, 4096 x 4096 8.2 /
+// 7.4, 8192 x 8192 16.2 / 18.6, 12288 x 8192 22.0 / 28.2; sixteen rows, 8192 x 8192
+// 30.5 / 24.8).
+//
+// Three workgroups of four waves (two of eight) a CU, all with the same number of
+// rounds: more of them at once ask memory for too many places (151936 x 2048, one
+// row: two 56.8, three 58.1, four 67.2, six 63.8 us; 100000 x 1024: 26.4, 23.8,
+// 24.2, 24.1).
+typedef void (*F8Kernel)(F8Args);
+template <F8Kernel EVEN, F8Kernel ODD>     // blocks of K
+bool few_launch(F8Args &a, uint32_t rows, uint32_t lists, uint32_t busy, size_t extra,
                 const char *name) {
-    const uint64_t tiles = (a.w_rows + 15) / 16;
-    const uint32_t chunks = (f8_blocks(a.cols) + 1) / 2;
+    const uint64_t tiles = (a.w_rows + 15) / 16, all = tiles * busy, cus = cu_count();
+    const uint32_t nb = f8_blocks(a.cols), chunks = (nb + 1) / 2;
+    a.seg = few_seg(a.cols, rows);
     a.ks = 1;
-    while (a.ks < kFewWaves && a.ks * 2 <= chunks && tiles * busy * a.ks < 8ull * cu_count())
-        a.ks *= 2;
-    const size_t lds = extra + few_fit(a, rows, 36 * 1024);
-    const uint64_t sets = (tiles * a.ks + kFewWaves - 1) / kFewWaves;
-    const uint64_t resident = std::max(1u, 4u * cu_count() / busy);
+    while (a.ks < kFewWaves && a.ks * 2 <= chunks && all * a.ks < 8 * cus) a.ks *= 2;
+    a.waves = a.ks == kFewWaves || few_lds(rows, a.seg) > kFewFour ? kFewWaves : kFewWaves / 2;
+    const size_t lds = extra + (few_lds(rows, a.seg) + 15) / 16 * 16 +
+                       (a.ks > 1 ? a.waves * 64 * sizeof(v4f) : 0);
+    const uint64_t sets = (tiles * a.ks + a.waves - 1) / a.waves;
+    const uint64_t resident = std::max<uint64_t>(1, (a.waves == kFewWaves ? 2 : 3) * cus / busy);
     const uint64_t rounds = (sets + resident - 1) / resident;
     a.blocks = (uint32_t)((sets + rounds - 1) / rounds);
-    auto k = pick(f8_blocks(a.cols) % 2 == 0);
-    k<<<dim3(a.blocks, lists), dim3(64 * kFewWaves), lds, stream()>>>(a);
+    static DynLds st[2];
+    const F8Kernel k = nb % 2 ? ODD : EVEN;
+    if (!dyn_lds_ok((const void *)k, lds, 80 * 1024, st[nb % 2], name)) return false;
+    k<<<dim3(a.blocks, lists), dim3(64 * a.waves), lds, stream()>>>(a);
     return launch_ok(name);
 }
-typedef void (*F8Kernel)(F8Args);
-F8Kernel few_kernel(bool full) { return full ? f8_few_k<true> : f8_few_k<false>; }
-F8Kernel sel_kernel(bool full) { return full ? f8_sel_k<true, false> : f8_sel_k<false, false>; }
-F8Kernel sel_group_kernel(bool full) {
-    return full ? f8_sel_k<true, true> : f8_sel_k<false, true>;
-}
-
 // fp32 outputs are summed in fp32 throughout, 16-bit ones on the 8-bit matrix
 // instruction, whose cut-off lies 2^-6 below their rounding.
 bool wide(const F8Args &a) { return a.y_type == kTypeF32; }
@@ -782,12 +815,14 @@ bool tile_pick(F8Args &a) {
                    : tile_launch<BM, BN, WM, WN, S, false>(a);
 }
 
-// Which kernel a product of more than sixteen rows takes.
+// Which kernel a product takes.
 bool mul_pick(F8Args &a) {
     const uint64_t cus = cu_count();
     auto tiles = [&](uint64_t bm, uint64_t bn) {
         return ((a.n + bm - 1) / bm) * ((a.w_rows + bn - 1) / bn);
     };
+    if (a.n <= kFewRows)
+        return few_launch<f8_few_k<true>, f8_few_k<false>>(a, (uint32_t)a.n, 1, 1, 0, "f8_few_k");
     if (tiles(32, 32) <= 2 * cus) return tile_pick<32, 32, 2, 2, 8>(a);
     if (tiles(64, 64) <= cus) return tile_pick<64, 64, 2, 2, 8>(a);
     if (tiles(128, 64) <= cus) return tile_pick<128, 64, 2, 2, 6>(a);
@@ -825,8 +860,6 @@ bool q4mi_f8_mul(const uint8_t *d_w, const float *d_ws, uint64_t w_rows, uint64_
         return false;
     }
     if (!n) return true;
-    if (n <= kFewRows)
-        return few_launch(a, (uint32_t)n, 1, 1, 0, few_kernel, "f8_few_k");
     return mul_pick(a);
 }
 
@@ -847,10 +880,12 @@ bool q4mi_f8_mul_sel(const uint8_t *d_w, const float *d_ws, uint64_t w_rows, uin
     }
     if (!n) return true;
     const uint32_t lists = (uint32_t)n;
-    if (4 * n < n_expert) return few_launch(a, 1, lists, lists, 0, sel_kernel, "f8_sel_k");
-    return few_launch(a, std::min(lists, kFewRows), lists,
-                      std::min(lists, n_expert + lists / kFewRows), kSelList, sel_group_kernel,
-                      "f8_sel_k");
+    if (4 * n < n_expert)
+        return few_launch<f8_sel_k<true, false>, f8_sel_k<false, false>>(a, 1, lists, lists, 0,
+                                                                         "f8_sel_k");
+    return few_launch<f8_sel_k<true, true>, f8_sel_k<false, true>>(
+        a, std::min(lists, kFewRows), lists, std::min(lists, n_expert + lists / kFewRows), kSelList,
+        "f8_sel_k");
 }
 
 /* Packed rows, each expert's in one stretch (see include/q4mi.h). */
