@@ -461,9 +461,14 @@ __device__ inline void tile(const F8Args &a, const uint8_t *w, const float *ws, 
         const uint32_t c = wave * RA + q, to = base + kScales + (v & 1u) * kWin + c * 256;
         const uint32_t d = min(8 * v + ((lane & 7u) ^ (c & 7u)), nb - 1);
         if (GATHER) {
-            uint32_t r = xo[0];
+            // not xo[q], nor choices that become it: an index puts the array into memory
+            uint32_t r = 0;
 #pragma unroll
-            for (uint32_t j = 1; j < RA; j++) r = q == j ? xo[j] : r;
+            for (uint32_t j = 0; j < RA; j++) {
+                uint32_t mask = q == j ? ~0u : 0u;
+                asm("" : "+v"(mask));
+                r |= xo[j] & mask;
+            }
             copy4(xs + (uint64_t)r * nb + d, to);
         } else {
             copy4(xs, 4 * (min(c * 8 + l8, xlast) * nb + d), to);
