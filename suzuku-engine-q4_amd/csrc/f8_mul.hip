@@ -415,8 +415,11 @@ __device__ inline void tile(const F8Args &a, const uint8_t *w, const float *ws, 
     static_assert(S - 2 + RA <= 8, "a window's scales land in time");
     constexpr uint32_t kX = BM * 128, kW = BN * 128, kWin = BM * 32;
     constexpr uint32_t kWeights = S * kX, kScales = S * (kX + kW);
-    const uint32_t lane = threadIdx.x & 63u, l8 = lane >> 3;
-    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    // opaque, or what follows from it would be kept from one tile to the next, spilled
+    uint32_t tid = threadIdx.x;
+    asm volatile("" : "+v"(tid));
+    const uint32_t lane = tid & 63u, l8 = lane >> 3;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const uint32_t nb = f8_blocks(a.cols);
     const uint32_t base = (uint32_t)(uintptr_t)lds;     // LDS offset: low half of the address
     const uint32_t row_bytes = 128 * nb;
@@ -609,23 +612,32 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void f8_tile_k(F8Args a) {
 
 // ------------------------------------------------------------- packed rows
 //
-// Persistent workgroups, two a CU, go over the experts' sets of up to 128 rows x
-// 128 weight rows, each in the tile that its rows fill: mostly a few rows, so that
-// reading the weights bounds it, and one workgroup's first copies and last stores
-// are covered by the other's stages.  Every workgroup makes the lists of sets by
+// Persistent workgroups go over the experts' sets of up to ROWS rows x ROWS weight
+// rows, each in the tile that its rows fill.  With 128, two a CU: mostly a few
+// rows, so that reading the weights bounds it, and one workgroup's first copies and
+// last stores are covered by the other's stages.  With 256, one a CU: many rows an
+// expert, so that a tile's two sides should be read as seldom as they can be.
+// Every workgroup makes the lists of sets by
 // itself, as prefix sums over the experts' stretches in LDS: no scratch in memory,
 // no launch before.  It takes every a.blocks-th of them, the large ones first, so
 // that all have as many of each size (512 experts of 1024 x 2048, 2048 tokens of
-// ten picks: 257 us, 280 in the experts' order, with Zipf's popularities, 235 and
+// ten picks: 254 us, 280 in the experts' order, with Zipf's popularities, 235 and
 // 248 with equal ones; 4.4 and 4.8 TB/s).
-constexpr uint32_t kIdExperts = 1024, kIdRows = 128, kIdCols = 128, kIdWaves = 4;
-// LDS: each expert's last set of more than 64 rows, of 33 to 64, of up to 32
+constexpr uint32_t kIdExperts = 1024;
+// LDS: each expert's last set of more than half of ROWS, of less, of up to a quarter
 struct IdLists {
     uint32_t most[kIdExperts];
     uint16_t half[kIdExperts], few[kIdExperts];
 };
-constexpr uint32_t kIdTiles = tile_lds<128, kIdCols, 2>();     // the largest of them
-static_assert(2 * (sizeof(IdLists) + kIdTiles) <= 160 * 1024, "two workgroups a CU");
+// Sets of up to ROWS rows x ROWS weight rows: LDS of the largest tile.
+template <uint32_t ROWS>
+constexpr uint32_t id_tiles() {
+    return ROWS == 128 ? tile_lds<128, 128, 2>() : tile_lds<128, 256, 3>();
+}
+template <uint32_t ROWS>
+constexpr size_t id_lds() { return sizeof(IdLists) + id_tiles<ROWS>(); }
+static_assert(2 * id_lds<128>() <= 160 * 1024, "two workgroups a CU");
+static_assert(id_lds<256>() <= 160 * 1024 && tile_lds<256, 256, 2>() <= id_tiles<256>(), "one");
 
 // The first of n ascending sums that is above i.
 template <class T>
@@ -641,9 +653,10 @@ __device__ inline uint32_t owner(const T *ends, uint32_t n, uint32_t i) {
     return __builtin_amdgcn_readfirstlane(lo);
 }
 
-template <bool WIDE>
-__global__ __launch_bounds__(64 * kIdWaves, 2) void f8_id_k(F8Args a) {
+template <uint32_t ROWS, bool WIDE>
+__global__ __launch_bounds__(ROWS * 2, 2) void f8_id_k(F8Args a) {
     extern __shared__ __align__(16) uint8_t lds[];
+    constexpr uint32_t kWaves = ROWS / 32;
     IdLists &list = *(IdLists *)lds;
     uint8_t *work = lds + sizeof(IdLists);
     // without a row list, packed row p is activation row p: those past xrows do not exist
@@ -654,16 +667,16 @@ __global__ __launch_bounds__(64 * kIdWaves, 2) void f8_id_k(F8Args a) {
         return min((int64_t)a.bounds[e + 1], end) - *lo;
     };
     // sums of the experts' sets: of more than 64 rows, and in one word the others
-    constexpr uint32_t kEach = kIdExperts / (64 * kIdWaves);
+    constexpr uint32_t kEach = kIdExperts / (64 * kWaves);
     uint32_t most[kEach], less[kEach], m = 0, l = 0;
 #pragma unroll
     for (uint32_t i = 0; i < kEach; i++) {
         const uint32_t e = threadIdx.x * kEach + i;
         int64_t lo, rows = e < n ? stretch(e, &lo) : 0;
         rows = max(rows, (int64_t)0);
-        const uint32_t rest = (uint32_t)rows % kIdRows;
-        m += (uint32_t)(rows / kIdRows) + (rest > 64 ? 1u : 0u);
-        l += rest == 0 || rest > 64 ? 0u : rest > 32 ? 1u << 16 : 1u;
+        const uint32_t rest = (uint32_t)rows % ROWS;
+        m += (uint32_t)(rows / ROWS) + (rest > ROWS / 2 ? 1u : 0u);
+        l += rest == 0 || rest > ROWS / 2 ? 0u : rest > ROWS / 4 ? 1u << 16 : 1u;
         most[i] = m, less[i] = l;
     }
     uint32_t *tmp = (uint32_t *)work, vm = m, vl = l;
@@ -673,13 +686,13 @@ __global__ __launch_bounds__(64 * kIdWaves, 2) void f8_id_k(F8Args a) {
         const uint32_t om = __shfl_up(vm, d, 64), ol = __shfl_up(vl, d, 64);
         if (lane >= d) vm += om, vl += ol;
     }
-    if (lane == 63) tmp[wave] = vm, tmp[kIdWaves + wave] = vl;
+    if (lane == 63) tmp[wave] = vm, tmp[kWaves + wave] = vl;
     __syncthreads();
     uint32_t all_m = 0, all_l = 0;
     vm -= m, vl -= l;
-    for (uint32_t i = 0; i < kIdWaves; i++) {
-        if (i < wave) vm += tmp[i], vl += tmp[kIdWaves + i];
-        all_m += tmp[i], all_l += tmp[kIdWaves + i];
+    for (uint32_t i = 0; i < kWaves; i++) {
+        if (i < wave) vm += tmp[i], vl += tmp[kWaves + i];
+        all_m += tmp[i], all_l += tmp[kWaves + i];
     }
 #pragma unroll
     for (uint32_t i = 0; i < kEach; i++) {
@@ -689,7 +702,7 @@ __global__ __launch_bounds__(64 * kIdWaves, 2) void f8_id_k(F8Args a) {
         list.few[e] = (uint16_t)(vl + less[i]);
     }
     __syncthreads();
-    const uint32_t slices = (uint32_t)((a.w_rows + kIdCols - 1) / kIdCols);
+    const uint32_t slices = (uint32_t)((a.w_rows + ROWS - 1) / ROWS);
     const uint32_t n_most = __builtin_amdgcn_readfirstlane(all_m);
     const uint32_t n_less = __builtin_amdgcn_readfirstlane(all_l), n_half = n_less >> 16;
     const uint64_t items = ((uint64_t)n_most + n_half + (n_less & 0xffffu)) * slices;
@@ -701,24 +714,26 @@ __global__ __launch_bounds__(64 * kIdWaves, 2) void f8_id_k(F8Args a) {
             e = owner(list.most, n, unit);
             const uint32_t before = e ? list.most[e - 1] : 0u;
             all = stretch(e, &lo);
-            skip = (int64_t)__builtin_amdgcn_readfirstlane(unit - before) * kIdRows;
+            skip = (int64_t)__builtin_amdgcn_readfirstlane(unit - before) * ROWS;
         } else {
             e = unit - n_most < n_half ? owner(list.half, n, unit - n_most)
                                        : owner(list.few, n, unit - n_most - n_half);
             all = stretch(e, &lo);
-            skip = all / kIdRows * kIdRows;
+            skip = all / ROWS * ROWS;
         }
         if (skip < 0 || skip >= all) continue;      // never, with bounds that ascend
-        const uint32_t rows = (uint32_t)min((int64_t)kIdRows, all - skip);
+        const uint32_t rows = (uint32_t)min((int64_t)ROWS, all - skip);
         const uint8_t *w = a.w + e * a.w_stride;
         const float *ws = (const float *)((const uint8_t *)a.ws + e * a.ws_stride);
-        const uint64_t r0 = (uint64_t)part * kIdCols, p0 = (uint64_t)(lo + skip), phi = p0 + rows;
-        if (rows <= 32)
-            tile<32, kIdCols, 2, 2, 3, WIDE, true>(a, w, ws, r0, p0, phi, work);
-        else if (rows <= 64)
-            tile<64, kIdCols, 2, 2, 2, WIDE, true>(a, w, ws, r0, p0, phi, work);
+        const uint64_t r0 = (uint64_t)part * ROWS, p0 = (uint64_t)(lo + skip), phi = p0 + rows;
+        constexpr uint32_t kWn = ROWS / 64;
+        if (rows <= ROWS / 4)
+            tile<ROWS / 4, ROWS, 2, kWn, 3, WIDE, true>(a, w, ws, r0, p0, phi, work);
+        else if (rows <= ROWS / 2)
+            tile<ROWS / 2, ROWS, 2, kWn, ROWS == 128 ? 2 : 3, WIDE, true>(a, w, ws, r0, p0, phi,
+                                                                          work);
         else
-            tile<128, kIdCols, 2, 2, 2, WIDE, true>(a, w, ws, r0, p0, phi, work);
+            tile<ROWS, ROWS, 2, kWn, 2, WIDE, true>(a, w, ws, r0, p0, phi, work);
         __syncthreads();    // the next item overwrites what slower waves may still read
     }
 }
@@ -858,14 +873,22 @@ bool mul_pick(F8Args &a) {
     return wide(a) ? tile_launch<128, 256, 2, 4, 2, true>(a) : tile_launch<256, 256, 2, 4, 2, false>(a);
 }
 
+template <uint32_t ROWS, bool WIDE>
 bool id_launch(F8Args &a) {
-    constexpr size_t lds = sizeof(IdLists) + kIdTiles;
-    a.blocks = 2 * (uint32_t)cu_count();
-    static DynLds st[2];
-    auto k = wide(a) ? f8_id_k<true> : f8_id_k<false>;
-    if (!dyn_lds_ok((const void *)k, lds, lds, st[wide(a)], "f8_id_k")) return false;
-    k<<<dim3(a.blocks), dim3(64 * kIdWaves), lds, stream()>>>(a);
+    constexpr size_t lds = id_lds<ROWS>();
+    a.blocks = (ROWS == 128 ? 2 : 1) * (uint32_t)cu_count();
+    static DynLds st;
+    auto k = f8_id_k<ROWS, WIDE>;
+    if (!dyn_lds_ok((const void *)k, lds, lds, st, "f8_id_k")) return false;
+    k<<<dim3(a.blocks), dim3(2 * ROWS), lds, stream()>>>(a);
     return launch_ok("f8_id_k");
+}
+// Sets of 256 rows from 128 rows an expert on (128 experts of 1024 x 2048, 128 / 256
+// rows a set, us: 64 rows each 73 / 75, 128 rows 99 / 91, 256 rows 156 / 136, 1024
+// rows 530 / 419).  fp32 sums on the bf16 instruction have no registers for them.
+bool id_pick(F8Args &a) {
+    if (wide(a)) return id_launch<128, true>(a);
+    return a.n >= 128ull * a.n_expert ? id_launch<256, false>(a) : id_launch<128, false>(a);
 }
 
 }  // namespace
@@ -932,7 +955,7 @@ bool q4mi_f8_mul_id(const uint8_t *d_w, const float *d_ws, uint64_t w_rows, uint
         return false;
     }
     if (!total_rows || !xrows) return true;
-    return id_launch(a);
+    return id_pick(a);
 }
 
 }  // extern "C"
