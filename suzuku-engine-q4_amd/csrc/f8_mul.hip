@@ -778,8 +778,10 @@ bool mul_ok(const char *who, const F8Args &a, bool rows) {
 
 constexpr uint64_t kFloatRows = 16;     // float rows that q4mi_f8_mul takes
 
-constexpr uint32_t kFewLds = 76 * 1024;     // of activation rows: two workgroups a CU
-constexpr uint32_t kFewFour = 48 * 1024;    // three
+// LDS for activation rows: two workgroups a CU with a list and the waves' sums; three
+constexpr size_t kFewAll = 80 * 1024;
+constexpr size_t kFewLds = kFewAll - kSelList - kFewWaves * 64 * sizeof(v4f) - 16;
+constexpr size_t kFewFour = 48 * 1024;
 inline uint64_t few_lds(uint32_t rows, uint32_t seg) {
     return (uint64_t)rows * (few_code_ld(seg) + few_scale_ld(seg));
 }
@@ -827,7 +829,7 @@ bool few_launch(F8Args &a, uint32_t rows, uint32_t lists, uint32_t busy, size_t 
     a.blocks = (uint32_t)((sets + rounds - 1) / rounds);
     static DynLds st[2];
     const F8Kernel k = nb % 2 ? ODD : EVEN;
-    if (!dyn_lds_ok((const void *)k, lds, 80 * 1024, st[nb % 2], name)) return false;
+    if (!dyn_lds_ok((const void *)k, lds, kFewAll, st[nb % 2], name)) return false;
     k<<<dim3(a.blocks, lists), dim3(64 * a.waves), lds, stream()>>>(a);
     return launch_ok(name);
 }

@@ -11,7 +11,9 @@ Codes and scales are exact.  Products come in two kinds of data:
     (2^-24 if to nearest; hardware sums may cut off); the two scales' product and
     its use with the addition 2^-24 each; nb blocks and at most 32 parts of them
     are added.  So y is off by at most (2 * 128 + 2 + nb + 32) * 2^-24 * S, then
-    by one rounding to its type.
+    by one rounding to its type.  16-bit outputs of more than sixteen rows may lose
+    more in one eight of products (test_gpu_f8_paths has that bound); the data here
+    stay within the narrower one.
 """
 import numpy as np
 import pytest
