@@ -169,3 +169,75 @@ def test_router_front(gpu, wt, T, gate):
 def test_no_tokens(gpu):
     q4mi.check(gpu.q4mi_route_scored(None, 0, 8, 0, 8, None, 1, 1, 1, 1, 2, True, 1.0, None, None,
                                      None, 2, -1, None), "route")
+
+
+GROUPS = [(1, 1, 1), (8, 4, 2), (8, 2, 1), (12, 5, 2)]
+
+
+def bias_and_logits(E, T, seed):
+    rng = np.random.default_rng(seed)
+    z = rng.integers(-6, 7, (T, E)) / 4
+    return rng, z.astype(np.float32)
+
+
+@pytest.mark.parametrize("sigmoid", [0, 1])
+@pytest.mark.parametrize("with_bias", [False, True])
+@pytest.mark.parametrize("groups,keep,group_top", GROUPS)
+@pytest.mark.parametrize("E,topk", [(48, 8), (480, 10), (480, 64), (960, 33)])
+def test_many_ties(gpu, E, topk, groups, keep, group_top, with_bias, sigmoid):
+    """Logits of 13 values and biases of 4: most keys have equals, also at the last
+    pick and the last group, and more than 64 of them may be in question."""
+    rng, z = bias_and_logits(E, 40, E + topk)
+    z[3], z[4, ::2], z[5] = 0.25, -1.0, -np.inf
+    # one bias a group: two of a group's sum with each other's biases would be a tie
+    # of the mathematics, not of the rounded keys
+    bias = rng.integers(0, 4, E) if groups == 1 else np.repeat(rng.integers(0, 4, groups),
+                                                               E // groups)
+    bias = (bias / 64).astype(np.float32) if with_bias else None
+    got = route(gpu, dev(z), 0, topk, sigmoid, None if bias is None else dev(bias), groups, keep,
+                group_top)
+    same(got, ref.route(z, topk, sigmoid, bias, groups, keep, group_top))
+
+
+@pytest.mark.parametrize("sigmoid", [0, 1])
+@pytest.mark.parametrize("groups,keep,group_top", GROUPS)
+def test_biases_that_cancel(gpu, groups, keep, group_top, sigmoid):
+    """A group's two best keys of opposite signs and 10^4 times the scores, so that
+    the groups differ in the last bits of an fp32 of either; biases next to one
+    another in fp32."""
+    rng, z = bias_and_logits(480, 60, 5)
+    z += rng.standard_normal(z.shape).astype(np.float32) / 8
+    bias = np.full(480, -2.0 ** 13, np.float32)
+    bias[::480 // groups] = 2.0 ** 13
+    for b in (bias, bias * 2.0 ** -11, bias + rng.integers(0, 2, 480).astype(np.float32) / 1024):
+        got = route(gpu, dev(z), 0, 9, sigmoid, dev(b), groups, keep, group_top)
+        same(got, ref.route(z, 9, sigmoid, b, groups, keep, group_top))
+
+
+@pytest.mark.parametrize("sigmoid", [0, 1])
+@pytest.mark.parametrize("groups,keep,group_top", GROUPS)
+def test_largest_biases(gpu, groups, keep, group_top, sigmoid):
+    """Biases of +-inf, NaN and the largest finite ones (two of which are no fp32)."""
+    rng, z = bias_and_logits(480, 30, 6)
+    z[2, 10:30] = np.finfo(np.float32).max
+    z[3] = np.finfo(np.float32).min
+    z[4, 5] = np.inf
+    big = np.finfo(np.float32).max
+    b = rng.choice(np.array([0, 1, big, -big, np.inf, -np.inf, np.nan], np.float32), 480,
+                   p=[.3, .3, .1, .1, .05, .1, .05])
+    got = route(gpu, dev(z), 0, 12, sigmoid, dev(b), groups, keep, group_top)
+    same(got, ref.route(z, 12, sigmoid, b, groups, keep, group_top))
+
+
+def test_nearest_keys(gpu):
+    """Keys a few last bits of an fp32 apart, of which the hardware's exponential
+    says nothing: the order of 64 bits."""
+    rng = np.random.default_rng(8)
+    E, T = 512, 200
+    base = np.float32(1.5) + np.arange(E, dtype=np.float32) * np.float32(2.0 ** -23)
+    z = np.stack([rng.permutation(base) for _ in range(T)])
+    for sigmoid in (0, 1):
+        for bias in (None, np.full(E, 2.0 ** -9, np.float32)):
+            for g in ((1, 1, 1), (8, 4, 2)):
+                got = route(gpu, dev(z), 0, 10, sigmoid, None if bias is None else dev(bias), *g)
+                same(got, ref.route(z, 10, sigmoid, bias, *g))
