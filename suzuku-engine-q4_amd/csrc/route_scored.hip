@@ -122,6 +122,7 @@ struct ScorePlaces {
         return (l >> shift) * size + (l & ((1u << shift) - 1)) + (j << shift);
     }
     __device__ uint32_t mine(uint32_t j) const { return of(lane, j); }
+    __device__ uint32_t last() const { return (lane >> shift) * size + size - 1; }
     __device__ bool is(uint32_t j) const {
         return (lane & ((1u << shift) - 1)) + (j << shift) < size;
     }
@@ -230,7 +231,7 @@ __device__ inline bool keys_fast(const ScoreArgs &a, const ScorePlaces &at, cons
         for (uint32_t j = 0; j < NJ; j++) key[j] += bias[j];
     }
 #pragma unroll
-    for (uint32_t j = 0; j < NJ; j++) key[j] = z[j] == none || key[j] != key[j] ? none : key[j];
+    for (uint32_t j = 0; j < NJ; j++) key[j] = z[j] == none ? none : fmaxf(key[j], none);  // NaN
     if (a.n_group == 1) return true;
     float b0 = none, b1 = none;
     auto merge = [](float &x0, float &x1, float y0, float y1) {
@@ -267,9 +268,12 @@ __device__ inline bool keys_fast(const ScoreArgs &a, const ScorePlaces &at, cons
     }
     const bool stays = ahead < a.topk_group && best != none;
     const bool sure = best == none || ahead >= a.topk_group || near < a.topk_group;
+    if (!a.bias) {
 #pragma unroll
-    for (uint32_t j = 0; j < NJ; j++)
-        key[j] = !stays || key[j] == none ? none : a.bias ? key[j] : z[j];
+        for (uint32_t j = 0; j < NJ; j++) key[j] = z[j];
+    }
+#pragma unroll
+    for (uint32_t j = 0; j < NJ; j++) key[j] = stays ? key[j] : none;
     return __all(sure);
 }
 
@@ -277,8 +281,8 @@ __device__ inline bool keys_fast(const ScoreArgs &a, const ScorePlaces &at, cons
 // (-inf: none) that are off by at most half of gap + 2^-22 of their size, or not at
 // all (gap 0: equal ones may differ in 64 bits).  exact(e): expert e's key there.
 //
-// A key is an unsigned number of the same order whose lowest bits give way to the
-// lane's slot.  Finds go on until one is behind the last pick for certain; if
+// A key is an unsigned number of the same order (-inf: below kFinite) whose lowest
+// bits give way to the lane's slot.  Finds go on until one is behind the last pick for certain; if
 // some of them are not apart, their 64-bit keys, after ready(), give their order.
 template <uint32_t NJ, class Ready, class Exact>
 __device__ inline int32_t pick_experts(const ScoreArgs &a, const ScorePlaces &at, const float *key,
@@ -286,17 +290,14 @@ __device__ inline int32_t pick_experts(const ScoreArgs &a, const ScorePlaces &at
                                        Exact exact) {
     const double none = -(double)INFINITY;
     const uint32_t lane = at.lane;
-    constexpr uint32_t kSlot = NJ - 1;
+    constexpr uint32_t kSlot = NJ - 1, kFinite = 0x00800000;
     const float part = gap > 0.f ? 0x1p-22f : 0.f;
     // the highest and lowest that a key stands for
     auto above = [](uint32_t m) { return key2f(m | kSlot); };
     auto below = [](uint32_t m) { return key2f(m & ~kSlot); };
-    uint32_t high[NJ], alive = 0;
+    uint32_t high[NJ];
 #pragma unroll
-    for (uint32_t j = 0; j < NJ; j++) {
-        alive |= key[j] == -INFINITY ? 0u : 1u << j;
-        high[j] = key[j] == -INFINITY ? 0u : (f2key(key[j]) & ~kSlot) | (kSlot - j);
-    }
+    for (uint32_t j = 0; j < NJ; j++) high[j] = (f2key(key[j]) & ~kSlot) | (kSlot - j);
     // a lane's in descending order (odd-even merge sort): its best is the first
 #pragma unroll
     for (uint32_t p = 1; p < NJ; p *= 2)
@@ -316,7 +317,7 @@ __device__ inline int32_t pick_experts(const ScoreArgs &a, const ScorePlaces &at
     bool done = false;
     for (; k < 64; k++) {
         const uint32_t m = wave_max_u32(high[0]);
-        if (!m || (k >= a.topk && above(m) < end)) {
+        if (m < kFinite || (k >= a.topk && above(m) < end)) {
             done = true;
             break;
         }
@@ -353,6 +354,9 @@ __device__ inline int32_t pick_experts(const ScoreArgs &a, const ScorePlaces &at
     }
     // more near ones than lanes: the best key, on a tie of the lowest expert, topk times
     ready();
+    uint32_t alive = 0;
+#pragma unroll
+    for (uint32_t j = 0; j < NJ; j++) alive |= key[j] == -INFINITY ? 0u : 1u << j;
     pick = -1;
     for (k = 0; k < a.topk; k++) {
         double best = none;
@@ -382,8 +386,8 @@ __device__ inline int32_t pick_experts(const ScoreArgs &a, const ScorePlaces &at
 // picks alone where those are near each other.
 //
 // Measured at 8192 tokens, fp32 logits: 512 experts, 10 picks with bias and 4 of 8
-// groups 18 us (55 us with 64-bit scores of every expert), without either 12.5 us
-// (1.35 TB/s), 128 experts 7 us; one token 3.6 to 5.4 us.  8 waves a SIMD, at the
+// groups 17 us (55 us with 64-bit scores of every expert; 14.6 us where no keys are
+// near), without either 12 us (1.4 TB/s), 128 experts 7 us; one token 3.6 to 5 us.  8 waves a SIMD, at the
 // price of spills in the 64-bit path, against 5 without: 11.8 against 12.4 us
 // without bias and groups, 8.7 against 9.7 us for 256 experts with a bias.
 template <uint32_t NJ>
@@ -395,35 +399,42 @@ __global__ __launch_bounds__(64 * kScoreWaves, NJ <= 8 ? 8 : 4) void route_score
     const ScorePlaces at(a, lane);
     // Of the logits +inf counts as the largest finite one, NaN as -inf.
     auto counted = [](float z) { return z != z ? -INFINITY : fminf(z, 3.402823466e38f); };
-    // all loads go out before the first is used: one choice of the type for them
-    float z[NJ], bias[NJ], top = -INFINITY;
-    if (a.type == kTypeF32) {
+    // All loads go out before the first is used, with one choice of the type for
+    // them, at 32-bit offsets from the row; a lane without a jth expert reads the last
+    // one's place of its group.
+    float z[NJ], bias[NJ];
+    uint32_t off[NJ];
 #pragma unroll
-        for (uint32_t j = 0; j < NJ; j++)
-            z[j] = at.is(j) ? ((const float *)a.logits + row)[at.mine(j)] : -INFINITY;
+    for (uint32_t j = 0; j < NJ; j++) off[j] = at.is(j) ? at.mine(j) : at.last();
+    if (a.type == kTypeF32) {
+        const char *base = (const char *)a.logits + row * 4;
+#pragma unroll
+        for (uint32_t j = 0; j < NJ; j++) z[j] = *(const float *)(base + off[j] * 4u);
     } else {
+        const char *base = (const char *)a.logits + row * 2;
         uint16_t q[NJ];
 #pragma unroll
-        for (uint32_t j = 0; j < NJ; j++)
-            q[j] = at.is(j) ? ((const uint16_t *)a.logits + row)[at.mine(j)] : 0;
+        for (uint32_t j = 0; j < NJ; j++) q[j] = *(const uint16_t *)(base + off[j] * 2u);
 #pragma unroll
-        for (uint32_t j = 0; j < NJ; j++) {
-            const float v = a.type == kTypeF16 ? (float)__builtin_bit_cast(_Float16, q[j])
-                                               : bits_f32((uint32_t)q[j] << 16);
-            z[j] = at.is(j) ? v : -INFINITY;
-        }
+        for (uint32_t j = 0; j < NJ; j++)
+            z[j] = a.type == kTypeF16 ? (float)__builtin_bit_cast(_Float16, q[j])
+                                      : bits_f32((uint32_t)q[j] << 16);
     }
     if (a.bias) {
 #pragma unroll
-        for (uint32_t j = 0; j < NJ; j++) bias[j] = at.is(j) ? a.bias[at.mine(j)] : 0.f;
+        for (uint32_t j = 0; j < NJ; j++)
+            bias[j] = *(const float *)((const char *)a.bias + off[j] * 4u);
     }
 #pragma unroll
-    for (uint32_t j = 0; j < NJ; j++) {
-        z[j] = counted(z[j]);
-        top = fmaxf(top, z[j]);
-    }
+    for (uint32_t j = 0; j < NJ; j++) z[j] = at.is(j) ? counted(z[j]) : -INFINITY;
     const bool softmax = !a.sigmoid;
-    const float zmax = softmax ? key2f(wave_max_u32(f2key(top))) : 0.f;
+    float zmax = 0.f;
+    if (softmax) {
+        float top = z[0];
+#pragma unroll
+        for (uint32_t j = 1; j < NJ; j++) top = fmaxf(top, z[j]);
+        zmax = key2f(wave_max_u32(f2key(top)));
+    }
     Scores score = {softmax, (double)zmax, 1.};
     bool far = false;       // a sigmoid below 2^-1000
     bool settled = false;
