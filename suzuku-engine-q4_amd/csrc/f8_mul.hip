@@ -629,15 +629,21 @@ struct IdLists {
     uint32_t most[kIdExperts];
     uint16_t half[kIdExperts], few[kIdExperts];
 };
-// Sets of up to ROWS rows x ROWS weight rows: LDS of the largest tile.
+// Sets of up to ROWS rows x ROWS weight rows: waves and workgroups a CU, the sizes
+// of the sets that have tiles of their own, stages of each, the largest tile's LDS.
 template <uint32_t ROWS>
-constexpr uint32_t id_tiles() {
-    return ROWS == 128 ? tile_lds<128, 128, 2>() : tile_lds<128, 256, 3>();
-}
-template <uint32_t ROWS>
-constexpr size_t id_lds() { return sizeof(IdLists) + id_tiles<ROWS>(); }
-static_assert(2 * id_lds<128>() <= 160 * 1024, "two workgroups a CU");
-static_assert(id_lds<256>() <= 160 * 1024 && tile_lds<256, 256, 2>() <= id_tiles<256>(), "one");
+struct IdSets {
+    static constexpr uint32_t kWaves = ROWS == 256 ? 8 : 4;
+    static constexpr uint32_t kCu = ROWS == 32 || ROWS == 128 ? 2 : 1;
+    static constexpr uint32_t kHalf = ROWS == 32 ? 0 : ROWS / 2, kFew = ROWS < 128 ? 0 : ROWS / 4;
+    static constexpr uint32_t kAllS = ROWS < 128 ? 8 : 2;
+    static constexpr uint32_t kHalfS = ROWS < 128 ? 8 : ROWS == 128 ? 2 : 3, kFewS = 3;
+    static constexpr uint32_t kTiles =
+        std::max({tile_lds<ROWS, ROWS, kAllS>(), tile_lds<kHalf, ROWS, kHalfS>(),
+                  tile_lds<kFew, ROWS, kFewS>()});
+    static constexpr size_t kLds = sizeof(IdLists) + kTiles;
+    static_assert(kCu * kLds <= 160 * 1024, "workgroups a CU");
+};
 
 // The first of n ascending sums that is above i.
 template <class T>
@@ -654,9 +660,10 @@ __device__ inline uint32_t owner(const T *ends, uint32_t n, uint32_t i) {
 }
 
 template <uint32_t ROWS, bool WIDE>
-__global__ __launch_bounds__(ROWS * 2, 2) void f8_id_k(F8Args a) {
+__global__ __launch_bounds__(64 * IdSets<ROWS>::kWaves, 2) void f8_id_k(F8Args a) {
     extern __shared__ __align__(16) uint8_t lds[];
-    constexpr uint32_t kWaves = ROWS / 32;
+    typedef IdSets<ROWS> Sets;
+    constexpr uint32_t kWaves = Sets::kWaves, kHalf = Sets::kHalf, kFew = Sets::kFew;
     IdLists &list = *(IdLists *)lds;
     uint8_t *work = lds + sizeof(IdLists);
     // without a row list, packed row p is activation row p: those past xrows do not exist
@@ -675,8 +682,8 @@ __global__ __launch_bounds__(ROWS * 2, 2) void f8_id_k(F8Args a) {
         int64_t lo, rows = e < n ? stretch(e, &lo) : 0;
         rows = max(rows, (int64_t)0);
         const uint32_t rest = (uint32_t)rows % ROWS;
-        m += (uint32_t)(rows / ROWS) + (rest > ROWS / 2 ? 1u : 0u);
-        l += rest == 0 || rest > ROWS / 2 ? 0u : rest > ROWS / 4 ? 1u << 16 : 1u;
+        m += (uint32_t)(rows / ROWS) + (rest > kHalf ? 1u : 0u);
+        l += rest == 0 || rest > kHalf ? 0u : rest > kFew ? 1u << 16 : 1u;
         most[i] = m, less[i] = l;
     }
     uint32_t *tmp = (uint32_t *)work, vm = m, vl = l;
@@ -726,14 +733,16 @@ __global__ __launch_bounds__(ROWS * 2, 2) void f8_id_k(F8Args a) {
         const uint8_t *w = a.w + e * a.w_stride;
         const float *ws = (const float *)((const uint8_t *)a.ws + e * a.ws_stride);
         const uint64_t r0 = (uint64_t)part * ROWS, p0 = (uint64_t)(lo + skip), phi = p0 + rows;
-        constexpr uint32_t kWn = ROWS / 64;
-        if (rows <= ROWS / 4)
-            tile<ROWS / 4, ROWS, 2, kWn, 3, WIDE, true>(a, w, ws, r0, p0, phi, work);
-        else if (rows <= ROWS / 2)
-            tile<ROWS / 2, ROWS, 2, kWn, ROWS == 128 ? 2 : 3, WIDE, true>(a, w, ws, r0, p0, phi,
-                                                                          work);
-        else
-            tile<ROWS, ROWS, 2, kWn, 2, WIDE, true>(a, w, ws, r0, p0, phi, work);
+        if (rows > kHalf) {
+            tile<ROWS, ROWS, 2, kWaves / 2, Sets::kAllS, WIDE, true>(a, w, ws, r0, p0, phi, work);
+        } else if (rows > kFew) {
+            if constexpr (kHalf > 0)
+                tile<kHalf, ROWS, 2, kWaves / 2, Sets::kHalfS, WIDE, true>(a, w, ws, r0, p0, phi,
+                                                                           work);
+        } else {
+            if constexpr (kFew > 0)
+                tile<kFew, ROWS, 2, kWaves / 2, Sets::kFewS, WIDE, true>(a, w, ws, r0, p0, phi, work);
+        }
         __syncthreads();    // the next item overwrites what slower waves may still read
     }
 }
@@ -872,25 +881,42 @@ bool mul_pick(F8Args &a) {
     if (tiles(128, 64) <= cus) return tile_pick<128, 64, 2, 2, 6>(a);
     if (tiles(128, 128) <= cus) return tile_pick<128, 128, 2, 2, 4>(a);
     if (tiles(256, 128) <= cus) return tile_pick<256, 128, 4, 2, 3>(a);
-    return wide(a) ? tile_launch<128, 256, 2, 4, 2, true>(a) : tile_launch<256, 256, 2, 4, 2, false>(a);
+    return wide(a) ? tile_launch<128, 128, 2, 2, 2, true>(a)
+                   : tile_launch<256, 256, 2, 4, 2, false>(a);
 }
 
 template <uint32_t ROWS, bool WIDE>
 bool id_launch(F8Args &a) {
-    constexpr size_t lds = id_lds<ROWS>();
-    a.blocks = (ROWS == 128 ? 2 : 1) * (uint32_t)cu_count();
+    constexpr size_t lds = IdSets<ROWS>::kLds;
+    a.blocks = IdSets<ROWS>::kCu * (uint32_t)cu_count();
     static DynLds st;
     auto k = f8_id_k<ROWS, WIDE>;
     if (!dyn_lds_ok((const void *)k, lds, lds, st, "f8_id_k")) return false;
-    k<<<dim3(a.blocks), dim3(2 * ROWS), lds, stream()>>>(a);
+    k<<<dim3(a.blocks), dim3(64 * IdSets<ROWS>::kWaves), lds, stream()>>>(a);
     return launch_ok("f8_id_k");
 }
-// Sets of 256 rows from 128 rows an expert on (128 experts of 1024 x 2048, 128 / 256
-// rows a set, us: 64 rows each 73 / 75, 128 rows 99 / 91, 256 rows 156 / 136, 1024
-// rows 530 / 419).  fp32 sums on the bf16 instruction have no registers for them.
+template <uint32_t ROWS>
+bool id_wide(F8Args &a) {
+    return wide(a) ? id_launch<ROWS, true>(a) : id_launch<ROWS, false>(a);
+}
+
+// Small sets with deep rings where the chip has room for all at once: then a set's
+// stages in a row are the time (8 experts of 1024 x 2048, 32 rows each, us: sets of
+// 32 rows 9.2, 64 11.4, 128 17.8; one of 2048 x 2048, 256 rows: 64 10.5, 128 35).
+// Sets of 256 rows from 128 rows an expert on, where they occupy the chip (128
+// experts of 1024 x 2048, 128 / 256 rows a set, us: 64 rows each 73 / 75, 128 rows
+// 99 / 91, 256 rows 156 / 136, 1024 rows 530 / 419; 8 experts of 2048 x 2048, 128
+// rows each, 96 sets at most: 24 / 37); fp32 sums on the bf16 instruction have no
+// registers for them.
 bool id_pick(F8Args &a) {
-    if (wide(a)) return id_launch<128, true>(a);
-    return a.n >= 128ull * a.n_expert ? id_launch<256, false>(a) : id_launch<128, false>(a);
+    const uint64_t cus = cu_count();
+    auto sets = [&](uint64_t rows) {    // at most
+        return (a.n / rows + std::min<uint64_t>(a.n, a.n_expert)) * ((a.w_rows + rows - 1) / rows);
+    };
+    if (sets(32) <= 2 * cus) return id_wide<32>(a);
+    if (sets(64) <= cus) return id_wide<64>(a);
+    if (a.n >= 128ull * a.n_expert && sets(256) > cus && !wide(a)) return id_launch<256, false>(a);
+    return id_wide<128>(a);
 }
 
 }  // namespace

@@ -96,14 +96,17 @@ def test_sums_below_a_large_product(gpu, n, yt):
     out.check()
 
 
-# Stretches of each size a set can have, of few rows an expert and of many (sets of
-# 128 and of 256 rows), more sets than workgroups, 1024 experts.
+# Stretches of each size a set can have, in sets of 32, 64, 128 and 256 rows (few of
+# them in all; rows an expert), more sets than workgroups, 1024 experts.
 @pytest.mark.parametrize("exact", [True, False])
 @pytest.mark.parametrize("counts,rows,cols,yt", [
     ([256, 1, 512, 64, 65, 128, 129, 300, 0, 257], 700, 900, 30),
     ([256, 1, 512, 64, 65, 128, 129, 300, 0, 257], 260, 900, 0),
     ([400, 600], 1030, 128, 1), ([130] * 9, 256, 1100, 30), ([32, 33, 64, 65, 96, 128, 1], 129, 130, 30),
-    ([0, 2, 1, 0] * 256, 40, 256, 30), ([3000], 300, 300, 1), ([31, 95, 127] * 30, 2050, 128, 0)])
+    ([0, 2, 1, 0] * 256, 40, 256, 30), ([3000], 300, 300, 1), ([31, 95, 127] * 30, 2050, 128, 0),
+    ([31, 95, 127, 0, 128, 200] * 15, 2050, 300, 30), ([700, 64, 65, 128, 129, 1, 256, 300], 6500, 300, 30),
+    ([700, 64, 65, 128, 129, 1, 256, 300], 6500, 130, 0), ([33, 40, 32, 1, 70], 1030, 1100, 30),
+    ([33, 40, 32, 1, 70], 1030, 1100, 0)])
 def test_id_every_set(gpu, counts, rows, cols, yt, exact):
     rng = np.random.default_rng(rows + len(counts))
     E, total = len(counts), sum(counts)
