@@ -36,13 +36,16 @@ struct F8Args {
     uint32_t m_tiles;               // tiles along the activations
 };
 
-// Four adjacent outputs, rounded once.
+// Four adjacent outputs, rounded once.  STREAM: around the caches, of large outputs.
+template <bool STREAM>
 __device__ inline void store4(void *y, uint32_t yt, uint64_t at, v4f v) {
     if (yt == kTypeF32) {
-        *(f32x4_a4 *)((float *)y + at) = (f32x4)v;
+        f32x4_a4 *p = (f32x4_a4 *)((float *)y + at);
+        STREAM ? __builtin_nontemporal_store((f32x4)v, p) : (void)(*p = (f32x4)v);
     } else {
         const u32x2 q = {f32_to_16x2(v[0], v[1], yt), f32_to_16x2(v[2], v[3], yt)};
-        *(u32x2_a2 *)((uint16_t *)y + at) = q;
+        u32x2_a2 *p = (u32x2_a2 *)((uint16_t *)y + at);
+        STREAM ? __builtin_nontemporal_store(q, p) : (void)(*p = q);
     }
 }
 
@@ -255,7 +258,7 @@ __device__ inline void few_rows(const F8Args &a, const uint8_t *w, const float *
         if (tile >= last || m >= f.rows) return;
         const uint64_t r = (uint64_t)tile * 16 + 4 * g, at = f.row(m) * a.ldy + r;
         if (r + 4 <= a.w_rows)
-            store4(a.y, a.y_type, at, acc);
+            store4<false>(a.y, a.y_type, at, acc);
         else
             for (uint32_t k = 0; k < 4; k++)
                 if (r + k < a.w_rows) store_from_f32(a.y, a.y_type, at + k, acc[k]);
@@ -563,6 +566,9 @@ __device__ inline void tile(const F8Args &a, const uint8_t *w, const float *ws, 
     constexpr uint32_t kRow = FN * 16 + 4, kLanes = FN * 4;   // floats a row, lanes that store one
     static_assert(NW * 16 * kRow * 4 <= tile_lds<BM, BN, S>(), "sums fit the stages");
     static_assert(kLanes <= 64, "a row's stores");
+    // (8192 x 8192 x 2048, us: through the caches 150, around them 135; K = 8192 465 and
+    // 454; 2048 rows 122 and 113.  Small outputs stay for who reads them next.)
+    constexpr bool kStream = BM * BN >= 128 * 128 || (GATHER && BN >= 128);
     landed_barrier<0>();
     float *sums = (float *)lds + wave * 16 * kRow;
     const uint64_t rw = r0 + wn * FN * 16 + lane % kLanes * 4;   // weight row of this lane's stores
@@ -583,7 +589,7 @@ __device__ inline void tile(const F8Args &a, const uint8_t *w, const float *ws, 
             const uint64_t at = (p1 + t) * a.ldy + rw;
             if (p1 + t >= phi || !listed(p1 + t)) continue;
             if (rw + 4 <= a.w_rows)
-                store4(a.y, a.y_type, at, v);
+                store4<kStream>(a.y, a.y_type, at, v);
             else
                 for (uint32_t n = 0; n < 4; n++)
                     if (rw + n < a.w_rows) store_from_f32(a.y, a.y_type, at + n, v[n]);
