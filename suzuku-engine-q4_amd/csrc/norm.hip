@@ -23,7 +23,7 @@ struct NormArgs {
     uint8_t *codes;
     float *scales;
     uint64_t ldx, ldr, ldy, rows;
-    uint32_t cols, x_type, r_type, w_type, y_type, q_type;
+    uint32_t cols, lanes, x_type, r_type, w_type, y_type, q_type;
     float eps;
 };
 
@@ -76,6 +76,7 @@ __device__ inline void load_raw8(const void *p, uint64_t row, uint32_t c0, uint3
 #pragma unroll
         for (uint32_t i = 0; i < B / 2; i++) r.q[i] = (u32x4){0, 0, 0, 0};
         // columns past the last are 0
+        if (c0 >= cols) return;
 #pragma unroll
         for (uint32_t i = 0; i < 8; i++) {
             if (c0 + i >= cols) continue;
@@ -153,15 +154,18 @@ __device__ inline void norm_out(const NormArgs &a, uint64_t r, uint32_t c0, cons
 
 constexpr uint32_t kNormGridX = 1u << 20;   // fewer than 2^32 threads along x
 
-// L lanes a row, I chunks of eight columns a lane in registers (lane l has
-// chunks l, l + L, ..); I = 0: any length, h read again after the sum.  XB, RB:
-// bytes of x's values and the residual's.
-template <uint32_t L, uint32_t I, uint32_t XB, uint32_t RB>
-__global__ __launch_bounds__(L < 256 ? 256 : L) void rms_norm_k(NormArgs a) {
-    constexpr uint32_t T = L < 256 ? 256 : L, NW = L / 64;
-    const uint64_t r = ((uint64_t)blockIdx.y * kNormGridX + blockIdx.x) * (T / L) + threadIdx.x / L;
-    if (r >= a.rows) return;    // whole waves; with L > 64 the whole workgroup
-    const uint32_t l = threadIdx.x % L;
+// a.lanes lanes a row (64: four rows a workgroup, else the workgroup), I chunks of
+// eight columns a lane in registers (lane l has chunks l, l + lanes, ..); I = 0: any
+// length, h read again after the sum.  XB, RB: bytes of x's values and the
+// residual's.
+template <uint32_t I, uint32_t XB, uint32_t RB>
+__global__ __launch_bounds__(I == 1 ? 256 : 1024) void rms_norm_k(NormArgs a) {
+    const uint32_t L = a.lanes, nw = L / 64;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint64_t block = (uint64_t)blockIdx.y * kNormGridX + blockIdx.x;
+    const uint64_t r = nw == 1 ? block * 4 + wave : block;
+    if (r >= a.rows) return;    // whole waves; with more than one a row the whole workgroup
+    const uint32_t l = nw == 1 ? threadIdx.x & 63u : threadIdx.x;
     float v[I ? I : 1][8], w[I ? I : 1][8];
     double sum = 0.;
     auto add = [&](const float *h) __attribute__((always_inline)) {
@@ -169,7 +173,7 @@ __global__ __launch_bounds__(L < 256 ? 256 : L) void rms_norm_k(NormArgs a) {
         for (int i = 0; i < 8; i++) sum = fma((double)h[i], (double)h[i], sum);
     };
     auto weights = [&](uint32_t c0, float *u) __attribute__((always_inline)) {
-        if (a.w) {
+        if (a.w && c0 < a.cols) {
             load_row8(a.w, a.w_type, 0, c0, a.cols, u);
         } else {
 #pragma unroll
@@ -199,13 +203,18 @@ __global__ __launch_bounds__(L < 256 ? 256 : L) void rms_norm_k(NormArgs a) {
     sum = __builtin_bit_cast(
         double, (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(bits >> 32), 63) << 32 |
                     (uint32_t)__builtin_amdgcn_readlane((int)bits, 63));
-    if constexpr (NW > 1) {
-        __shared__ double part[NW];
-        if ((threadIdx.x & 63u) == 0) part[threadIdx.x >> 6] = sum;
+    if (nw > 1) {
+        __shared__ double part[16];
+        if ((threadIdx.x & 63u) == 0) part[wave] = sum;
         __syncthreads();
         sum = 0.;
+        for (uint32_t k = 0; k < nw; k += 4) {      // four reads at once; past nw is nothing
+            double p[4];
 #pragma unroll
-        for (uint32_t k = 0; k < NW; k++) sum += part[k];
+            for (uint32_t i = 0; i < 4; i++) p[i] = part[k + i];
+#pragma unroll
+            for (uint32_t i = 0; i < 4; i++) sum += k + i < nw ? p[i] : 0.;
+        }
     }
     const float inv = (float)(1. / sqrt(sum / (double)a.cols + (double)a.eps));
     auto out = [&](uint32_t c0, float *h, const float *u) __attribute__((always_inline)) {
@@ -272,16 +281,23 @@ bool norm_ok(const NormArgs &a, uint64_t cols) {
     return true;
 }
 
-template <uint32_t L, uint32_t I>
-bool norm_launch(const NormArgs &a) {
-    constexpr uint32_t T = L < 256 ? 256 : L, per = T / L;
-    const uint64_t blocks = (a.rows + per - 1) / per;
+// As many waves a row as its chunks need, I a lane: one up to 2048 columns, then two,
+// as four waves' loads already cover memory's latency (bf16 with residual, 8 bits out,
+// 33.5 M values, us: 8192 x 4096 47, 46 with one; 6990 x 4800 58, 90 with four a lane
+// in 256; 4096 x 8192 49 and 59; 32768 x 1024 49, 70 with 256 lanes).  Memory bounds
+// it: 4 to 5.5 TB/s.
+template <uint32_t I>
+bool norm_launch(NormArgs &a) {
+    const uint32_t chunks = (a.cols + 7) / 8;
+    const uint32_t waves = I ? (chunks + 64 * I - 1) / (64 * I) : 16;
+    a.lanes = 64 * waves;
+    const uint64_t per = a.lanes == 64 ? 4 : 1, blocks = (a.rows + per - 1) / per;
     const dim3 grid((uint32_t)std::min<uint64_t>(blocks, kNormGridX),
                     (uint32_t)((blocks + kNormGridX - 1) / kNormGridX));
     const bool x4 = a.x_type == kTypeF32, r4 = !(a.res || a.sum) || a.r_type == kTypeF32;
-    auto k = x4 ? (r4 ? rms_norm_k<L, I, 4, 4> : rms_norm_k<L, I, 4, 2>)
-                : (r4 ? rms_norm_k<L, I, 2, 4> : rms_norm_k<L, I, 2, 2>);
-    k<<<grid, dim3(T), 0, stream()>>>(a);
+    auto k = x4 ? (r4 ? rms_norm_k<I, 4, 4> : rms_norm_k<I, 4, 2>)
+                : (r4 ? rms_norm_k<I, 2, 4> : rms_norm_k<I, 2, 2>);
+    k<<<grid, dim3(a.lanes * (uint32_t)per), 0, stream()>>>(a);
     return launch_ok("rms_norm_k");
 }
 
@@ -294,17 +310,14 @@ bool q4mi_rms_norm(const void *d_x, uint32_t x_type, uint64_t ld_x, const void *
                    uint32_t r_type, uint64_t ld_r, const void *d_w, uint32_t w_type, float eps,
                    uint64_t rows, uint64_t cols, void *d_y, uint32_t y_type, uint64_t ld_y,
                    uint32_t q_type, void *d_codes, float *d_scales) {
-    const NormArgs a = {d_x, d_res, d_w, d_sum, d_y, (uint8_t *)d_codes, d_scales, ld_x, ld_r,
-                        ld_y, rows, (uint32_t)cols, x_type, r_type, w_type, y_type, q_type, eps};
+    NormArgs a = {d_x, d_res, d_w, d_sum, d_y, (uint8_t *)d_codes, d_scales, ld_x, ld_r, ld_y,
+                  rows, (uint32_t)cols, 0, x_type, r_type, w_type, y_type, q_type, eps};
     if (!norm_ok(a, cols)) return false;
     if (!rows) return true;
-    if (cols <= 512) return norm_launch<64, 1>(a);
-    if (cols <= 2048) return norm_launch<256, 1>(a);
-    if (cols <= 4096) return norm_launch<256, 2>(a);
-    if (cols <= 8192) return norm_launch<256, 4>(a);
-    if (cols <= 16384) return norm_launch<1024, 2>(a);
-    if (cols <= 32768) return norm_launch<1024, 4>(a);
-    return norm_launch<1024, 0>(a);
+    if (cols <= 2048) return norm_launch<1>(a);
+    if (cols <= 16384) return norm_launch<2>(a);
+    if (cols <= 32768) return norm_launch<4>(a);
+    return norm_launch<0>(a);
 }
 
 }  // extern "C"
