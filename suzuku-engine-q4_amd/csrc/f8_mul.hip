@@ -875,6 +875,19 @@ bool tile_pick(F8Args &a) {
 }
 
 // Which kernel a product takes.
+//
+// While all its tiles are resident at once, the smallest of them, with as deep a
+// ring as LDS has room for: a CU takes in 43 to 56 KB/us that way, and a tile's time
+// is its bytes (8192 x 8192, us: 32 rows, 32 x 32 14.7, 64 x 64 23; 128 rows, 32 x 32
+// 31.4, 64 x 64 23.4, 128 x 64 34.9; 256 rows, 64 x 64 44, 128 x 64 35.2, 128 x 128
+// 48.5; 512 rows, 128 x 64 67.9, 128 x 128 48.9, 256 x 128 60; 1024 rows, 128 x 128
+// 95, 256 x 128 69.6, 256 x 256 101; 2048 rows, 256 x 128 140, 256 x 256 120).
+//
+// More tiles: of up to 128 rows those that hold them all, two workgroups a CU, so
+// that the weights come once (151936 x 2048, us, that / 256 x 256: 32 rows 61.6 / 99,
+// 64 rows 67.8 / 102, 128 rows 82 / 109); else the largest, which read the sides
+// least often (fp32 outputs have no registers for them: 128 x 128 in two workgroups
+// a CU, 8192 x 8192 x 2048 277 us, 128 x 256 in one 285).
 bool mul_pick(F8Args &a) {
     const uint64_t cus = cu_count();
     auto tiles = [&](uint64_t bm, uint64_t bn) {
@@ -883,12 +896,14 @@ bool mul_pick(F8Args &a) {
     if (a.n <= kFewRows)
         return few_launch<f8_few_k<true>, f8_few_k<false>>(a, (uint32_t)a.n, 1, 1, 0, "f8_few_k");
     if (tiles(32, 32) <= 2 * cus) return tile_pick<32, 32, 2, 2, 8>(a);
+    if (a.n <= 32) return tile_pick<32, 128, 2, 2, 3>(a);
     if (tiles(64, 64) <= cus) return tile_pick<64, 64, 2, 2, 8>(a);
+    if (a.n <= 64) return tile_pick<64, 128, 2, 2, 3>(a);
     if (tiles(128, 64) <= cus) return tile_pick<128, 64, 2, 2, 6>(a);
     if (tiles(128, 128) <= cus) return tile_pick<128, 128, 2, 2, 4>(a);
-    if (tiles(256, 128) <= cus) return tile_pick<256, 128, 4, 2, 3>(a);
-    return wide(a) ? tile_launch<128, 128, 2, 2, 2, true>(a)
-                   : tile_launch<256, 256, 2, 4, 2, false>(a);
+    if (a.n > 128 && tiles(256, 128) <= cus) return tile_pick<256, 128, 4, 2, 3>(a);
+    if (a.n <= 128 || wide(a)) return tile_pick<128, 128, 2, 2, 2>(a);
+    return tile_launch<256, 256, 2, 4, 2, false>(a);
 }
 
 template <uint32_t ROWS, bool WIDE>

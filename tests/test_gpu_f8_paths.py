@@ -27,12 +27,13 @@ def tall(rng, rows, cols):
     return (dev(c)[dev(to)].contiguous(), dev(s[pick])), lambda x: (x @ v.T)[:, to]
 
 
-# More tiles than a chip of 256 units has at once of each kind but the largest,
-# and the sizes at which 64 x 64, 128 x 64, 128 x 128, 256 x 128 and the largest
-# tiles begin there; whole numbers, so that sums are exact.
+# The sizes at which 64 x 64, 128 x 64, 128 x 128, 256 x 128 and the largest tiles
+# begin on a chip of 256 units, and more tiles than it has at once of up to 32, 64
+# and 128 rows; whole numbers, so that sums are exact.
 @pytest.mark.parametrize("yt", [0, 30])
 @pytest.mark.parametrize("n,rows", [(64, 8200), (130, 8100), (300, 8100), (520, 8100), (1100, 8100),
-                                    (257, 16300), (17, 17000)])
+                                    (257, 16300), (17, 17000),
+                                    (32, 40001), (33, 17000), (64, 70000), (65, 17000), (128, 40003)])
 @pytest.mark.parametrize("cols", [200, 1290])
 def test_mul_every_tile(gpu, n, rows, cols, yt):
     rng = np.random.default_rng(n + cols)
