@@ -89,4 +89,52 @@ __device__ inline void f8_unpack4(uint32_t q, float *v) {
     v[0] = a.x, v[1] = a.y, v[2] = b.x, v[3] = b.y;
 }
 
+// Eight columns as they are in memory (B bytes a value), so that a lane's loads
+// all go out before the first is converted.
+template <uint32_t B>
+struct Raw8 {
+    u32x4 q[B / 2];
+};
+template <uint32_t B>
+__device__ inline void load_raw8(const void *p, uint64_t row, uint32_t c0, uint32_t cols,
+                                 Raw8<B> &r) {
+    const uint8_t *at = (const uint8_t *)p + (row + c0) * B;
+    if (c0 + 8 <= cols) {
+#pragma unroll
+        for (uint32_t i = 0; i < B / 2; i++) {
+            if constexpr (B == 4)
+                r.q[i] = *(const u32x4_a4 *)(at + 16 * i);
+            else
+                r.q[i] = *(const u32x4_a2 *)(at + 16 * i);
+        }
+    } else {
+#pragma unroll
+        for (uint32_t i = 0; i < B / 2; i++) r.q[i] = (u32x4){0, 0, 0, 0};
+        // columns past the last are 0
+        if (c0 >= cols) return;
+#pragma unroll
+        for (uint32_t i = 0; i < 8; i++) {
+            if (c0 + i >= cols) continue;
+            if constexpr (B == 4)
+                r.q[i / 4][i % 4] = ((const uint32_t *)at)[i];
+            else
+                r.q[0][i / 2] |= (uint32_t)((const uint16_t *)at)[i] << (16 * (i % 2));
+        }
+    }
+}
+template <uint32_t B>
+__device__ inline void raw8_to_f32(const Raw8<B> &r, uint32_t t, float *v) {
+    if constexpr (B == 4) {
+#pragma unroll
+        for (int i = 0; i < 8; i++) v[i] = bits_f32(r.q[i / 4][i % 4]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            const uint32_t h = i % 2 ? r.q[0][i / 2] >> 16 : r.q[0][i / 2] & 0xffffu;
+            v[i] = t == kTypeF16 ? (float)__builtin_bit_cast(_Float16, (uint16_t)h)
+                                 : bits_f32(h << 16);
+        }
+    }
+}
+
 }  // namespace q4mi

@@ -137,9 +137,42 @@ struct FewRange {
     }
 };
 
+// Blocks [b0, b0 + seg) of float rows (XB bytes a value) into LDS: sixteen lanes a
+// block, eight values each, two blocks' loads on their way at once.
+template <uint32_t XB>
+__device__ inline void few_stage_floats(const F8Args &a, const FewRange &f, uint32_t b0,
+                                        uint32_t seg, uint32_t nb, uint8_t *codes,
+                                        uint8_t *scales) {
+    const uint32_t cld = few_code_ld(seg), sld = few_scale_ld(seg);
+    const uint32_t step = 64 * a.waves, end = f.rows * seg * 16, at = 8 * (threadIdx.x & 15u);
+    for (uint32_t i = threadIdx.x; i < end; i += 2 * step) {
+        Raw8<XB> raw[2];
+        uint32_t t[2], b[2];
+#pragma unroll
+        for (uint32_t u = 0; u < 2; u++) {
+            const uint32_t q = (i + u * step) >> 4;
+            t[u] = q / seg, b[u] = q - t[u] * seg;
+            // past the end and past K as columns past the last: zeros
+            const bool in = i + u * step < end && b0 + b[u] < nb;
+            load_raw8<XB>(a.x, f.x_row(in ? t[u] : 0) * a.ldx, 128u * (b0 + b[u]) + at,
+                          in ? (uint32_t)a.cols : 0u, raw[u]);
+        }
+#pragma unroll
+        for (uint32_t u = 0; u < 2; u++) {
+            if (i + u * step >= end) break;
+            float v[8];
+            raw8_to_f32<XB>(raw[u], a.x_type, v);
+            uint32_t code[2], s = f8_scale_of(f8_max_lanes<16>(f8_top<8>(v)));
+            f8_pack<8>(v, s, code);
+            if (b0 + b[u] >= nb) s = 0;
+            *(u32x2 *)(codes + t[u] * cld + 128u * b[u] + at) = (u32x2){code[0], code[1]};
+            if (at == 0) *(uint32_t *)(scales + t[u] * sld + 4u * b[u]) = s;
+        }
+    }
+}
+
 // Blocks [b0, b0 + seg) of the rows into LDS; blocks from nb on get codes and
-// scales of 0.  Four loads a lane are on their way at once (of float rows, two
-// blocks).
+// scales of 0.  Four loads a lane are on their way at once.
 __device__ inline void few_stage(const F8Args &a, const FewRange &f, uint32_t b0, uint32_t seg,
                                  uint32_t nb, uint8_t *codes, uint8_t *scales) {
     const uint32_t cld = few_code_ld(seg), sld = few_scale_ld(seg);
@@ -163,32 +196,10 @@ __device__ inline void few_stage(const F8Args &a, const FewRange &f, uint32_t b0
         }
         return;
     }
-    // sixteen lanes a block, eight values each
-    const uint32_t step = 64 * a.waves, end = f.rows * seg * 16;
-    for (uint32_t i = threadIdx.x; i < end; i += 2 * step) {
-        float v[2][8];
-        uint32_t t[2], b[2];
-#pragma unroll
-        for (uint32_t u = 0; u < 2; u++) {
-            const uint32_t q = (i + u * step) >> 4;
-            t[u] = q / seg, b[u] = q - t[u] * seg;
-#pragma unroll
-            for (int k = 0; k < 8; k++) v[u][k] = 0.f;
-            if (i + u * step < end && b0 + b[u] < nb)
-                load_row8(a.x, a.x_type, f.x_row(t[u]) * a.ldx, 128u * (b0 + b[u]) + 8u * (i & 15u),
-                          (uint32_t)a.cols, v[u]);
-        }
-#pragma unroll
-        for (uint32_t u = 0; u < 2; u++) {
-            if (i + u * step >= end) break;
-            uint32_t code[2], s = f8_scale_of(f8_max_lanes<16>(f8_top<8>(v[u])));
-            f8_pack<8>(v[u], s, code);
-            if (b0 + b[u] >= nb) s = 0;
-            *(u32x2 *)(codes + t[u] * cld + 128u * b[u] + 8u * (i & 15u)) =
-                (u32x2){code[0], code[1]};
-            if ((i & 15u) == 0) *(uint32_t *)(scales + t[u] * sld + 4u * b[u]) = s;
-        }
-    }
+    if (a.x_type == kTypeF32)
+        few_stage_floats<4>(a, f, b0, seg, nb, codes, scales);
+    else
+        few_stage_floats<2>(a, f, b0, seg, nb, codes, scales);
 }
 
 // Weight tiles of 16 rows, of which workgroup `block` of a.blocks takes every

@@ -54,7 +54,9 @@ __global__ __launch_bounds__(256) void f8_quant_k(const void *__restrict__ x, ui
 
 // A scale for each 128 x 128 values: one workgroup a block, sixteen lanes a
 // row of it with eight values each, so sixteen rows a step and eight steps,
-// whose values stay in registers until the block's largest is known.
+// whose values stay in registers until the block's largest is known.  XB: bytes of
+// a value; all loads go out before the first is converted.
+template <uint32_t XB>
 __global__ __launch_bounds__(256) void f8_quant_blocks_k(const void *__restrict__ x, uint32_t xt,
                                                          uint64_t ld,
                                                          const int32_t *__restrict__ ids,
@@ -67,6 +69,7 @@ __global__ __launch_bounds__(256) void f8_quant_blocks_k(const void *__restrict_
     const uint64_t rb = (rows + 127) / 128;
     const F8Place p(blockIdx.x, group, rb, nb);
     if (p.r >= rb) return;      // the whole workgroup
+    Raw8<XB> raw[8];
     float v[8][8];
     uint32_t top = 0;
 #pragma unroll
@@ -74,10 +77,13 @@ __global__ __launch_bounds__(256) void f8_quant_blocks_k(const void *__restrict_
         const uint64_t r = p.r * 128 + i * 16 + (threadIdx.x >> 4);
         const uint64_t src = ids && r < rows ? (uint64_t)(int64_t)ids[r] : r;
         // rows past the last have no values
-        load_row8(x, xt, src * ld, p.b * 128 + sub * 8, r < rows ? cols : 0u, v[i]);
+        load_raw8<XB>(x, src * ld, p.b * 128 + sub * 8, r < rows ? cols : 0u, raw[i]);
     }
 #pragma unroll
-    for (uint32_t i = 0; i < 8; i++) top = max(top, f8_top<8>(v[i]));
+    for (uint32_t i = 0; i < 8; i++) {
+        raw8_to_f32<XB>(raw[i], xt, v[i]);
+        top = max(top, f8_top<8>(v[i]));
+    }
     top = f8_max_lanes<16>(top);
     top = max(top, (uint32_t)__shfl_xor((int)top, 16, 64));
     top = max(top, (uint32_t)__shfl_xor((int)top, 32, 64));
@@ -202,8 +208,9 @@ bool q4mi_f8_quant(const void *d_x, uint32_t x_type, uint64_t ld_x, const int32_
     uint64_t group;
     if (block_rows == 128) {
         const dim3 grid = f8_grid(1, (rows + 127) / 128, cols, &group);
-        f8_quant_blocks_k<<<grid, dim3(256), 0, stream()>>>(d_x, x_type, ld_x, d_ids, rows, group,
-                                                            (uint32_t)cols, d_codes, d_scales);
+        auto k = x_type == kTypeF32 ? f8_quant_blocks_k<4> : f8_quant_blocks_k<2>;
+        k<<<grid, dim3(256), 0, stream()>>>(d_x, x_type, ld_x, d_ids, rows, group, (uint32_t)cols,
+                                            d_codes, d_scales);
         return launch_ok("f8_quant_blocks_k");
     }
     const bool f32 = x_type == kTypeF32;
