@@ -184,6 +184,11 @@ class Layer:
         f = [rng.standard_normal((E, H)) / 16, rng.standard_normal(H) + 2, rng.random(E) / 10]
         return ([[dev(a) for a in p] for p in q], [dev(a.astype(np.float32)) for a in f])
 
+    def pack(self, L):
+        o = [self.o[k].data_ptr() for k in ("ids", "wts", "atok", "rsrc", "rw", "stg", "stgn", "ek",
+                                            "bounds")]
+        q4mi.check(L.q4mi_assign(*o, self.T, self.K, self.E, self.T), "pack", L)
+
     def run(self, L, wt):
         (gu, dn, lm), (wr, nw, bias) = wt
         T, E, K, H, F, V = self.T, self.E, self.K, self.H, self.F, self.V
@@ -203,8 +208,7 @@ class Layer:
                                    None), "route")
         ok(L.q4mi_route_scored(p["logits"], 0, E, T, E, None, 0, 1, 1, 1, K, False, 1.0, p["ids2"],
                                p["wts2"], None, K, -1, None), "route")
-        ok(L.q4mi_assign(p["ids"], p["wts"], p["atok"], p["rsrc"], p["rw"], p["stg"], p["stgn"],
-                         p["ek"], p["bounds"], T, K, E, T), "pack")
+        self.pack(L)
         ok(L.q4mi_f8_mul_id(*arena(gu, 2 * F, H), p["c"], p["s"], T, p["atok"], p["bounds"], R,
                             p["g"], 0, 2 * F), "gate/up")
         ok(L.q4_mmq_swiglu(p["g"], p["hid"], R, F), "swiglu")
@@ -298,25 +302,26 @@ def test_layer(gpu):
     assert (off <= room + 2.0 ** -8 * (np.abs(want) + room)).all()
 
 
-def test_layer_in_a_graph(gpu):
-    """Two captured graphs of the layer, on buffers of their own, replayed in turn
-    with eager work between: the bits that eager runs give."""
+def test_layer_in_a_graph(gpu, gpu_meas):
+    """Two captured graphs of the layer, on buffers of their own and of a library whose
+    first calls they are, replayed in turn with eager work between: the bits that eager
+    runs give."""
     rng = np.random.default_rng(22)
     wt = Layer.weights(rng)
     got, eager, graphs = [Layer(rng), Layer(rng)], Layer(rng), []
-    for a in got:
-        a.fill(rng)
-        a.run(gpu, wt)
+    eager.fill(rng)
+    eager.run(gpu, wt)
+    eager.pack(gpu_meas)        # has scratch of its own, allocated outside of captures
     torch.cuda.synchronize()
     try:
         for a in got:
             g = torch.cuda.CUDAGraph()
             with torch.cuda.graph(g):
-                q4mi.use_torch_stream()
-                a.run(gpu, wt)
+                q4mi.use_torch_stream(gpu_meas)
+                a.run(gpu_meas, wt)
             graphs.append(g)
     finally:
-        q4mi.use_torch_stream()
+        q4mi.use_torch_stream(gpu_meas)
     for i in range(4):
         for a, g in zip(got, graphs):
             a.fill(rng)
@@ -356,3 +361,17 @@ def test_layer_on_two_streams(gpu):
     for a, w in zip(layers, want):
         for k in w:
             assert torch.equal(a.o[k], w[k]), k
+
+
+@pytest.mark.parametrize("yt", sorted(TYPES))
+@pytest.mark.parametrize("rows,cols,pad,block", [(5000, 4099, 2, 1), (4200, 4096, 0, 128)])
+def test_dequant_large(gpu, yt, rows, cols, pad, block):
+    """Outputs past 32 MiB."""
+    rng = np.random.default_rng(rows)
+    c, s, v = random_rows(rng, rows, cols, False, block)
+    y = torch.full((rows, cols + pad), 77.0, dtype=TYPES[yt], device="cuda")
+    d = [dev(a) for a in (c, s)]
+    q4mi.check(gpu.q4mi_f8_dequant(d[0].data_ptr(), d[1].data_ptr(), None, rows, cols, block,
+                                   y.data_ptr(), yt, cols + pad), "dequant")
+    assert torch.equal(y[:, :cols], dev(v.astype(np.float32)).to(TYPES[yt]))
+    assert (y[:, cols:] == 77).all()
