@@ -145,3 +145,24 @@ def test_many_rows(gpu):
     v = x.double()
     want = v / torch.sqrt((v * v).mean(1, keepdim=True) + 1e-6)
     assert ((y.double() - want).abs() <= (2.0 ** -8 + 4 * 2.0 ** -24) * want.abs()).all()
+
+
+@pytest.mark.parametrize("cols", [512, 513, 1024, 1030, 1536, 2048, 2049, 2100, 3000, 4800, 5900,
+                                  6400, 7168, 8190, 9000, 10240, 11000, 12289, 13000, 14336, 15400,
+                                  16384, 16385, 20000, 32768, 32769])
+def test_every_number_of_waves(gpu, cols):
+    """Rows of one wave to sixteen, one to four chunks a lane, and beyond."""
+    g, rows = gen(cols), 6
+    x = torch.randn((rows, cols), device="cuda", generator=g).to(torch.bfloat16)
+    r = torch.randn((rows, cols), device="cuda", generator=g)
+    w = torch.randn(cols, device="cuda", generator=g)
+    s, y = torch.empty_like(r), torch.empty_like(r)
+    c, sc = room(None, cols, F8, rows)
+    norm(gpu, x, 30, cols, r, s, 0, cols, w, 0, 1e-6, rows, cols, y, 0, cols, F8, c, sc)
+    h = x.float() + r
+    assert torch.equal(s, h)
+    h = h.double()
+    want = h / torch.sqrt((h * h).mean(1, keepdim=True) + float(np.float32(1e-6))) * w.double()
+    assert ((y.double() - want).abs() <= 3.1 * 2.0 ** -24 * want.abs()).all()
+    wc, wsc = ref.quant(host(y))
+    assert np.array_equal(host(c), wc) and np.array_equal(host(sc), wsc)
