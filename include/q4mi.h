@@ -507,14 +507,14 @@ bool q4mi_f8_dequant(const uint8_t *d_codes, const float *d_scales, const int32_
  * matrix instruction, which of each aligned eight of products may lose what is
  * less than 2^-13 of the largest (1.5e-5 of y in the 2-norm on normal values).
  * Blocks are taken whole: codes past cols must be 0 in W or in x and not NaN in
- * either, as the quantiser leaves them. */
+ * either, as the quantiser leaves them.  cols <= 2^24, w_rows and n <= 2^30. */
 bool q4mi_f8_mul(const uint8_t *d_w, const float *d_ws, uint64_t w_rows, uint64_t cols,
                  const void *d_x, const float *d_xs, uint32_t x_type, uint64_t ld_x, uint64_t n,
                  void *d_y, uint32_t y_type, uint64_t ld_y);
 /* Routed experts of a decode step: row p < n (n <= 65535) is expert eid[p]
- * (codes at w + e*w_stride, scales at ws + e*ws_stride, both in bytes) times x
- * row p / x_div (x_div = topk: the token's hidden state; 1: a row each).  x as
- * for q4mi_f8_mul, any number of float rows.  A row whose eid is outside
+ * (codes at w + e*w_stride, scales at ws + e*ws_stride, both in bytes, multiples
+ * of 16 and 4) times x row p / x_div (x_div = topk: the token's hidden state; 1:
+ * a row each).  x as for q4mi_f8_mul, any number of float rows.  A row whose eid is outside
  * 0..n_expert-1 is left as it was.  eid is what q4mi_route_scored and
  * q4mi_moe_route write (ostride topk). */
 bool q4mi_f8_mul_sel(const uint8_t *d_w, const float *d_ws, uint64_t w_rows, uint64_t cols,
