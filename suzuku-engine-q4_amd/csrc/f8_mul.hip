@@ -36,16 +36,16 @@ struct F8Args {
     uint32_t m_tiles;               // tiles along the activations
 };
 
-// Four adjacent outputs, rounded once.  STREAM: around the caches, of large outputs.
-template <bool STREAM>
+// Four adjacent outputs, rounded once; AROUND: past the caches.
+template <bool AROUND>
 __device__ inline void store4(void *y, uint32_t yt, uint64_t at, v4f v) {
     if (yt == kTypeF32) {
         f32x4_a4 *p = (f32x4_a4 *)((float *)y + at);
-        STREAM ? __builtin_nontemporal_store((f32x4)v, p) : (void)(*p = (f32x4)v);
+        AROUND ? __builtin_nontemporal_store((f32x4)v, p) : (void)(*p = (f32x4)v);
     } else {
         const u32x2 q = {f32_to_16x2(v[0], v[1], yt), f32_to_16x2(v[2], v[3], yt)};
         u32x2_a2 *p = (u32x2_a2 *)((uint16_t *)y + at);
-        STREAM ? __builtin_nontemporal_store(q, p) : (void)(*p = q);
+        AROUND ? __builtin_nontemporal_store(q, p) : (void)(*p = q);
     }
 }
 
@@ -417,8 +417,10 @@ constexpr uint32_t tile_lds() { return (BM + BN) * S * 128 + BM * 2 * 32; }
 
 // Weight rows [r0, r0 + BN) of w against activation rows [p0, p0 + BM), of which
 // those below phi exist; the row read for p is act[p] with GATHER, else p.  Rows
-// past either end are read as the last one and not stored.
-template <uint32_t BM, uint32_t BN, uint32_t WM, uint32_t WN, uint32_t S, bool WIDE, bool GATHER>
+// past either end are read as the last one and not stored.  AROUND: outputs past the
+// caches.
+template <uint32_t BM, uint32_t BN, uint32_t WM, uint32_t WN, uint32_t S, bool WIDE, bool GATHER,
+          bool AROUND>
 __device__ inline void tile(const F8Args &a, const uint8_t *w, const float *ws, uint64_t r0,
                             uint64_t p0, uint64_t phi, uint8_t *lds) {
     constexpr uint32_t NW = WM * WN;
@@ -577,9 +579,6 @@ __device__ inline void tile(const F8Args &a, const uint8_t *w, const float *ws, 
     constexpr uint32_t kRow = FN * 16 + 4, kLanes = FN * 4;   // floats a row, lanes that store one
     static_assert(NW * 16 * kRow * 4 <= tile_lds<BM, BN, S>(), "sums fit the stages");
     static_assert(kLanes <= 64, "a row's stores");
-    // (8192 x 8192 x 2048, us: through the caches 150, around them 135; K = 8192 465 and
-    // 454; 2048 rows 122 and 113.  Small outputs stay for who reads them next.)
-    constexpr bool kStream = BM * BN >= 128 * 128 || (GATHER && BN >= 128);
     landed_barrier<0>();
     float *sums = (float *)lds + wave * 16 * kRow;
     const uint64_t rw = r0 + wn * FN * 16 + lane % kLanes * 4;   // weight row of this lane's stores
@@ -600,7 +599,7 @@ __device__ inline void tile(const F8Args &a, const uint8_t *w, const float *ws, 
             const uint64_t at = (p1 + t) * a.ldy + rw;
             if (p1 + t >= phi || !listed(p1 + t)) continue;
             if (rw + 4 <= a.w_rows)
-                store4<kStream>(a.y, a.y_type, at, v);
+                store4<AROUND>(a.y, a.y_type, at, v);
             else
                 for (uint32_t n = 0; n < 4; n++)
                     if (rw + n < a.w_rows) store_from_f32(a.y, a.y_type, at + n, v[n]);
@@ -614,7 +613,7 @@ __device__ inline void tile(const F8Args &a, const uint8_t *w, const float *ws, 
 // own: a die takes a contiguous run of tiles, in groups of kGroup activation
 // tiles, so that its L2 holds what its tiles share.
 constexpr uint32_t kGroup = 4;
-template <uint32_t BM, uint32_t BN, uint32_t WM, uint32_t WN, uint32_t S, bool WIDE>
+template <uint32_t BM, uint32_t BN, uint32_t WM, uint32_t WN, uint32_t S, bool WIDE, bool AROUND>
 __global__ __launch_bounds__(64 * WM * WN, 2) void f8_tile_k(F8Args a) {
     extern __shared__ __align__(16) uint8_t lds[];
     const uint32_t die = blockIdx.x & 7u, i = blockIdx.x >> 3;
@@ -624,7 +623,8 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void f8_tile_k(F8Args a) {
     const uint32_t group = t / (kGroup * n_tiles), in = t - group * kGroup * n_tiles;
     const uint32_t gm = min(kGroup, a.m_tiles - group * kGroup);
     const uint32_t mt = group * kGroup + in % gm, nt = in / gm;
-    tile<BM, BN, WM, WN, S, WIDE, false>(a, a.w, a.ws, (uint64_t)nt * BN, (uint64_t)mt * BM, a.n, lds);
+    tile<BM, BN, WM, WN, S, WIDE, false, AROUND>(a, a.w, a.ws, (uint64_t)nt * BN,
+                                                 (uint64_t)mt * BM, a.n, lds);
 }
 
 // ------------------------------------------------------------- packed rows
@@ -676,7 +676,7 @@ __device__ inline uint32_t owner(const T *ends, uint32_t n, uint32_t i) {
     return __builtin_amdgcn_readfirstlane(lo);
 }
 
-template <uint32_t ROWS, bool WIDE>
+template <uint32_t ROWS, bool WIDE, bool AROUND>
 __global__ __launch_bounds__(64 * IdSets<ROWS>::kWaves, 2) void f8_id_k(F8Args a) {
     extern __shared__ __align__(16) uint8_t lds[];
     typedef IdSets<ROWS> Sets;
@@ -751,14 +751,14 @@ __global__ __launch_bounds__(64 * IdSets<ROWS>::kWaves, 2) void f8_id_k(F8Args a
         const float *ws = (const float *)((const uint8_t *)a.ws + e * a.ws_stride);
         const uint64_t r0 = (uint64_t)part * ROWS, p0 = (uint64_t)(lo + skip), phi = p0 + rows;
         if (rows > kHalf) {
-            tile<ROWS, ROWS, 2, kWaves / 2, Sets::kAllS, WIDE, true>(a, w, ws, r0, p0, phi, work);
+            tile<ROWS, ROWS, 2, kWaves / 2, Sets::kAllS, WIDE, true, AROUND>(a, w, ws, r0, p0, phi, work);
         } else if (rows > kFew) {
             if constexpr (kHalf > 0)
-                tile<kHalf, ROWS, 2, kWaves / 2, Sets::kHalfS, WIDE, true>(a, w, ws, r0, p0, phi,
+                tile<kHalf, ROWS, 2, kWaves / 2, Sets::kHalfS, WIDE, true, AROUND>(a, w, ws, r0, p0, phi,
                                                                            work);
         } else {
             if constexpr (kFew > 0)
-                tile<kFew, ROWS, 2, kWaves / 2, Sets::kFewS, WIDE, true>(a, w, ws, r0, p0, phi, work);
+                tile<kFew, ROWS, 2, kWaves / 2, Sets::kFewS, WIDE, true, AROUND>(a, w, ws, r0, p0, phi, work);
         }
         __syncthreads();    // the next item overwrites what slower waves may still read
     }
@@ -863,11 +863,19 @@ bool few_launch(F8Args &a, uint32_t rows, uint32_t lists, uint32_t busy, size_t 
 // instruction, whose cut-off lies 2^-6 below their rounding.
 bool wide(const F8Args &a) { return a.y_type == kTypeF32; }
 
-template <uint32_t BM, uint32_t BN, uint32_t WM, uint32_t WN, uint32_t S, bool WIDE>
+// Large outputs go around the caches where rows begin at whole 64 bytes (8192 x 8192
+// x 2048, us: through the caches 150, around them 135; 8192 x 8192 x 8192 465 and 454;
+// 2048 rows of that 122 and 113; packed, 512 experts 234 and 224.  4266 x 54613 x
+// 128, rows at odd addresses: 156 and 252).  Small ones stay for who reads them next.
+bool around(const F8Args &a) {
+    return ((uintptr_t)a.y | a.ldy * type_bytes(a.y_type)) % 64 == 0;
+}
+
+template <uint32_t BM, uint32_t BN, uint32_t WM, uint32_t WN, uint32_t S, bool WIDE, bool AROUND>
 bool tile_launch(F8Args &a) {
     static DynLds st;
     constexpr size_t lds = tile_lds<BM, BN, S>();
-    auto k = f8_tile_k<BM, BN, WM, WN, S, WIDE>;
+    auto k = f8_tile_k<BM, BN, WM, WN, S, WIDE, AROUND>;
     if (!dyn_lds_ok((const void *)k, lds, lds, st, "f8_tile_k")) return false;
     const uint64_t m = (a.n + BM - 1) / BM, n = (a.w_rows + BN - 1) / BN;
     if (m * n > 0x7fffffu) {
@@ -879,10 +887,16 @@ bool tile_launch(F8Args &a) {
     return launch_ok("f8_tile_k");
 }
 
+template <uint32_t BM, uint32_t BN, uint32_t WM, uint32_t WN, uint32_t S, bool WIDE>
+bool tile_stores(F8Args &a) {
+    constexpr bool kLarge = BM * BN >= 128 * 128;
+    return kLarge && around(a) ? tile_launch<BM, BN, WM, WN, S, WIDE, kLarge>(a)
+                               : tile_launch<BM, BN, WM, WN, S, WIDE, false>(a);
+}
 template <uint32_t BM, uint32_t BN, uint32_t WM, uint32_t WN, uint32_t S>
 bool tile_pick(F8Args &a) {
-    return wide(a) ? tile_launch<BM, BN, WM, WN, S, true>(a)
-                   : tile_launch<BM, BN, WM, WN, S, false>(a);
+    return wide(a) ? tile_stores<BM, BN, WM, WN, S, true>(a)
+                   : tile_stores<BM, BN, WM, WN, S, false>(a);
 }
 
 // Which kernel a product takes.
@@ -914,22 +928,27 @@ bool mul_pick(F8Args &a) {
     if (tiles(128, 128) <= cus) return tile_pick<128, 128, 2, 2, 4>(a);
     if (a.n > 128 && tiles(256, 128) <= cus) return tile_pick<256, 128, 4, 2, 3>(a);
     if (a.n <= 128 || wide(a)) return tile_pick<128, 128, 2, 2, 2>(a);
-    return tile_launch<256, 256, 2, 4, 2, false>(a);
+    return tile_stores<256, 256, 2, 4, 2, false>(a);
 }
 
-template <uint32_t ROWS, bool WIDE>
+template <uint32_t ROWS, bool WIDE, bool AROUND>
 bool id_launch(F8Args &a) {
     constexpr size_t lds = IdSets<ROWS>::kLds;
     a.blocks = IdSets<ROWS>::kCu * (uint32_t)cu_count();
     static DynLds st;
-    auto k = f8_id_k<ROWS, WIDE>;
+    auto k = f8_id_k<ROWS, WIDE, AROUND>;
     if (!dyn_lds_ok((const void *)k, lds, lds, st, "f8_id_k")) return false;
     k<<<dim3(a.blocks), dim3(64 * IdSets<ROWS>::kWaves), lds, stream()>>>(a);
     return launch_ok("f8_id_k");
 }
+template <uint32_t ROWS, bool WIDE>
+bool id_stores(F8Args &a) {
+    constexpr bool kLarge = ROWS >= 128;
+    return kLarge && around(a) ? id_launch<ROWS, WIDE, kLarge>(a) : id_launch<ROWS, WIDE, false>(a);
+}
 template <uint32_t ROWS>
 bool id_wide(F8Args &a) {
-    return wide(a) ? id_launch<ROWS, true>(a) : id_launch<ROWS, false>(a);
+    return wide(a) ? id_stores<ROWS, true>(a) : id_stores<ROWS, false>(a);
 }
 
 // Small sets with deep rings where the chip has room for all at once: then a set's
@@ -947,7 +966,7 @@ bool id_pick(F8Args &a) {
     };
     if (sets(32) <= 2 * cus) return id_wide<32>(a);
     if (sets(64) <= cus) return id_wide<64>(a);
-    if (a.n >= 128ull * a.n_expert && sets(256) > cus && !wide(a)) return id_launch<256, false>(a);
+    if (a.n >= 128ull * a.n_expert && sets(256) > cus && !wide(a)) return id_stores<256, false>(a);
     return id_wide<128>(a);
 }
 

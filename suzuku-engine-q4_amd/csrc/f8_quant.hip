@@ -240,8 +240,9 @@ bool q4mi_f8_dequant(const uint8_t *d_codes, const float *d_scales, const int32_
     const dim3 grid = f8_grid(f32 ? 8 : 16, rows, cols, &group);
     // Outputs larger than the eight L2s together would only take the place of what
     // else is read (16384 x 4096 bf16, quantised and back: 79 us through the caches,
-    // 69.6 around them).
-    const bool large = rows * cols * type_bytes(y_type) > 32ull << 20;
+    // 69.6 around them); but parts of lines cost more there.
+    const bool large = rows * cols * type_bytes(y_type) > 32ull << 20 &&
+                       ((uintptr_t)d_y | ld_y * type_bytes(y_type)) % 64 == 0;
     auto k = f32 ? (large ? f8_dequant_k<4, true> : f8_dequant_k<4, false>)
                  : (large ? f8_dequant_k<8, true> : f8_dequant_k<8, false>);
     k<<<grid, dim3(256), 0, stream()>>>(d_codes, d_scales, d_ids, rows, group, (uint32_t)cols,

@@ -29,7 +29,8 @@ def tall(rng, rows, cols):
 
 # The sizes at which 64 x 64, 128 x 64, 128 x 128, 256 x 128 and the largest tiles
 # begin on a chip of 256 units, and more tiles than it has at once of up to 32, 64
-# and 128 rows; whole numbers, so that sums are exact.
+# and 128 rows; whole numbers, so that sums are exact.  Rows at odd addresses and at
+# whole lines.
 @pytest.mark.parametrize("yt", [0, 30])
 @pytest.mark.parametrize("n,rows", [(64, 8200), (130, 8100), (300, 8100), (520, 8100), (1100, 8100),
                                     (257, 16300), (17, 17000),
@@ -39,10 +40,12 @@ def test_mul_every_tile(gpu, n, rows, cols, yt):
     rng = np.random.default_rng(n + cols)
     w, times = tall(rng, rows, cols)
     x, xs, xv = random_rows(rng, n, cols, True, 1)
-    out = Output(n, rows, yt, rows + 1)
-    out.set(slice(None), times(xv), 0)
-    mul(gpu, w, rows, cols, dev(x), dev(xs), F8, 0, n, out.y, yt, out.ld)
-    out.check()
+    x, xs, want = dev(x), dev(xs), times(xv)
+    for ld in (rows + 1, -(-rows // 64) * 64):
+        out = Output(n, rows, yt, ld)
+        out.set(slice(None), want, 0)
+        mul(gpu, w, rows, cols, x, xs, F8, 0, n, out.y, yt, ld)
+        out.check()
 
 
 # Several rounds of weight tiles, K in parts, odd numbers of blocks, waves without
@@ -98,8 +101,9 @@ def test_sums_below_a_large_product(gpu, n, yt):
 
 
 # Stretches of each size a set can have, in sets of 32, 64, 128 and 256 rows (few of
-# them in all; rows an expert), more sets than workgroups, 1024 experts.
-@pytest.mark.parametrize("exact", [True, False])
+# them in all; rows an expert), more sets than workgroups, 1024 experts.  Rows at any
+# address and at whole lines.
+@pytest.mark.parametrize("exact,lines", [(True, False), (True, True), (False, False)])
 @pytest.mark.parametrize("counts,rows,cols,yt", [
     ([256, 1, 512, 64, 65, 128, 129, 300, 0, 257], 700, 900, 30),
     ([256, 1, 512, 64, 65, 128, 129, 300, 0, 257], 260, 900, 0),
@@ -108,7 +112,7 @@ def test_sums_below_a_large_product(gpu, n, yt):
     ([31, 95, 127, 0, 128, 200] * 15, 2050, 300, 30), ([700, 64, 65, 128, 129, 1, 256, 300], 6500, 300, 30),
     ([700, 64, 65, 128, 129, 1, 256, 300], 6500, 130, 0), ([33, 40, 32, 1, 70], 1030, 1100, 30),
     ([33, 40, 32, 1, 70], 1030, 1100, 0)])
-def test_id_every_set(gpu, counts, rows, cols, yt, exact):
+def test_id_every_set(gpu, counts, rows, cols, yt, exact, lines):
     rng = np.random.default_rng(rows + len(counts))
     E, total = len(counts), sum(counts)
     nb, rb = ref.blocks(cols), -(-rows // 128)
@@ -120,7 +124,7 @@ def test_id_every_set(gpu, counts, rows, cols, yt, exact):
     x, xs, xv = random_rows(rng, xrows, cols, exact, 1)
     act = rng.integers(0, xrows, total)
     bounds = np.concatenate([[0], np.cumsum(counts)])
-    out = Output(total, rows, yt, rows)
+    out = Output(total, rows, yt, -(-rows // 64) * 64 if lines else rows)
     for e in range(E):
         v, wv = xv[act[bounds[e]:bounds[e + 1]]], few[pick[e]][2]
         room = room_of(wv, v, cols, exact)
@@ -131,7 +135,7 @@ def test_id_every_set(gpu, counts, rows, cols, yt, exact):
     q4mi.check(gpu.q4mi_f8_mul_id(w.data_ptr(), ws.data_ptr(), rows, cols, rows * nb * 128,
                                   4 * rb * nb, E, d[0].data_ptr(), d[1].data_ptr(), xrows,
                                   d[2].data_ptr(), d[3].data_ptr(), total, out.y.data_ptr(), yt,
-                                  rows), "id")
+                                  out.ld), "id")
     out.check()
 
 
