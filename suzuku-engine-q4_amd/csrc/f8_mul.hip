@@ -954,11 +954,12 @@ bool id_wide(F8Args &a) {
 // Small sets with deep rings where the chip has room for all at once: then a set's
 // stages in a row are the time (8 experts of 1024 x 2048, 32 rows each, us: sets of
 // 32 rows 9.2, 64 11.4, 128 17.8; one of 2048 x 2048, 256 rows: 64 10.5, 128 35).
-// Sets of 256 rows from 128 rows an expert on, where they occupy the chip (128
-// experts of 1024 x 2048, 128 / 256 rows a set, us: 64 rows each 73 / 75, 128 rows
-// 99 / 91, 256 rows 156 / 136, 1024 rows 530 / 419; 8 experts of 2048 x 2048, 128
-// rows each, 96 sets at most: 24 / 37); fp32 sums on the bf16 instruction have no
-// registers for them.
+// Sets of 256 rows from 128 rows an expert on, where (half a set an expert left over)
+// they occupy half of the chip (128 experts of 1024 x 2048, 128 / 256 rows a set, us:
+// 64 rows each 73 / 75, 128 rows 99 / 91, 256 rows 156 / 136, 1024 rows 530 / 419; 26
+// experts of 925 x 5888, 360 rows each, 196 sets: 126 / 98; 8 experts of 2048 x 2048,
+// 128 rows each, 64 sets: 24 / 37); fp32 sums on the bf16 instruction have no registers
+// for them.
 bool id_pick(F8Args &a) {
     const uint64_t cus = cu_count();
     auto sets = [&](uint64_t rows) {    // at most
@@ -966,7 +967,8 @@ bool id_pick(F8Args &a) {
     };
     if (sets(32) <= 2 * cus) return id_wide<32>(a);
     if (sets(64) <= cus) return id_wide<64>(a);
-    if (a.n >= 128ull * a.n_expert && sets(256) > cus && !wide(a)) return id_stores<256, false>(a);
+    const uint64_t twice = (a.n / 128 + a.n_expert) * ((a.w_rows + 255) / 256);   // sets of 256
+    if (a.n >= 128ull * a.n_expert && twice > cus && !wide(a)) return id_stores<256, false>(a);
     return id_wide<128>(a);
 }
 
