@@ -1010,8 +1010,12 @@ bool q4mi_f8_mul_sel(const uint8_t *d_w, const float *d_ws, uint64_t w_rows, uin
         return false;
     }
     if (!n) return true;
+    // Groups from more rows on than a wave's tile holds and there are experts, or from 64
+    // on: before, two rows of one expert find its weights in a cache (1024 x 2048, picks
+    // even, us, alone / in groups: 10 of 128 7.7 / 8.5, 16 of 8 8.4 / 9.0, 32 of 8 12.2 /
+    // 10.8, 40 of 128 15.7 / 17.1, 128 of 64 42 / 33, 128 of 8 38 / 17.6).
     const uint32_t lists = (uint32_t)n;
-    if (4 * n < n_expert)
+    if (n <= kFewRows || (n < 64 && n <= n_expert))
         return few_launch<f8_sel_k<true, false>, f8_sel_k<false, false>>(a, 1, lists, lists, 0,
                                                                          "f8_sel_k");
     return few_launch<f8_sel_k<true, true>, f8_sel_k<false, true>>(

@@ -379,3 +379,25 @@ def test_dequant_large(gpu, yt, rows, cols, pad, block):
                                    y.data_ptr(), yt, cols + pad), "dequant")
     assert torch.equal(y[:, :cols], dev(v.astype(np.float32)).to(TYPES[yt]))
     assert (y[:, cols:] == 77).all()
+
+
+@pytest.mark.parametrize("n,E", [(16, 2), (17, 16), (17, 17), (63, 64), (64, 64), (64, 512), (90, 64),
+                                 (300, 40)])
+def test_sel_alone_and_in_groups(gpu, n, E):
+    """Rows each on its own and in groups of an expert's, also of one that most name."""
+    rng = np.random.default_rng(n + E)
+    rows, cols = 70, 300
+    w, ws, wst, sst, wv = experts(rng, E, rows, cols, True)
+    x, xs, xv = random_rows(rng, n, cols, True, 1)
+    for even in (True, False):
+        eid = rng.integers(0, E, n) if even else np.where(rng.random(n) < 0.8, E - 1, rng.integers(0, E, n))
+        eid[n // 2] = -1
+        out = Output(n, rows, 0, rows + 2)
+        for p in range(n):
+            if eid[p] >= 0:
+                out.set(p, xv[p] @ wv[eid[p]].T, 0)
+        d = [dev(a) for a in (x, xs, eid.astype(np.int32))]
+        q4mi.check(gpu.q4mi_f8_mul_sel(w.data_ptr(), ws.data_ptr(), rows, cols, wst, sst, E,
+                                       d[0].data_ptr(), d[1].data_ptr(), F8, 0, 1, d[2].data_ptr(),
+                                       n, out.y.data_ptr(), 0, out.ld), "sel")
+        out.check()
