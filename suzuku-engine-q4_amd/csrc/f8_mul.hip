@@ -531,7 +531,9 @@ __device__ inline void tile(const F8Args &a, const uint8_t *w, const float *ws, 
     // A stage begins with its weights and its first activations in registers.  The
     // barrier that says that the next stage has landed and this one is read stands
     // before the last activations' products, which cover the next stage's first
-    // reads.  Sums are added two products later.
+    // reads.  Sums are added two products later, copies go out three an activation
+    // fragment (8192 x 8192 x 8192, us: one to four products later 490, 473, 472, 483;
+    // two, three, four, eight copies 482, 473, 476, 484).
     auto stage = [&](uint32_t k, Frag<WIDE> *now, Frag<WIDE> *next) __attribute__((always_inline)) {
         const float s_next = wsp[min(k + 1, nb - 1)];
         constexpr uint32_t kPairs = FM * FN, kLag = 2;
@@ -611,7 +613,8 @@ __device__ inline void tile(const F8Args &a, const uint8_t *w, const float *ws, 
 // Tiles of a dense product, `a.blocks` of them, a.m_tiles along the
 // activations.  Workgroups go to the eight dies in turn, each with an L2 of its
 // own: a die takes a contiguous run of tiles, in groups of kGroup activation
-// tiles, so that its L2 holds what its tiles share.
+// tiles, so that its L2 holds what its tiles share (8192 x 8192 x 8192, us: groups of
+// four 467, eight 473, sixteen 485).
 constexpr uint32_t kGroup = 4;
 template <uint32_t BM, uint32_t BN, uint32_t WM, uint32_t WN, uint32_t S, bool WIDE, bool AROUND>
 __global__ __launch_bounds__(64 * WM * WN, 2) void f8_tile_k(F8Args a) {
