@@ -372,6 +372,10 @@ __global__ __launch_bounds__(64 * kFewWaves) void f8_sel_k(F8Args a) {
 // fragments of a stage, and the next stage's as it is read, over its activation
 // fragments one by one.
 //
+// Measured, codes to BF16: 8192 x 8192 x 8192 455 us (2.4 PFLOP/s; products and
+// additions alone, from registers, 394: power), 2048 rows of that 112 us, 512 rows 49
+// us, 32 rows 15 us (4.5 TB/s), 77 x 2560 x 2560 5.8 us.
+//
 // LDS places: chunk c (16 bytes) of row r at c ^ ((r >> 1) & 7), dword d of a
 // row's scales at d ^ ((r >> 3) & 7), so that a fragment's reads spread over all
 // 64 banks; the copies fill LDS in lane order, so the lanes permute their source
