@@ -50,6 +50,9 @@ int q4mi_grow_selftest(void);
  * sets them again; a failure is tried again), on the host alone; 1 = every
  * case behaves as documented. */
 int q4mi_per_device_selftest(void);
+/* The row of the weights' scales ([ceil(w_rows / 128)]) that a wave of the 8-bit
+ * tiles reads whose weight rows begin at r0 + first (host arithmetic alone). */
+uint64_t q4mi_f8_tile_scale_row(uint64_t w_rows, uint64_t r0, uint32_t first);
 
 #ifdef __cplusplus
 }

@@ -419,6 +419,13 @@ __device__ inline void landed_barrier() {
 template <uint32_t BM, uint32_t BN, uint32_t S>
 constexpr uint32_t tile_lds() { return (BM + BN) * S * 128 + BM * 2 * 32; }
 
+// The row of the weights' scales that a wave reads whose weight rows begin at r0 +
+// first: the last one where all of them are past the last row (a tile wider than 128
+// reaches there), as their codes are the last row's.
+__host__ __device__ inline uint64_t tile_scale_row(uint64_t w_rows, uint64_t r0, uint32_t first) {
+    return (r0 + first < w_rows ? r0 + first : w_rows - 1) / 128;
+}
+
 // Weight rows [r0, r0 + BN) of w against activation rows [p0, p0 + BM), of which
 // those below phi exist; the row read for p is act[p] with GATHER, else p.  Rows
 // past either end are read as the last one and not stored.  AROUND: outputs past the
@@ -502,7 +509,8 @@ __device__ inline void tile(const F8Args &a, const uint8_t *w, const float *ws, 
     const uint32_t lo = 16 * (g ^ tile_swz(m)), hi = lo ^ 64;
     // read by scalar loads: one of the compiler's vector loads would wait for every copy
     typedef const float __attribute__((address_space(4))) *Constant;
-    const Constant wsp = (Constant)(uintptr_t)(ws + (r0 + wn * FN * 16) / 128 * nb);
+    const Constant wsp =
+        (Constant)(uintptr_t)(ws + tile_scale_row(a.w_rows, r0, wn * FN * 16) * nb);
 
     v4f acc[FN][FM];
 #pragma unroll
@@ -1049,5 +1057,11 @@ bool q4mi_f8_mul_id(const uint8_t *d_w, const float *d_ws, uint64_t w_rows, uint
     if (!total_rows || !xrows) return true;
     return id_pick(a);
 }
+
+#ifdef Q4MI_MEASURE
+uint64_t q4mi_f8_tile_scale_row(uint64_t w_rows, uint64_t r0, uint32_t first) {
+    return tile_scale_row(w_rows, r0, first);
+}
+#endif
 
 }  // extern "C"
