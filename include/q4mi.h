@@ -503,11 +503,10 @@ bool q4mi_f8_dequant(const uint8_t *d_codes, const float *d_scales, const int32_
  * block, both scales and the sum over blocks in fp32, rounded once to y_type.
  * x_type 248: x and xs are codes and scales (ld_x unused).  x_type 0 / 1 / 30:
  * float rows, at most 16, quantised as by q4mi_f8_quant on the way in (the same
- * bits in y), xs NULL.  16-bit outputs of more than 16 rows come from the 8-bit
- * matrix instruction, which of each aligned eight of products may lose what is
- * less than 2^-13 of the largest (1.5e-5 of y in the 2-norm on normal values).
- * Blocks are taken whole: codes past cols must be 0 in W or in x and not NaN in
- * either, as the quantiser leaves them.  cols <= 2^24, w_rows and n <= 2^30. */
+ * bits in y), xs NULL.  A 16-bit y is the fp32 y of the same call, rounded; in
+ * which order a sum is added depends on the call's sizes.  Blocks are taken
+ * whole: codes past cols must be 0 in W or in x and not NaN in either, as the
+ * quantiser leaves them.  cols <= 2^24, w_rows and n <= 2^30. */
 bool q4mi_f8_mul(const uint8_t *d_w, const float *d_ws, uint64_t w_rows, uint64_t cols,
                  const void *d_x, const float *d_xs, uint32_t x_type, uint64_t ld_x, uint64_t n,
                  void *d_y, uint32_t y_type, uint64_t ld_y);
@@ -526,8 +525,7 @@ bool q4mi_f8_mul_sel(const uint8_t *d_w, const float *d_ws, uint64_t w_rows, uin
  * expert e, packed row p reading x row act_row ? act_row[p] : p (of xrows);
  * bounds (ascending) and act_row as q4mi_assign writes them; n_expert <= 1024.
  * Rows outside every stretch, past total_rows or with act_row outside
- * 0..xrows-1 are left as they were.  16-bit outputs as q4mi_f8_mul's of more
- * than 16 rows. */
+ * 0..xrows-1 are left as they were. */
 bool q4mi_f8_mul_id(const uint8_t *d_w, const float *d_ws, uint64_t w_rows, uint64_t cols,
                     uint64_t w_stride, uint64_t ws_stride, uint32_t n_expert, const uint8_t *d_xq,
                     const float *d_xs, uint64_t xrows, const int32_t *d_act_row,

@@ -7,8 +7,9 @@
 //
 // The 8-bit matrix instructions add eight neighbouring products with only 14 bits
 // below the largest of them (measured: a product 2^-14 of its neighbour is lost,
-// one in another eight only at 2^-24), which leaves y 1.5e-5 off (2-norm).  Codes
-// are exact in bf16, whose instruction adds in fp32 (1e-8 off) at half the rate.
+// one in another eight only at 2^-24): with large products that cancel nothing of
+// the others is left.  Codes are exact in bf16, whose instruction adds in fp32 (y 1e-8
+// off, 2-norm) at half the rate, so every sum here comes from that one.
 #include <algorithm>
 
 #include "f8.h"
@@ -18,7 +19,6 @@ using namespace q4mi;
 
 namespace {
 
-typedef int v8i __attribute__((ext_vector_type(8)));
 typedef float v4f __attribute__((ext_vector_type(4)));
 typedef __bf16 v8b __attribute__((ext_vector_type(8)));
 
@@ -63,34 +63,20 @@ __device__ inline v8b widen(uint32_t lo, uint32_t hi) {
 // A lane's part of a block of sixteen rows.  Which of the block's values that is
 // is free as long as both sides agree: lane (row, g) has bytes 16g .. and 64 +
 // 16g .. of its row, so that four lanes read 64 bytes.
-template <bool WIDE>
-struct Frag;
-template <>
-struct Frag<true> {
+struct Frag {
     v8b v[4];
     __device__ Frag() {}
     __device__ Frag(u32x4 a, u32x4 b)
         : v{widen(a.x, a.y), widen(a.z, a.w), widen(b.x, b.y), widen(b.z, b.w)} {}
 };
-template <>
-struct Frag<false> {
-    v8i v;
-    __device__ Frag() {}
-    __device__ Frag(u32x4 a, u32x4 b)
-        : v{(int)a.x, (int)a.y, (int)a.z, (int)a.w, (int)b.x, (int)b.y, (int)b.z, (int)b.w} {}
-};
 
 // Sixteen rows against sixteen over one block, from zero.
-__device__ inline v4f block_sums(const Frag<true> &w, const Frag<true> &x) {
+__device__ inline v4f block_sums(const Frag &w, const Frag &x) {
     v4f d = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int i = 0; i < 4; i++)
         d = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w.v[i], x.v[i], d, 0, 0, 0);
     return d;
-}
-__device__ inline v4f block_sums(const Frag<false> &w, const Frag<false> &x) {
-    const v4f zero = {0.f, 0.f, 0.f, 0.f};
-    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w.v, x.v, zero, 0, 0, 0, 0, 0, 0);
 }
 
 // acc += d * s, here: the compiler would rather keep every block's sums in
@@ -250,8 +236,8 @@ __device__ inline void few_rows(const F8Args &a, const uint8_t *w, const float *
             if (!FULL && h == 1 && sg * seg + 2 * c + 1 >= nb) break;
             const uint8_t *xp = codes + xc + 256u * c + 128u * h;
             const v4f d = block_sums(
-                Frag<true>(q.codes[2 * h], q.codes[2 * h + 1]),
-                Frag<true>(*(const u32x4 *)xp, *(const u32x4 *)(xp + 64)));
+                Frag(q.codes[2 * h], q.codes[2 * h + 1]),
+                Frag(*(const u32x4 *)xp, *(const u32x4 *)(xp + 64)));
             const float s = q.s[h] * xs[h];
 #pragma unroll
             for (int k = 0; k < 4; k++) acc[k] = fmaf(d[k], s, acc[k]);
@@ -372,9 +358,10 @@ __global__ __launch_bounds__(64 * kFewWaves) void f8_sel_k(F8Args a) {
 // fragments of a stage, and the next stage's as it is read, over its activation
 // fragments one by one.
 //
-// Measured, codes to BF16: 8192 x 8192 x 8192 455 us (2.4 PFLOP/s; products and
-// additions alone, from registers, 394: power), 2048 rows of that 112 us, 512 rows 49
-// us, 32 rows 15 us (4.5 TB/s), 77 x 2560 x 2560 5.8 us.
+// Measured, codes to BF16: 8192 x 8192 x 8192 938 us (1.17 PFLOP/s; a library's bf16
+// product 1.37), 2048 rows of that 238 us, 512 rows 78 us, 32 rows 22 us (3.1 TB/s),
+// 77 x 2560 x 2560 8.4 us.  The bf16 instruction's rate bounds it, and the widening ahead
+// of it: two codes an instruction, each by the two waves that read it.
 //
 // LDS places: chunk c (16 bytes) of row r at c ^ ((r >> 1) & 7), dword d of a
 // row's scales at d ^ ((r >> 3) & 7), so that a fragment's reads spread over all
@@ -420,8 +407,8 @@ template <uint32_t BM, uint32_t BN, uint32_t S>
 constexpr uint32_t tile_lds() { return (BM + BN) * S * 128 + BM * 2 * 32; }
 
 // The row of the weights' scales that a wave reads whose weight rows begin at r0 +
-// first: the last one where all of them are past the last row (a tile wider than 128
-// reaches there), as their codes are the last row's.
+// first: the last one where all of them are past the last row, as their codes are
+// the last row's.
 __host__ __device__ inline uint64_t tile_scale_row(uint64_t w_rows, uint64_t r0, uint32_t first) {
     return (r0 + first < w_rows ? r0 + first : w_rows - 1) / 128;
 }
@@ -430,8 +417,7 @@ __host__ __device__ inline uint64_t tile_scale_row(uint64_t w_rows, uint64_t r0,
 // those below phi exist; the row read for p is act[p] with GATHER, else p.  Rows
 // past either end are read as the last one and not stored.  AROUND: outputs past the
 // caches.
-template <uint32_t BM, uint32_t BN, uint32_t WM, uint32_t WN, uint32_t S, bool WIDE, bool GATHER,
-          bool AROUND>
+template <uint32_t BM, uint32_t BN, uint32_t WM, uint32_t WN, uint32_t S, bool GATHER, bool AROUND>
 __device__ inline void tile(const F8Args &a, const uint8_t *w, const float *ws, uint64_t r0,
                             uint64_t p0, uint64_t phi, uint8_t *lds) {
     constexpr uint32_t NW = WM * WN;
@@ -525,15 +511,15 @@ __device__ inline void tile(const F8Args &a, const uint8_t *w, const float *ws, 
 #pragma unroll
         for (uint32_t q = 0; q < RA + RB; q++) fetch(k, q);
     landed_barrier<kLeft>();
-    Frag<WIDE> wf[2][FN], xf[2];
+    Frag wf[2][FN], xf[2];
     float sx[2], s = wsp[0];
-    auto read_w = [&](uint32_t k, Frag<WIDE> *f, uint32_t j) __attribute__((always_inline)) {
+    auto read_w = [&](uint32_t k, Frag *f, uint32_t j) __attribute__((always_inline)) {
         const uint8_t *p = lds + kWeights + k % S * kW + rb * 128 + j * 2048;
-        f[j] = Frag<WIDE>(*(const u32x4 *)(p + lo), *(const u32x4 *)(p + hi));
+        f[j] = Frag(*(const u32x4 *)(p + lo), *(const u32x4 *)(p + hi));
     };
     auto read_x = [&](uint32_t k, uint32_t i) __attribute__((always_inline)) {
         const uint8_t *p = lds + k % S * kX + ra * 128 + i * 2048;
-        xf[i & 1u] = Frag<WIDE>(*(const u32x4 *)(p + lo), *(const u32x4 *)(p + hi));
+        xf[i & 1u] = Frag(*(const u32x4 *)(p + lo), *(const u32x4 *)(p + hi));
         const uint32_t d = 4 * ((k & 7u) ^ ((ra + 16 * i) >> 3 & 7u));
         sx[i & 1u] = *(const float *)(lds + kScales + (k >> 3 & 1u) * kWin + ra * 32 + i * 512 + d);
     };
@@ -543,14 +529,14 @@ __device__ inline void tile(const F8Args &a, const uint8_t *w, const float *ws, 
     // A stage begins with its weights and its first activations in registers.  The
     // barrier that says that the next stage has landed and this one is read stands
     // before the last activations' products, which cover the next stage's first
-    // reads.  Sums are added two products later, copies go out three an activation
-    // fragment (8192 x 8192 x 8192, us: one to four products later 490, 473, 472, 483;
-    // two, three, four, eight copies 482, 473, 476, 484).
-    auto stage = [&](uint32_t k, Frag<WIDE> *now, Frag<WIDE> *next) __attribute__((always_inline)) {
+    // reads.  Sums are added two products later, copies go out four an activation
+    // fragment (8192 x 8192 x 8192, us: one to four products later 972, 959, 961, 957;
+    // two, three, four, eight copies 960, 959, 938, 936).
+    auto stage = [&](uint32_t k, Frag *now, Frag *next) __attribute__((always_inline)) {
         const float s_next = wsp[min(k + 1, nb - 1)];
         constexpr uint32_t kPairs = FM * FN, kLag = 2;
         constexpr uint32_t kFirst = FM > 1 ? FM - 1 : 1;
-        constexpr uint32_t kNeed = (RA + RB + kFirst - 1) / kFirst, kEach = kNeed > 3 ? kNeed : 3;
+        constexpr uint32_t kNeed = (RA + RB + kFirst - 1) / kFirst, kEach = kNeed > 4 ? kNeed : 4;
         v4f d[kLag + 1];
         float ds[kLag + 1];
 #pragma unroll
@@ -626,9 +612,9 @@ __device__ inline void tile(const F8Args &a, const uint8_t *w, const float *ws, 
 // activations.  Workgroups go to the eight dies in turn, each with an L2 of its
 // own: a die takes a contiguous run of tiles, in groups of kGroup activation
 // tiles, so that its L2 holds what its tiles share (8192 x 8192 x 8192, us: groups of
-// four 467, eight 473, sixteen 485).
+// four 959, eight 965, sixteen 989).
 constexpr uint32_t kGroup = 4;
-template <uint32_t BM, uint32_t BN, uint32_t WM, uint32_t WN, uint32_t S, bool WIDE, bool AROUND>
+template <uint32_t BM, uint32_t BN, uint32_t WM, uint32_t WN, uint32_t S, bool AROUND>
 __global__ __launch_bounds__(64 * WM * WN, 2) void f8_tile_k(F8Args a) {
     extern __shared__ __align__(16) uint8_t lds[];
     const uint32_t die = blockIdx.x & 7u, i = blockIdx.x >> 3;
@@ -638,23 +624,21 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void f8_tile_k(F8Args a) {
     const uint32_t group = t / (kGroup * n_tiles), in = t - group * kGroup * n_tiles;
     const uint32_t gm = min(kGroup, a.m_tiles - group * kGroup);
     const uint32_t mt = group * kGroup + in % gm, nt = in / gm;
-    tile<BM, BN, WM, WN, S, WIDE, false, AROUND>(a, a.w, a.ws, (uint64_t)nt * BN,
-                                                 (uint64_t)mt * BM, a.n, lds);
+    tile<BM, BN, WM, WN, S, false, AROUND>(a, a.w, a.ws, (uint64_t)nt * BN, (uint64_t)mt * BM, a.n,
+                                           lds);
 }
 
 // ------------------------------------------------------------- packed rows
 //
 // Persistent workgroups go over the experts' sets of up to ROWS rows x ROWS weight
-// rows, each in the tile that its rows fill.  With 128, two a CU: mostly a few
-// rows, so that reading the weights bounds it, and one workgroup's first copies and
-// last stores are covered by the other's stages.  With 256, one a CU: many rows an
-// expert, so that a tile's two sides should be read as seldom as they can be.
+// rows, each in the tile that its rows fill.  With 128, two a CU, so that one
+// workgroup's first copies and last stores are covered by the other's stages.
 // Every workgroup makes the lists of sets by
 // itself, as prefix sums over the experts' stretches in LDS: no scratch in memory,
 // no launch before.  It takes every a.blocks-th of them, the large ones first, so
 // that all have as many of each size (512 experts of 1024 x 2048, 2048 tokens of
-// ten picks: 254 us, 280 in the experts' order, with Zipf's popularities, 235 and
-// 248 with equal ones; 4.4 and 4.8 TB/s).
+// ten picks: 284 us, 308 in the experts' order, with Zipf's popularities, 266 and
+// 280 with equal ones; 3.9 and 4.2 TB/s).
 constexpr uint32_t kIdExperts = 1024;
 // LDS: each expert's last set of more than half of ROWS, of less, of up to a quarter
 struct IdLists {
@@ -665,11 +649,11 @@ struct IdLists {
 // of the sets that have tiles of their own, stages of each, the largest tile's LDS.
 template <uint32_t ROWS>
 struct IdSets {
-    static constexpr uint32_t kWaves = ROWS == 256 ? 8 : 4;
-    static constexpr uint32_t kCu = ROWS == 32 || ROWS == 128 ? 2 : 1;
+    static constexpr uint32_t kWaves = 4;
+    static constexpr uint32_t kCu = ROWS == 64 ? 1 : 2;
     static constexpr uint32_t kHalf = ROWS == 32 ? 0 : ROWS / 2, kFew = ROWS < 128 ? 0 : ROWS / 4;
     static constexpr uint32_t kAllS = ROWS < 128 ? 8 : 2;
-    static constexpr uint32_t kHalfS = ROWS < 128 ? 8 : ROWS == 128 ? 2 : 3, kFewS = 3;
+    static constexpr uint32_t kHalfS = ROWS < 128 ? 8 : 2, kFewS = 3;
     static constexpr uint32_t kTiles =
         std::max({tile_lds<ROWS, ROWS, kAllS>(), tile_lds<kHalf, ROWS, kHalfS>(),
                   tile_lds<kFew, ROWS, kFewS>()});
@@ -691,7 +675,7 @@ __device__ inline uint32_t owner(const T *ends, uint32_t n, uint32_t i) {
     return __builtin_amdgcn_readfirstlane(lo);
 }
 
-template <uint32_t ROWS, bool WIDE, bool AROUND>
+template <uint32_t ROWS, bool AROUND>
 __global__ __launch_bounds__(64 * IdSets<ROWS>::kWaves, 2) void f8_id_k(F8Args a) {
     extern __shared__ __align__(16) uint8_t lds[];
     typedef IdSets<ROWS> Sets;
@@ -705,7 +689,7 @@ __global__ __launch_bounds__(64 * IdSets<ROWS>::kWaves, 2) void f8_id_k(F8Args a
         *lo = max(a.bounds[e], 0);
         return min((int64_t)a.bounds[e + 1], end) - *lo;
     };
-    // sums of the experts' sets: of more than 64 rows, and in one word the others
+    // sums of the experts' sets: of more than kHalf rows, and in one word the others
     constexpr uint32_t kEach = kIdExperts / (64 * kWaves);
     uint32_t most[kEach], less[kEach], m = 0, l = 0;
 #pragma unroll
@@ -766,14 +750,13 @@ __global__ __launch_bounds__(64 * IdSets<ROWS>::kWaves, 2) void f8_id_k(F8Args a
         const float *ws = (const float *)((const uint8_t *)a.ws + e * a.ws_stride);
         const uint64_t r0 = (uint64_t)part * ROWS, p0 = (uint64_t)(lo + skip), phi = p0 + rows;
         if (rows > kHalf) {
-            tile<ROWS, ROWS, 2, kWaves / 2, Sets::kAllS, WIDE, true, AROUND>(a, w, ws, r0, p0, phi, work);
+            tile<ROWS, ROWS, 2, kWaves / 2, Sets::kAllS, true, AROUND>(a, w, ws, r0, p0, phi, work);
         } else if (rows > kFew) {
             if constexpr (kHalf > 0)
-                tile<kHalf, ROWS, 2, kWaves / 2, Sets::kHalfS, WIDE, true, AROUND>(a, w, ws, r0, p0, phi,
-                                                                           work);
+                tile<kHalf, ROWS, 2, kWaves / 2, Sets::kHalfS, true, AROUND>(a, w, ws, r0, p0, phi, work);
         } else {
             if constexpr (kFew > 0)
-                tile<kFew, ROWS, 2, kWaves / 2, Sets::kFewS, WIDE, true, AROUND>(a, w, ws, r0, p0, phi, work);
+                tile<kFew, ROWS, 2, kWaves / 2, Sets::kFewS, true, AROUND>(a, w, ws, r0, p0, phi, work);
         }
         __syncthreads();    // the next item overwrites what slower waves may still read
     }
@@ -874,9 +857,6 @@ bool few_launch(F8Args &a, uint32_t rows, uint32_t lists, uint32_t busy, size_t 
     k<<<dim3(a.blocks, lists), dim3(64 * a.waves), lds, stream()>>>(a);
     return launch_ok(name);
 }
-// fp32 outputs are summed in fp32 throughout, 16-bit ones on the 8-bit matrix
-// instruction, whose cut-off lies 2^-6 below their rounding.
-bool wide(const F8Args &a) { return a.y_type == kTypeF32; }
 
 // Large outputs go around the caches where rows begin at whole 64 bytes (8192 x 8192
 // x 2048, us: through the caches 150, around them 135; 8192 x 8192 x 8192 465 and 454;
@@ -886,11 +866,11 @@ bool around(const F8Args &a) {
     return ((uintptr_t)a.y | a.ldy * type_bytes(a.y_type)) % 64 == 0;
 }
 
-template <uint32_t BM, uint32_t BN, uint32_t WM, uint32_t WN, uint32_t S, bool WIDE, bool AROUND>
+template <uint32_t BM, uint32_t BN, uint32_t WM, uint32_t WN, uint32_t S, bool AROUND>
 bool tile_launch(F8Args &a) {
     static DynLds st;
     constexpr size_t lds = tile_lds<BM, BN, S>();
-    auto k = f8_tile_k<BM, BN, WM, WN, S, WIDE, AROUND>;
+    auto k = f8_tile_k<BM, BN, WM, WN, S, AROUND>;
     if (!dyn_lds_ok((const void *)k, lds, lds, st, "f8_tile_k")) return false;
     const uint64_t m = (a.n + BM - 1) / BM, n = (a.w_rows + BN - 1) / BN;
     if (m * n > 0x7fffffu) {
@@ -902,32 +882,26 @@ bool tile_launch(F8Args &a) {
     return launch_ok("f8_tile_k");
 }
 
-template <uint32_t BM, uint32_t BN, uint32_t WM, uint32_t WN, uint32_t S, bool WIDE>
-bool tile_stores(F8Args &a) {
-    constexpr bool kLarge = BM * BN >= 128 * 128;
-    return kLarge && around(a) ? tile_launch<BM, BN, WM, WN, S, WIDE, kLarge>(a)
-                               : tile_launch<BM, BN, WM, WN, S, WIDE, false>(a);
-}
 template <uint32_t BM, uint32_t BN, uint32_t WM, uint32_t WN, uint32_t S>
 bool tile_pick(F8Args &a) {
-    return wide(a) ? tile_stores<BM, BN, WM, WN, S, true>(a)
-                   : tile_stores<BM, BN, WM, WN, S, false>(a);
+    constexpr bool kLarge = BM * BN >= 128 * 128;
+    return kLarge && around(a) ? tile_launch<BM, BN, WM, WN, S, kLarge>(a)
+                               : tile_launch<BM, BN, WM, WN, S, false>(a);
 }
 
 // Which kernel a product takes.
 //
 // While all its tiles are resident at once, the smallest of them, with as deep a
-// ring as LDS has room for: a CU takes in 43 to 56 KB/us that way, and a tile's time
-// is its bytes (8192 x 8192, us: 32 rows, 32 x 32 14.7, 64 x 64 23; 128 rows, 32 x 32
-// 31.4, 64 x 64 23.4, 128 x 64 34.9; 256 rows, 64 x 64 44, 128 x 64 35.2, 128 x 128
-// 48.5; 512 rows, 128 x 64 67.9, 128 x 128 48.9, 256 x 128 60; 1024 rows, 128 x 128
-// 95, 256 x 128 69.6, 256 x 256 101; 2048 rows, 256 x 128 140, 256 x 256 120).
+// ring as LDS has room for, so that every CU has a part (8192 x 8192, us: 64 rows, 32 x
+// 32 26, 64 x 64 37; 128 rows, 32 x 32 49, 64 x 64 37, 128 x 64 57; 256 rows, 64 x 64
+// 73, 128 x 64 58, 128 x 128 77; 512 rows, 128 x 64 113, 128 x 128 78, 256 x 128 108;
+// 1024 rows, 128 x 128 154, 256 x 128 117).
 //
 // More tiles: of up to 128 rows those that hold them all, two workgroups a CU, so
-// that the weights come once (151936 x 2048, us, that / 256 x 256: 32 rows 61.6 / 99,
-// 64 rows 67.8 / 102, 128 rows 82 / 109); else the largest, which read the sides
-// least often (fp32 outputs have no registers for them: 128 x 128 in two workgroups
-// a CU, 8192 x 8192 x 2048 277 us, 128 x 256 in one 285).
+// that the weights come once (151936 x 2048, us: 32 rows, 32 x 128 63, 32 x 32 84; 64
+// rows, 64 x 128 75, 64 x 64 120; 128 rows, 128 x 128 105, in one workgroup a CU 123);
+// else 128 x 128 as well (8192 x 8192 x 128, 2048, 8192: 49, 259, 960 us; 256 x 128 in
+// one workgroup a CU 55, 262, 952).
 bool mul_pick(F8Args &a) {
     const uint64_t cus = cu_count();
     auto tiles = [&](uint64_t bm, uint64_t bn) {
@@ -942,49 +916,37 @@ bool mul_pick(F8Args &a) {
     if (tiles(128, 64) <= cus) return tile_pick<128, 64, 2, 2, 6>(a);
     if (tiles(128, 128) <= cus) return tile_pick<128, 128, 2, 2, 4>(a);
     if (a.n > 128 && tiles(256, 128) <= cus) return tile_pick<256, 128, 4, 2, 3>(a);
-    if (a.n <= 128 || wide(a)) return tile_pick<128, 128, 2, 2, 2>(a);
-    return tile_stores<256, 256, 2, 4, 2, false>(a);
+    return tile_pick<128, 128, 2, 2, 2>(a);
 }
 
-template <uint32_t ROWS, bool WIDE, bool AROUND>
+template <uint32_t ROWS, bool AROUND>
 bool id_launch(F8Args &a) {
     constexpr size_t lds = IdSets<ROWS>::kLds;
     a.blocks = IdSets<ROWS>::kCu * (uint32_t)cu_count();
     static DynLds st;
-    auto k = f8_id_k<ROWS, WIDE, AROUND>;
+    auto k = f8_id_k<ROWS, AROUND>;
     if (!dyn_lds_ok((const void *)k, lds, lds, st, "f8_id_k")) return false;
     k<<<dim3(a.blocks), dim3(64 * IdSets<ROWS>::kWaves), lds, stream()>>>(a);
     return launch_ok("f8_id_k");
 }
-template <uint32_t ROWS, bool WIDE>
+template <uint32_t ROWS>
 bool id_stores(F8Args &a) {
     constexpr bool kLarge = ROWS >= 128;
-    return kLarge && around(a) ? id_launch<ROWS, WIDE, kLarge>(a) : id_launch<ROWS, WIDE, false>(a);
-}
-template <uint32_t ROWS>
-bool id_wide(F8Args &a) {
-    return wide(a) ? id_stores<ROWS, true>(a) : id_stores<ROWS, false>(a);
+    return kLarge && around(a) ? id_launch<ROWS, kLarge>(a) : id_launch<ROWS, false>(a);
 }
 
 // Small sets with deep rings where the chip has room for all at once: then a set's
 // stages in a row are the time (8 experts of 1024 x 2048, 32 rows each, us: sets of
-// 32 rows 9.2, 64 11.4, 128 17.8; one of 2048 x 2048, 256 rows: 64 10.5, 128 35).
-// Sets of 256 rows from 128 rows an expert on, where (half a set an expert left over)
-// they occupy half of the chip (128 experts of 1024 x 2048, 128 / 256 rows a set, us:
-// 64 rows each 73 / 75, 128 rows 99 / 91, 256 rows 156 / 136, 1024 rows 530 / 419; 26
-// experts of 925 x 5888, 360 rows each, 196 sets: 126 / 98; 8 experts of 2048 x 2048,
-// 128 rows each, 64 sets: 24 / 37); fp32 sums on the bf16 instruction have no registers
-// for them.
+// 32 rows 11.8, 64 15.1, 128 21.5; one of 2048 x 2048, 256 rows: 64 14.5, 128 26; 8 of
+// 2048 x 2048, 128 rows each: 64 36.8, 128 30.5).
 bool id_pick(F8Args &a) {
     const uint64_t cus = cu_count();
     auto sets = [&](uint64_t rows) {    // at most
         return (a.n / rows + std::min<uint64_t>(a.n, a.n_expert)) * ((a.w_rows + rows - 1) / rows);
     };
-    if (sets(32) <= 2 * cus) return id_wide<32>(a);
-    if (sets(64) <= cus) return id_wide<64>(a);
-    const uint64_t twice = (a.n / 128 + a.n_expert) * ((a.w_rows + 255) / 256);   // sets of 256
-    if (a.n >= 128ull * a.n_expert && twice > cus && !wide(a)) return id_stores<256, false>(a);
-    return id_wide<128>(a);
+    if (sets(32) <= 2 * cus) return id_stores<32>(a);
+    if (sets(64) <= cus) return id_stores<64>(a);
+    return id_stores<128>(a);
 }
 
 }  // namespace
