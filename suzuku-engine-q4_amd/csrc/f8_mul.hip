@@ -995,9 +995,10 @@ bool q4mi_f8_mul_sel(const uint8_t *d_w, const float *d_ws, uint64_t w_rows, uin
     if (n <= kFewRows || (n < 64 && n <= n_expert))
         return few_launch<f8_sel_k<true, false>, f8_sel_k<false, false>>(a, 1, lists, lists, 0,
                                                                          "f8_sel_k");
+    // sets with work, at most; any n_expert is taken
+    const uint64_t sets = std::min<uint64_t>(lists, (uint64_t)n_expert + lists / kFewRows);
     return few_launch<f8_sel_k<true, true>, f8_sel_k<false, true>>(
-        a, std::min(lists, kFewRows), lists, std::min(lists, n_expert + lists / kFewRows), kSelList,
-        "f8_sel_k");
+        a, std::min(lists, kFewRows), lists, (uint32_t)sets, kSelList, "f8_sel_k");
 }
 
 /* Packed rows, each expert's in one stretch (see include/q4mi.h). */
