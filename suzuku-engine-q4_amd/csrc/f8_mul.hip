@@ -873,7 +873,7 @@ bool tile_launch(F8Args &a) {
     auto k = f8_tile_k<BM, BN, WM, WN, S, AROUND>;
     if (!dyn_lds_ok((const void *)k, lds, lds, st, "f8_tile_k")) return false;
     const uint64_t m = (a.n + BM - 1) / BM, n = (a.w_rows + BN - 1) / BN;
-    if (m * n > 0x7fffffu) {
+    if (m * n >= (1ull << 32) / (64 * WM * WN)) {    // threads along x; no 288 GB hold more
         set_error("q4mi_f8_mul: too many tiles");
         return false;
     }
