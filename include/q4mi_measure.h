@@ -53,6 +53,9 @@ int q4mi_per_device_selftest(void);
 /* The row of the weights' scales ([ceil(w_rows / 128)]) that a wave of the 8-bit
  * tiles reads whose weight rows begin at r0 + first (host arithmetic alone). */
 uint64_t q4mi_f8_tile_scale_row(uint64_t w_rows, uint64_t r0, uint32_t first);
+/* Whether 8-bit products store such an output around the caches (host arithmetic
+ * alone). */
+bool q4mi_f8_around(void *d_y, uint32_t y_type, uint64_t ld_y, uint64_t n, uint64_t w_rows);
 
 #ifdef __cplusplus
 }

@@ -858,15 +858,20 @@ bool few_launch(F8Args &a, uint32_t rows, uint32_t lists, uint32_t busy, size_t 
     return launch_ok(name);
 }
 
-// Large outputs go around the caches where rows begin at whole 64 bytes (8192 x 8192
-// x 2048, us: through the caches 150, around them 135; 8192 x 8192 x 8192 465 and 454;
-// 2048 rows of that 122 and 113; packed, 512 experts 234 and 224.  4266 x 54613 x
-// 128, rows at odd addresses: 156 and 252).  Small ones stay for who reads them next.
+// Outputs of more than 128 MiB go around the caches where rows begin at whole 64
+// bytes: half of the last cache, so that who reads them next finds little there
+// (product, and with the quantiser that reads it, us, through / around: 8192 x 9216 x
+// 1024 bf16 177 / 181 and 210 / 211; 4096 x 54656 x 128 196 / 161 and 331 / 320; packed, 128
+// experts, 20480 x 2048 x 1024 fp32 170 / 153 and 204 / 196).  Smaller ones stay for the
+// reader, though the product alone would be shorter around them (2048 x 8192 x 1024
+// fp32 45 / 43 and 55 / 57; 4096 x 8192 x 1024 bf16 76 / 75 and 93 / 97).  Rows at odd
+// addresses would write parts of lines (4266 x 54613 x 128 210 / 247).
 bool around(const F8Args &a) {
-    return ((uintptr_t)a.y | a.ldy * type_bytes(a.y_type)) % 64 == 0;
+    return a.n * a.w_rows * type_bytes(a.y_type) > 128ull << 20 &&
+           ((uintptr_t)a.y | a.ldy * type_bytes(a.y_type)) % 64 == 0;
 }
 
-template <uint32_t BM, uint32_t BN, uint32_t WM, uint32_t WN, uint32_t S, bool AROUND>
+template <uint32_t BM, uint32_t BN, uint32_t WM, uint32_t WN, uint32_t S, bool AROUND = false>
 bool tile_launch(F8Args &a) {
     static DynLds st;
     constexpr size_t lds = tile_lds<BM, BN, S>();
@@ -880,13 +885,6 @@ bool tile_launch(F8Args &a) {
     a.m_tiles = (uint32_t)m, a.blocks = (uint32_t)(m * n);
     k<<<dim3(a.blocks), dim3(64 * WM * WN), lds, stream()>>>(a);
     return launch_ok("f8_tile_k");
-}
-
-template <uint32_t BM, uint32_t BN, uint32_t WM, uint32_t WN, uint32_t S>
-bool tile_pick(F8Args &a) {
-    constexpr bool kLarge = BM * BN >= 128 * 128;
-    return kLarge && around(a) ? tile_launch<BM, BN, WM, WN, S, kLarge>(a)
-                               : tile_launch<BM, BN, WM, WN, S, false>(a);
 }
 
 // Which kernel a product takes.
@@ -909,14 +907,14 @@ bool mul_pick(F8Args &a) {
     };
     if (a.n <= kFewRows)
         return few_launch<f8_few_k<true>, f8_few_k<false>>(a, (uint32_t)a.n, 1, 1, 0, "f8_few_k");
-    if (tiles(32, 32) <= 2 * cus) return tile_pick<32, 32, 2, 2, 8>(a);
-    if (a.n <= 32) return tile_pick<32, 128, 2, 2, 3>(a);
-    if (tiles(64, 64) <= cus) return tile_pick<64, 64, 2, 2, 8>(a);
-    if (a.n <= 64) return tile_pick<64, 128, 2, 2, 3>(a);
-    if (tiles(128, 64) <= cus) return tile_pick<128, 64, 2, 2, 6>(a);
-    if (tiles(128, 128) <= cus) return tile_pick<128, 128, 2, 2, 4>(a);
-    if (a.n > 128 && tiles(256, 128) <= cus) return tile_pick<256, 128, 4, 2, 3>(a);
-    return tile_pick<128, 128, 2, 2, 2>(a);
+    if (tiles(32, 32) <= 2 * cus) return tile_launch<32, 32, 2, 2, 8>(a);
+    if (a.n <= 32) return tile_launch<32, 128, 2, 2, 3>(a);
+    if (tiles(64, 64) <= cus) return tile_launch<64, 64, 2, 2, 8>(a);
+    if (a.n <= 64) return tile_launch<64, 128, 2, 2, 3>(a);
+    if (tiles(128, 64) <= cus) return tile_launch<128, 64, 2, 2, 6>(a);
+    if (tiles(128, 128) <= cus) return tile_launch<128, 128, 2, 2, 4>(a);
+    if (a.n > 128 && tiles(256, 128) <= cus) return tile_launch<256, 128, 4, 2, 3>(a);
+    return around(a) ? tile_launch<128, 128, 2, 2, 2, true>(a) : tile_launch<128, 128, 2, 2, 2>(a);
 }
 
 template <uint32_t ROWS, bool AROUND>
@@ -1024,6 +1022,11 @@ bool q4mi_f8_mul_id(const uint8_t *d_w, const float *d_ws, uint64_t w_rows, uint
 #ifdef Q4MI_MEASURE
 uint64_t q4mi_f8_tile_scale_row(uint64_t w_rows, uint64_t r0, uint32_t first) {
     return tile_scale_row(w_rows, r0, first);
+}
+bool q4mi_f8_around(void *d_y, uint32_t y_type, uint64_t ld_y, uint64_t n, uint64_t w_rows) {
+    F8Args a = {};
+    a.y = d_y, a.y_type = y_type, a.ldy = ld_y, a.n = n, a.w_rows = w_rows;
+    return around(a);
 }
 #endif
 

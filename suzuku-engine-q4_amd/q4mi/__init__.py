@@ -159,6 +159,7 @@ _MEAS_SIGS = {
     "q4mi_grow_selftest": (_c.c_int, []),
     "q4mi_per_device_selftest": (_c.c_int, []),
     "q4mi_f8_tile_scale_row": (_u64, [_u64, _u64, _u32]),
+    "q4mi_f8_around": (_b, [_vp, _u32, _u64, _u64, _u64]),
 }
 
 _lib = None
