@@ -102,7 +102,7 @@ __device__ inline void add_scaled(v4f &acc, v4f d, float s) {
 //
 // Measured, codes to BF16: one row through 151936 x 2048 58 us (5.4 TB/s), 8192 x
 // 8192 14.6 us (4.6 TB/s), 2560 x 2560 4.7 us (an empty launch: 2 us); sixteen rows
-// 66.5, 20.5 and 5.8 us.  What bounds the middle ones is how much a CU can have on
+// 66.3, 17.4 and 5.8 us.  What bounds the middle ones is how much a CU can have on
 // its way with loads to registers, 30 KB/us.
 constexpr uint32_t kFewRows = 16, kFewWaves = 8;     // at most
 
@@ -358,10 +358,12 @@ __global__ __launch_bounds__(64 * kFewWaves) void f8_sel_k(F8Args a) {
 // fragments of a stage, and the next stage's as it is read, over its activation
 // fragments one by one.
 //
-// Measured, codes to BF16: 8192 x 8192 x 8192 938 us (1.17 PFLOP/s; a library's bf16
-// product 1.37), 2048 rows of that 238 us, 512 rows 78 us, 32 rows 22 us (3.1 TB/s),
-// 77 x 2560 x 2560 8.4 us.  The bf16 instruction's rate bounds it, and the widening ahead
-// of it: two codes an instruction, each by the two waves that read it.
+// Measured, codes to BF16: 8192 x 8192 x 8192 935 to 1000 us (1.1 to 1.18 PFLOP/s, by
+// the card; a library's bf16 product 1.37), 2048 rows of that 239 to 262 us, 512 rows 78
+// us, 32 rows 22 us (3.1 TB/s), 77 x 2560 x 2560 8.4 us.  The bf16 instruction and the
+// widening ahead of it bound it: at 8192^3 the matrix units are busy 57 % of the time, and
+// 134 M of the 237 M other vector instructions convert two codes each, every code in
+// both waves that read it.
 //
 // LDS places: chunk c (16 bytes) of row r at c ^ ((r >> 1) & 7), dword d of a
 // row's scales at d ^ ((r >> 3) & 7), so that a fragment's reads spread over all
