@@ -501,12 +501,13 @@ bool q4mi_f8_dequant(const uint8_t *d_codes, const float *d_scales, const int32_
                      uint32_t y_type, uint64_t ld_y);
 /* y[t][r] = W_r . x_t for t < n, r < w_rows, both sides in 8 bits: sums of a
  * block, the product of both its scales (which should not overflow) and the sum
- * over blocks in fp32, rounded once to y_type.  x_type 248: x and xs are codes and scales (ld_x unused).  x_type 0 / 1 / 30:
- * float rows, at most 16, quantised as by q4mi_f8_quant on the way in (the same
- * bits in y), xs NULL.  A 16-bit y is the fp32 y of the same call, rounded; in
- * which order a sum is added depends on the call's sizes.  Blocks are taken
- * whole: codes past cols must be 0 in W or in x and not NaN in either, as the
- * quantiser leaves them.  cols <= 2^24, w_rows and n <= 2^30. */
+ * over blocks in fp32, rounded once to y_type.  x_type 248: x and xs are codes
+ * and scales (ld_x unused).  x_type 0 / 1 / 30: float rows, at most 16, quantised
+ * as by q4mi_f8_quant on the way in (the same bits in y), xs NULL.  A 16-bit y is
+ * the fp32 y of the same call, rounded; in which order a sum is added depends on
+ * the call's sizes.  Blocks are taken whole: codes past cols must be 0 in W or in
+ * x and not NaN in either, as the quantiser leaves them.  cols <= 2^24, w_rows and
+ * n <= 2^30. */
 bool q4mi_f8_mul(const uint8_t *d_w, const float *d_ws, uint64_t w_rows, uint64_t cols,
                  const void *d_x, const float *d_xs, uint32_t x_type, uint64_t ld_x, uint64_t n,
                  void *d_y, uint32_t y_type, uint64_t ld_y);
@@ -570,8 +571,9 @@ bool q4mi_rms_norm(const void *d_x, uint32_t x_type, uint64_t ld_x, const void *
  * stands after the picks that were found (weight d_sg[t], 1 without), d_nh
  * (optional) receives how many entries that makes, so that the device lists of
  * q4_hip_moe_exec_win / _dev end there.  n_exp <= 1024, topk <= 64 (above 62
- * several times slower), n_tok <= 2^24.  Keeps no state and no scratch; n_tok 0 succeeds.  The reference routes by softmax alone
- * (src/q4_quant.c:715-755: q4_hip_route_pf). */
+ * several times slower), n_tok <= 2^24.  Keeps no state and no scratch; n_tok 0
+ * succeeds.  The reference routes by softmax alone (src/q4_quant.c:715-755:
+ * q4_hip_route_pf). */
 bool q4mi_route_scored(const void *d_logits, uint32_t type, uint64_t ld, uint32_t n_tok,
                        uint32_t n_exp, const float *d_bias, uint32_t sigmoid, uint32_t n_group,
                        uint32_t topk_group, uint32_t group_top, uint32_t topk, bool renorm,
